@@ -443,6 +443,61 @@ int lbd_attention_decode_ws(const float *qkv, int H, int KV, int D, const float 
                             float *k_cache, float *v_cache, int cap, float *out, void *work,
                             size_t work_bytes, void *stream);
 
+/* ---- paged 8-bit key / value cache of several sequences (no lowbit.h counterpart: the
+ *      reference's cache is one float32 array per sequence, src/lowbit/model.py:264-297).
+ *      Positions live in pages of `page` tokens of a pool that sequences share; a block
+ *      (one page, one KV head) holds OCP E4M3 codes and one E8M0 exponent e,
+ *      value = code * 2^(e - 127); e = 255: the whole block is NaN. ---- */
+typedef struct {
+  uint8_t *k, *v;   /* codes [pages][KV][page][D], 16-byte aligned */
+  uint8_t *ke, *ve; /* exponents [pages][KV] */
+  int pages;        /* pages in the pool */
+  int page;         /* tokens a page: 16, 32, 64 or 128 */
+  int KV, D;        /* KV heads; head width 32, 64 or 128 */
+} lbd_kv8_pool;
+/* The sequences of a call, in device memory, so that a recorded graph replays with other
+ * values. Sequence b's new tokens are rows q_start[b] .. q_start[b + 1] - 1 of the row
+ * buffers (non-decreasing, rows of none are left as they are: idle places of a batch, rows
+ * behind the last sequence), at positions past[b], past[b] + 1, ..; past[b] < 0: no new
+ * tokens. Position x lives in page table[b][x / page], slot x % page. An entry outside
+ * [0, pages) is no page: its positions are not written and not attended to. At most max_new
+ * tokens of a sequence take part; positions of max_pages * page and above are not written. */
+typedef struct {
+  const int32_t *q_start; /* [B + 1] */
+  const int32_t *past;    /* [B] */
+  const int32_t *table;   /* [B][max_pages] */
+  int B, max_pages;
+  int max_new; /* most new tokens of one sequence */
+  int T;       /* rows of the row buffers */
+} lbd_kv8_batch;
+/* The new tokens' rows qkv [T, H + 2 KV heads of D] (row stride `stride` floats): + bias
+ * (NULL: none), rotary embedding of q and k at the token's position from cos/sin
+ * [max_pos, D/2] ("rotate_half", src/lowbit/model.py:201-210; positions past the tables
+ * reuse the last angle), q to q_out (row stride q_stride; may be qkv itself with the same
+ * stride, must not overlap it otherwise), k and v into the cache. A block's exponent is the
+ * smallest that holds its largest element (|x| <= 448 * 2^(e - 127)); where a new token
+ * needs a larger one than the block has, the earlier codes are rounded to the new unit. Slot
+ * 0 of a page begins it: whatever it held is gone. A token that is not finite makes its
+ * blocks NaN until the page is begun again. A page that is appended to must belong to one
+ * sequence of the call; full pages may be shared. Strides are multiples of 4; qkv, bias,
+ * the tables and q_out 16-byte aligned. H is a multiple of KV. */
+int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *qkv,
+                   int stride, const float *bias, int H, const float *cos_table,
+                   const float *sin_table, int max_pos, float *q_out, int q_stride,
+                   void *stream);
+/* out rows = softmax(q k^T / sqrt(D)) v of the new tokens' query heads (rotated rows q,
+ * H heads of D, row stride q_stride; float32 throughout) over their sequence's positions 0
+ * .. their own, which the cache must hold: lbd_kv8_append first. A row whose positions are
+ * on no page at all gets zeros. Rows of no sequence are left as they are. out must not
+ * overlap q. Strides multiples of 4, q and out 16-byte aligned. work:
+ * lbd_kv8_attention_work_bytes of the same arguments, 16-byte aligned (NULL where that is
+ * 0); it needs no clearing, and calls that share it must be ordered (one stream). */
+size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch,
+                                    int H);
+int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q,
+                      int q_stride, int H, float *out, int out_stride, void *work,
+                      size_t work_bytes, void *stream);
+
 /* ---- device plumbing for the ctypes layer and benchmarks ---- */
 int lb_dev_malloc(void **ptr, size_t bytes);
 int lb_dev_free(void *ptr);

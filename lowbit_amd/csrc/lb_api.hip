@@ -1515,3 +1515,78 @@ int lbd_copy_kernel(void *dst, const void *src, size_t bytes, void *stream) {
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------- paged 8-bit cache
+
+namespace {
+
+int kv8_args(const lbd_kv8_pool *p, const lbd_kv8_batch *b, int H, lbk::Kv8Args &a) {
+  if (!p || !b) return fail(LB_ERR_ARG, "null pointer");
+  int shift = 4;
+  while (shift < 7 && (1 << shift) != p->page) shift++;
+  if ((1 << shift) != p->page) return fail(LB_ERR_SHAPE, "pages hold 16, 32, 64 or 128 tokens");
+  if (p->pages <= 0 || p->KV <= 0 || H <= 0 || H % p->KV || (p->D != 32 && p->D != 64 && p->D != 128) || b->B <= 0 ||
+      b->max_pages <= 0 || b->max_new <= 0 || b->T <= 0)
+    return fail(LB_ERR_SHAPE, "bad shape");
+  if (H > 65535 || b->B > lbk::kKv8MaxRows || b->T > lbk::kKv8MaxRows ||
+      (long long)b->max_pages * p->page > lbk::kKv8MaxPos)
+    return fail(LB_ERR_SHAPE, "at most 65535 heads, 2^24 sequences and rows, 2^30 positions");
+  a = {p->k, p->v, p->ke, p->ve, p->pages, shift, p->KV, b->q_start, b->past, b->table, b->B, b->max_pages,
+       std::min(b->max_new, b->T), b->T};
+  return 0;
+}
+
+int kv8_pointers(const lbk::Kv8Args &a) {
+  if (!a.k || !a.v || !a.ke || !a.ve || !a.q_start || !a.past || !a.table) return fail(LB_ERR_ARG, "null pointer");
+  if (!aligned16(a.k) || !aligned16(a.v)) return fail(LB_ERR_ARG, "the pool's codes must be 16-byte aligned");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *qkv, int stride,
+                   const float *bias, int H, const float *cos_table, const float *sin_table, int max_pos,
+                   float *q_out, int q_stride, void *stream) {
+  lbk::Kv8Args a;
+  int rc = kv8_args(pool, batch, H, a);
+  if (rc < 0) return rc;
+  if (max_pos <= 0 || stride % 4 || q_stride % 4 || stride < (long long)(H + 2 * pool->KV) * pool->D ||
+      q_stride < (long long)H * pool->D)
+    return fail(LB_ERR_SHAPE, "bad shape: strides are multiples of 4 floats that hold a row");
+  if (!qkv || !cos_table || !sin_table || !q_out) return fail(LB_ERR_ARG, "null pointer");
+  if ((rc = kv8_pointers(a)) < 0) return rc;
+  if (!aligned16(qkv) || !aligned16(cos_table) || !aligned16(sin_table) || !aligned16(q_out) ||
+      (bias && !aligned16(bias)))
+    return fail(LB_ERR_ARG, "qkv, bias, the tables and q_out must be 16-byte aligned");
+  if (q_out == qkv && q_stride != stride) return fail(LB_ERR_ARG, "q_out on qkv takes the same stride");
+  LB_LAUNCH(lbk::launch_kv8_append(a, pool->D, qkv, stride, bias, H, cos_table, sin_table, max_pos, q_out, q_stride,
+                                   static_cast<hipStream_t>(stream)),
+            "kv8 append launch");
+}
+
+size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, int H) {
+  lbk::Kv8Args a;
+  return kv8_args(pool, batch, H, a) < 0 ? 0 : lbk::kv8_attention_work_bytes(a, pool->D, H);
+}
+
+int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q, int q_stride, int H,
+                      float *out, int out_stride, void *work, size_t work_bytes, void *stream) {
+  lbk::Kv8Args a;
+  int rc = kv8_args(pool, batch, H, a);
+  if (rc < 0) return rc;
+  if (q_stride % 4 || out_stride % 4 || q_stride < (long long)H * pool->D || out_stride < (long long)H * pool->D)
+    return fail(LB_ERR_SHAPE, "bad shape: strides are multiples of 4 floats that hold a row");
+  if (!q || !out) return fail(LB_ERR_ARG, "null pointer");
+  if ((rc = kv8_pointers(a)) < 0) return rc;
+  if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ARG, "q and out must be 16-byte aligned");
+  const size_t need = lbk::kv8_attention_work_bytes(a, pool->D, H);
+  if (need && (!work || work_bytes < need)) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
+  if (need && !aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
+  LB_LAUNCH(lbk::launch_kv8_attention(a, pool->D, q, q_stride, H, out, out_stride, work,
+                                      static_cast<hipStream_t>(stream)),
+            "kv8 attention launch");
+}
+
+}  // extern "C"

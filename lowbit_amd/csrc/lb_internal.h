@@ -259,4 +259,22 @@ hipError_t launch_attention_slices(const float *qkv, int H, int KV, int D, const
 hipError_t launch_attention_merge(const float *part, int H, int D, const int32_t *pos, int cap, float *out,
                                   hipStream_t s);
 
+// The paged 8-bit cache (lb_kv8.hip): lbd_kv8_pool and lbd_kv8_batch as the kernels take
+// them. Pages and positions are counted in 32 bits (max_pages page <= kKv8MaxPos), bytes of
+// the pool in 64.
+constexpr int kKv8MaxPos = 1 << 30;
+constexpr int kKv8MaxRows = 1 << 24;
+struct Kv8Args {
+  uint8_t *k, *v, *ke, *ve;
+  int pages, page_shift, KV;  // page = 1 << page_shift tokens
+  const int32_t *q_start, *past, *table;
+  int B, max_pages, max_new, T;
+};
+hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stride, const float *bias, int H,
+                             const float *cosT, const float *sinT, int max_pos, float *q_out, int q_stride,
+                             hipStream_t s);
+size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H);
+hipError_t launch_kv8_attention(const Kv8Args &a, int D, const float *q, int q_stride, int H, float *out,
+                                int out_stride, void *work, hipStream_t s);
+
 }  // namespace lbk

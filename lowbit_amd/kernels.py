@@ -173,6 +173,9 @@ SIGNATURES = {
     "lbd_attention_merge": ([_vp, _sz, _int, _int, _vp, _int, _vp, _vp], _int),
     "lbd_gemm_w4a16_g32": ([_vp, _int, _int, _vp, _vp, _vp, _int, _vp, _vp], _int),
     "lbd_gemm_w4a8_g32": ([_vp, _int, _int, _vp, _vp, _vp, _int, _vp, _vp], _int),
+    "lbd_kv8_append": ([_vp, _vp, _vp, _int, _vp, _int, _vp, _vp, _int, _vp, _int, _vp], _int),
+    "lbd_kv8_attention_work_bytes": ([_vp, _vp, _int], _sz),
+    "lbd_kv8_attention": ([_vp, _vp, _vp, _int, _int, _vp, _int, _vp, _sz, _vp], _int),
     "lbd_quantize_int4_g32": ([_vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
 }
 
@@ -209,6 +212,18 @@ class LbdFusion(C.Structure):
     _fields_ = [("norm_w", C.c_void_p), ("norm_eps", C.c_float), ("swiglu", C.c_int),
                 ("bias", C.c_void_p), ("residual", C.c_void_p), ("argmax_key", C.c_void_p),
                 ("glu", C.c_int), ("attn_part", C.c_void_p), ("attn_cap", C.c_int), ("attn_head_dim", C.c_int)]
+
+
+class LbdKv8Pool(C.Structure):
+    """lbd_kv8_pool of include/lowbit_hip.h: the pages of a paged 8-bit cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ke", C.c_void_p), ("ve", C.c_void_p), ("pages", C.c_int),
+                ("page", C.c_int), ("KV", C.c_int), ("D", C.c_int)]
+
+
+class LbdKv8Batch(C.Structure):
+    """lbd_kv8_batch of include/lowbit_hip.h: the sequences of a call on such a cache."""
+    _fields_ = [("q_start", C.c_void_p), ("past", C.c_void_p), ("table", C.c_void_p), ("B", C.c_int),
+                ("max_pages", C.c_int), ("max_new", C.c_int), ("T", C.c_int)]
 
 
 @lru_cache(maxsize=1)
