@@ -1529,8 +1529,8 @@ int kv8_args(const lbd_kv8_pool *p, const lbd_kv8_batch *b, int H, lbk::Kv8Args 
       b->max_pages <= 0 || b->max_new <= 0 || b->T <= 0)
     return fail(LB_ERR_SHAPE, "bad shape");
   if (H > 65535 || b->B > lbk::kKv8MaxRows || b->T > lbk::kKv8MaxRows ||
-      (long long)b->max_pages * p->page > lbk::kKv8MaxPos)
-    return fail(LB_ERR_SHAPE, "at most 65535 heads, 2^24 sequences and rows, 2^30 positions");
+      (long long)b->T * H > (1 << 30) || (long long)b->max_pages * p->page > lbk::kKv8MaxPos)
+    return fail(LB_ERR_SHAPE, "at most 65535 heads, 2^24 sequences and rows, 2^30 rows of heads and positions");
   a = {p->k, p->v, p->ke, p->ve, p->pages, shift, p->KV, b->q_start, b->past, b->table, b->B, b->max_pages,
        std::min(b->max_new, b->T), b->T};
   return 0;

@@ -66,22 +66,30 @@ __device__ __forceinline__ Kv8Seq kv8_lane(const Kv8Seq &s, int lane) {
 }
 
 // Unit u of the batch's units (sequence b has units(its Kv8Seq) of them, in order): its
-// sequence in s and its index there in `at`. False past the last. By the whole wave: 64
-// sequences a step, one round trip of loads each.
-template <class F>
-__device__ __forceinline__ bool kv8_locate(const Kv8Args &a, int u, F units, Kv8Seq &s, int &at) {
+// sequence in s, its index there in `at` and, where asked, the sum of weight(..) over the
+// sequences before it. False past the last. By the whole wave: 64 sequences a step, one round
+// trip of loads each.
+struct Kv8None {
+  __device__ int operator()(const Kv8Seq &) const { return 0; }
+};
+template <class F, class W = Kv8None>
+__device__ __forceinline__ bool kv8_locate(const Kv8Args &a, int u, F units, Kv8Seq &s, int &at, W weight = W(),
+                                           int *before = nullptr) {
   const int lane = threadIdx.x & (kWave - 1);
-  int base = 0;
+  int base = 0, sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const Kv8Seq q = kv8_seq(a, b0 + lane);
     const int c = units(q), inc = wave_scan(c), all = __builtin_amdgcn_readlane(inc, 63);
+    const int wt = before ? weight(q) : 0, winc = before ? wave_scan(wt) : 0;
     if (u < base + all) {
       const int l = __ffsll((unsigned long long)__ballot(u - base < inc)) - 1;
       s = kv8_lane(q, l);
       at = u - base - __builtin_amdgcn_readlane(inc - c, l);
+      if (before) *before = sum + __builtin_amdgcn_readlane(winc - wt, l);
       return true;
     }
     base += all;
+    if (before) sum += __builtin_amdgcn_readlane(winc, 63);
   }
   return false;
 }
@@ -249,18 +257,519 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 }
 
 // ---------------------------------------------------------------- attention
+//
+// A sequence's query rows of one KV head are its new tokens' G = H / KV heads, row
+// r = token G + head, cut into row blocks of R; a row block's keys are cut into slices, each
+// one workgroup's. Slices that share a row block leave partial sums that a second launch adds.
+//
+// Scores are kept in base 2: x = q k log2(e) / sqrt(D). A block's V exponent ev joins the
+// exponential: a row's reference m is the largest x + ev so far, rounded up to a whole number
+// (so rescaling by 2^(m - m') is exact), and its weights w = 2^(x + ev - m) <= 1 multiply V's
+// codes as they are, so that what a row sees of V decides its precision, however far apart the
+// blocks' exponents are. The denominator is sum w 2^(mid - ev), in the unit 2^(m - mid), with
+// mid 50 below the slice's largest ev: every factor stays within 2^+-50. Blocks of V more than
+// 2^100 below the largest (blocks of zeros among them) count as zeros.
+//
+// The matrix products run on float16: an E4M3 code is exact there, q and w are taken as two
+// terms each (hi + lo: 22 bits; q relative to its row's largest element, w times 2^14, so that
+// the subnormals that the matrix cores flush lie 2^-28 below).
+
+constexpr float kKv8WUp = 14.0f;   // weights are scaled by 2^14
+constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
+constexpr float kKv8Log2e = 1.4426950408889634f;
+
+// How a launch cuts its rows and keys: the sequences of rows_min .. rows_max rows a KV head,
+// row blocks of R rows, about `slots` slices a KV head of at least min_keys keys.
+struct Kv8Cut {
+  int G, R, rows_min, rows_max, slots, min_keys;
+};
+
+__device__ __forceinline__ int kv8_row_blocks(const Kv8Cut &c, const Kv8Seq &s) {
+  const long long rows = (long long)s.n * c.G;
+  return rows >= c.rows_min && rows <= c.rows_max ? (int)((rows + c.R - 1) / c.R) : 0;
+}
+__device__ __forceinline__ int kv8_keys(const Kv8Args &a, const Kv8Seq &s) {
+  return min(s.past + s.n, a.max_pages << a.page_shift);
+}
+
+__device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+// Keys a slice: the batch's row blocks times keys over the slots, so that however the lengths
+// differ the slices are alike, in steps of 256. (The sum in float, 1 % up: never more slices
+// than slots and row blocks together.)
+__device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c) {
+  float sum = 0.0f;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const Kv8Seq s = kv8_seq(a, b0 + (int)(threadIdx.x & (kWave - 1)));
+    sum += (float)kv8_row_blocks(c, s) * (float)kv8_keys(a, s);
+  }
+  const float per = fminf(wave_sum(sum) * 1.01f / (float)c.slots, (float)kKv8MaxPos);
+  return max(c.min_keys, round_up((int)per + 1, 256));
+}
+
+// Row block and slice of unit u.
+struct Kv8Unit {
+  Kv8Seq s;
+  int rb, slice, slices, slice_keys;
+};
+__device__ __forceinline__ bool kv8_unit(const Kv8Args &a, const Kv8Cut &c, int u, Kv8Unit &w) {
+  w.slice_keys = kv8_slice_keys(a, c);
+  const auto slices = [&](const Kv8Seq &s) { return (kv8_keys(a, s) + w.slice_keys - 1) / w.slice_keys; };
+  int at;
+  if (!kv8_locate(a, u, [&](const Kv8Seq &s) { return kv8_row_blocks(c, s) * slices(s); }, w.s, at)) return false;
+  w.slices = slices(w.s);
+  w.rb = at / w.slices;
+  w.slice = at - w.rb * w.slices;
+  return true;
+}
+
+__device__ __forceinline__ v8h e4m3x8_h(uint32_t lo, uint32_t hi) {
+  const h2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  const h2v b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  const h2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  const h2v d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return v8h{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+__device__ __forceinline__ h2v pk_half(float a, float b) {  // toward zero: lo keeps what is left
+  return __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// The other term's share of x: x - hi (exact).
+__device__ __forceinline__ float half_rest(float x, _Float16 hi) { return x - (float)hi; }
+
+// 2^(13 - exponent of a row's largest |q|), which brings it into [2^13, 2^14), and the inverse;
+// NaN where the row is not finite.
+__device__ __forceinline__ void kv8_q_scale(int big, float &up, float &down) {
+  const int e = min(267 - (big >> 23), 253);
+  up = big >= 0x7F800000 ? __builtin_nanf("") : __int_as_float(e << 23);
+  down = __int_as_float((254 - e) << 23);
+}
+
+// Sum (or larger) of a value over the four lanes c, c + 16, c + 32, c + 48.
+__device__ __forceinline__ float quarters_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float quarters_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+
+// The unit 2^(m - mid) of a denominator. m may be too large for m - mid to keep mid, so units
+// are compared by it but differences are taken of m and mid apart.
+struct Kv8Unit2 {
+  float m, mid;
+};
+__device__ __forceinline__ Kv8Unit2 kv8_larger(Kv8Unit2 a, Kv8Unit2 b) { return b.m - b.mid > a.m - a.mid ? b : a; }
+
+// A tile of 16 keys as a wave holds it: page 0 stands in where there is none.
+struct Kv8Tile {
+  size_t at;       // first code row
+  bool held;       // some of its keys count
+  float kscale;    // 2^ke of K
+  float ev;        // V's exponent
+};
+
+// Few query rows a sequence (steps): R = 8 rows a block, or 16 (SEP). NW waves share a slice
+// in chunks of 32 keys, two 16-key tiles, each wave with its own running reference and sums,
+// merged in LDS. Everything is transposed, scores^T = K Q^T and out^T = V^T W^T, so a lane
+// keeps one query row (lane % 16) and what it gets from the first product (keys 4 (lane / 16)
+// + r of either tile) is the operand of the second as it is. R = 8: columns 8..15 hold the lo
+// terms of the rows in 0..7, one matrix instruction for both, and a row rotation by 8 adds
+// them; SEP: hi and lo one after the other.
+// K is read 16 bytes a lane (8 at D = 32), V D / 16 bytes a lane of eight keys: a lane's bytes
+// of two keys are interleaved by v_perm on their way to float16, which is all the transposing
+// that V needs, and its output elements come out contiguous. The next chunk's K is requested
+// once the scores are made, its V once the outputs are: loads are always in flight, and no
+// LDS lies between them and the matrix cores.
+template <int D, bool SEP, int NW>
+__global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
+                                                               int H, float *__restrict__ out, int out_stride,
+                                                               float *__restrict__ part, Kv8Cut cut) {
+  constexpr int R = SEP ? 16 : 8, KS = D / 32, CK = 32;
+  constexpr int KB = D >= 64 ? 16 : 8, KL = D / (4 * KB);  // bytes of a K load, loads per lane and tile
+  constexpr int VB = D / 16, VW = VB > 4 ? 2 : 1;           // bytes of a V load (a key's), words of it
+  constexpr int PS = D + 4;
+  __shared__ float sh[NW][R][PS];
+  __shared__ float sm[NW][R], sl[NW][R], smid[NW];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c = lane & 15, g = lane >> 4, row_c = SEP ? c : c & 7;
+  const int kv = (int)blockIdx.x % a.KV, unit = (int)blockIdx.x / a.KV;
+  Kv8Unit w;
+  if (!kv8_unit(a, cut, unit, w)) return;
+  const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
+  // this lane's query row, and the keys that it and the block's last row see
+  const int r = w.rb * R + row_c, tok = min(r, rows - 1) / G, head = kv * G + min(r, rows - 1) - tok * G;
+  const int lim = r < rows ? min(w.s.past + tok + 1, cap) : 0;
+  const int tok_last = (min(w.rb * R + R, rows) - 1) / G, tok_first = w.rb * R / G;
+  const int k_begin = w.slice * w.slice_keys;
+  const int k_end = min(min(w.s.past + tok_last + 1, cap), k_begin + w.slice_keys);
+  const int k_full = min(w.s.past + tok_first + 1, cap);  // keys below: every row sees them
+  const int chunks = max(0, (k_end - k_begin - CK * wave + CK * NW - 1) / (CK * NW));
+  const int32_t *table = a.table + (size_t)w.s.b * a.max_pages;
+
+  // ---- tiles of the wave's next 32 chunks, one a lane; `biggest`: their largest V exponent
+  int t_page = 0, t_ke = 0, t_ve = 0;
+  const auto tile_key = [&](int i) { return k_begin + CK * (wave + NW * (i >> 1)) + 16 * (i & 1); };
+  const auto load_tiles = [&](int i0) {
+    const int key = tile_key(i0 + lane);
+    const int pg = key < k_end ? table[key >> a.page_shift] : -1;
+    const bool in = (unsigned)pg < (unsigned)a.pages;
+    const size_t block = (size_t)(in ? pg : 0) * a.KV + kv;
+    t_page = in ? pg : -1;
+    t_ke = a.ke[block];
+    t_ve = in ? a.ve[block] : -1;
+    return wave_max_i32(t_ve == 255 ? -1 : t_ve);
+  };
+  const float *qr = q + (size_t)(w.s.row0 + tok) * q_stride + head * D;
+  v8h qh[KS], ql[SEP ? KS : 1];
+  float4 qf[KS][2];
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    const int d = D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    qf[s][0] = *reinterpret_cast<const float4 *>(qr + d);
+    qf[s][1] = *reinterpret_cast<const float4 *>(qr + d + 4);
+  }
+  int biggest = load_tiles(0);
+  for (int i = kWave; i < 2 * chunks; i += kWave) biggest = max(biggest, load_tiles(i));
+  if (2 * chunks > kWave) load_tiles(0);
+  const int least = max(biggest - kKv8Spread, 0);  // E8M0 exponents of V below count as zeros
+  const float mid = (float)(max(biggest, 0) - kKv8Spread / 2 - 127);
+
+  // ---- the query row in two terms
+  int big = 0;
+#pragma unroll
+  for (int s = 0; s < KS; s++) big = max(big, max(abs_bits(qf[s][0]), abs_bits(qf[s][1])));
+  big = max(big, __shfl_xor(big, 16));
+  big = max(big, __shfl_xor(big, 32));
+  float up, down;
+  kv8_q_scale(big, up, down);
+  const float cx = down * (kKv8Log2e / sqrtf((float)D));
+#pragma unroll
+  for (int s = 0; s < KS; s++) {
+    const float x[8] = {qf[s][0].x * up, qf[s][0].y * up, qf[s][0].z * up, qf[s][0].w * up,
+                        qf[s][1].x * up, qf[s][1].y * up, qf[s][1].z * up, qf[s][1].w * up};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const _Float16 hi = (_Float16)x[e], lo = (_Float16)half_rest(x[e], hi);
+      if constexpr (SEP) {
+        qh[s][e] = hi;
+        ql[s][e] = lo;
+      } else {
+        qh[s][e] = c < 8 ? hi : lo;
+      }
+    }
+  }
+
+  uint4 kf[2][KL];
+  uint2 vf[2][4];
+  Kv8Tile now[2], next[2];
+  const auto tile = [&](int i, Kv8Tile &t) {
+    const int l = i & (kWave - 1), key = tile_key(i);
+    const int pg = __builtin_amdgcn_readlane(t_page, l), ke = __builtin_amdgcn_readlane(t_ke, l);
+    const int ve = __builtin_amdgcn_readlane(t_ve, l);
+    t.held = pg >= 0;
+    t.at = (((size_t)max(pg, 0) * a.KV + kv) << a.page_shift) + (key & (page - 1));
+    t.kscale = e8m0_to_f32((uint32_t)ke);
+    t.ev = ve == 255 ? __builtin_nanf("") : (float)(max(ve, least) - 127);
+    return !t.held || (ve < least) || ve == 0;  // its codes are not to be used
+  };
+  bool mask_v[2], mask_n[2];
+  const auto load_k = [&](const Kv8Tile *t) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const uint8_t *p = a.k + t[x].at * D + c * D + KB * g;
+      if constexpr (D == 32) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        kf[x][0] = make_uint4(v.x, v.y, 0, 0);
+      } else {
+#pragma unroll
+        for (int l = 0; l < KL; l++) kf[x][l] = *reinterpret_cast<const uint4 *>(p + 64 * l);
+      }
+    }
+  };
+  const auto load_v = [&](const Kv8Tile *t) {
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const uint8_t *p = a.v + t[x].at * D + (4 * g + e) * D + VB * c;
+        if constexpr (VB == 8) vf[x][e] = *reinterpret_cast<const uint2 *>(p);
+        if constexpr (VB == 4) vf[x][e].x = *reinterpret_cast<const uint32_t *>(p);
+        if constexpr (VB == 2) vf[x][e].x = *reinterpret_cast<const uint16_t *>(p);
+      }
+  };
+  float m = -INFINITY, l = 0.0f;
+  bool huge = false;  // |m| with few bits left for fractions: x has to be rounded as it was for m
+  v4f acc[VB];
+#pragma unroll
+  for (int j = 0; j < VB; j++) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
+  if (chunks) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) mask_v[x] = tile(x, now[x]);
+    load_k(now);
+    load_v(now);
+  }
+  for (int i = 0; i < chunks; i++) {
+    const int key0 = tile_key(2 * i);
+    // ---- scores of 32 keys
+    v4f s[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      s[x] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        const uint4 kw = kf[x][k >> 1];
+        const v8h kk = k & 1 ? e4m3x8_h(kw.z, kw.w) : e4m3x8_h(kw.x, kw.y);
+        s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[k], s[x], 0, 0, 0);
+        if constexpr (SEP) s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[k], s[x], 0, 0, 0);
+      }
+    }
+    const bool more = i + 1 < chunks;
+    if (more) {
+      if (((2 * i + 2) & (kWave - 1)) == 0) load_tiles(2 * i + 2);
+#pragma unroll
+      for (int x = 0; x < 2; x++) mask_n[x] = tile(2 * i + 2 + x, next[x]);
+      load_k(next);
+    }
+    if constexpr (!SEP) {
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[x][e] += dpp_f<0x128>(s[x][e], 0.0f);  // row_ror:8
+    }
+    // ---- what some row does not see: scores -inf, and V's codes, which may be anything, 0
+    const bool edge = key0 + CK > k_full || mask_v[0] || mask_v[1];
+    if (edge) {
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = key0 + 16 * x + 4 * g + e;
+          s[x][e] = key < lim && now[x].held ? s[x][e] : -INFINITY;
+          if (key >= k_end || mask_v[x]) vf[x][e] = make_uint2(0, 0);
+        }
+    }
+    // ---- the running reference
+    const float c0 = cx * now[0].kscale, c1 = cx * now[1].kscale;
+    const float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+    const float t1 = fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]));
+    const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
+    if (__any(top > m)) {
+      const float mnew = fmaxf(m, ceilf(quarters_max(top)));
+      const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mnew);
+      m = mnew;
+      huge = __any(fabsf(m) > 0x1p22f);
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < VB; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[j][e] *= alpha;
+    }
+    // ---- weights, their sum, and their two terms
+    v8h ph, pl;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - (m == -INFINITY ? 0.0f : m);
+      const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[e] = __builtin_fmaf(s[x][e], cc, off);
+        if (huge) p[e] = (__builtin_fmaf(s[x][e], cc, now[x].ev) - m) + kKv8WUp;
+        p[e] = __builtin_amdgcn_exp2f(p[e]);
+        // a block whose exponent is NaN counts where it is seen
+        if (edge) p[e] = s[x][e] == -INFINITY ? 0.0f : p[e];
+        l = __builtin_fmaf(p[e], edge && p[e] == 0.0f ? 0.0f : unit_l, l);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const h2v hi = pk_half(p[e], p[e + 1]);
+        const h2v lo = pk_half(half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y));
+        if constexpr (SEP) {
+          ph[4 * x + e] = hi.x, ph[4 * x + e + 1] = hi.y;
+          pl[4 * x + e] = lo.x, pl[4 * x + e + 1] = lo.y;
+        } else {
+          ph[4 * x + e] = c < 8 ? hi.x : lo.x, ph[4 * x + e + 1] = c < 8 ? hi.y : lo.y;
+        }
+      }
+    }
+    // ---- out^T += V^T W^T, two output tiles (bytes 2 b, 2 b + 1 of a V load) at a time
+#pragma unroll
+    for (int b = 0; b < VB / 2; b++) {
+      uint32_t z[2][2];  // [tile][key pair]: both bytes of keys 0, 1 and 2, 3
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t u0 = b < 2 ? vf[x][2 * e].x : vf[x][2 * e].y;
+          const uint32_t u1 = b < 2 ? vf[x][2 * e + 1].x : vf[x][2 * e + 1].y;
+          z[x][e] = __builtin_amdgcn_perm(u1, u0, b & 1 ? 0x07030602u : 0x05010400u);
+        }
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const auto two = [&](uint32_t v) {
+          return y ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true)
+                   : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false);
+        };
+        const h2v e0 = two(z[0][0]), e1 = two(z[0][1]), e2 = two(z[1][0]), e3 = two(z[1][1]);
+        const v8h vv = {e0.x, e0.y, e1.x, e1.y, e2.x, e2.y, e3.x, e3.y};
+        v4f &o = acc[2 * b + y];
+        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o, 0, 0, 0);
+        if constexpr (SEP) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o, 0, 0, 0);
+      }
+    }
+    if (more) {
+      load_v(next);
+#pragma unroll
+      for (int x = 0; x < 2; x++) now[x] = next[x], mask_v[x] = mask_n[x];
+    }
+  }
+
+  // ---- the waves' sums, merged; element 4 VB g + VB e + j of row c is acc[j][e]
+  l = quarters_sum(l);
+  if constexpr (!SEP) {
+#pragma unroll
+    for (int j = 0; j < VB; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[j][e] += dpp_f<0x128>(acc[j][e], 0.0f);
+  }
+  if (c < R) {
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int j = 0; j < VB; j++) sh[wave][c][4 * VB * g + VB * e + j] = acc[j][e];
+    if (g == 0) {
+      sm[wave][c] = m;
+      sl[wave][c] = l;
+    }
+  }
+  if (lane == 0) smid[wave] = mid;
+  __syncthreads();
+  const size_t pu = (size_t)unit * a.KV + kv;
+  float *po = part + pu * R * D;
+  float4 *ps = reinterpret_cast<float4 *>(part + (size_t)gridDim.x * R * D) + pu * R;
+  for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
+    const int rr = i / (D / 4), d = 4 * (i % (D / 4)), ro = w.rb * R + rr;
+    if (ro >= rows) break;
+    float M = sm[0][rr];
+    Kv8Unit2 u = {sm[0][rr], smid[0]};
+#pragma unroll
+    for (int x = 1; x < NW; x++) {
+      M = fmaxf(M, sm[x][rr]);
+      u = kv8_larger(u, {sm[x][rr], smid[x]});
+    }
+    const float Mr = M == -INFINITY ? 0.0f : M;
+    if (u.m == -INFINITY) u.m = 0.0f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.0f;
+#pragma unroll
+    for (int x = 0; x < NW; x++) {
+      const float f = __builtin_amdgcn_exp2f(sm[x][rr] - Mr);  // 0 for a wave without keys
+      const float4 v = *reinterpret_cast<const float4 *>(&sh[x][rr][d]);
+      num.x = __builtin_fmaf(v.x, f, num.x);
+      num.y = __builtin_fmaf(v.y, f, num.y);
+      num.z = __builtin_fmaf(v.z, f, num.z);
+      num.w = __builtin_fmaf(v.w, f, num.w);
+      den = __builtin_fmaf(sl[x][rr], __builtin_amdgcn_exp2f((sm[x][rr] - u.m) - (smid[x] - u.mid)), den);
+    }
+    if (w.slices > 1) {
+      *reinterpret_cast<float4 *>(po + rr * D + d) = num;
+      if (d == 0) ps[rr] = make_float4(M, M == -INFINITY ? M : u.m, u.mid, den);
+    } else {
+      const float f = den == 0.0f ? 0.0f : 1.0f / den;
+      const int e = (int)((Mr - u.m) + u.mid), t = ro / G;
+      *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * G + ro - t * G) * D + d) =
+          make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
+    }
+  }
+}
+
+// Partial sums of a row block's slices -> out, a wave a row: lane s holds slice s's scalars (m, the
+// denominator's unit and it), then the lanes share the slices' D-element sums, 256 / D slices at a time.
+template <int D>
+__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
+                                                       size_t sums, int G, float *__restrict__ out, int out_stride) {
+  constexpr int LPR = D / 4, SP = kWave / LPR;
+  const int lane = threadIdx.x & (kWave - 1), e4 = lane % LPR;
+  const int idx = (int)blockIdx.x * 4 + (int)(threadIdx.x / kWave);
+  const int rr = idx % cut.R, kv = idx / cut.R % a.KV;
+  Kv8Seq s;
+  int rb, before;
+  const int keys = kv8_slice_keys(a, cut);
+  const auto slices = [&](const Kv8Seq &q) { return (kv8_keys(a, q) + keys - 1) / keys; };
+  const auto blocks = [&](const Kv8Seq &q) { return kv8_row_blocks(cut, q); };
+  if (!kv8_locate(a, idx / cut.R / a.KV, blocks, s, rb, [&](const Kv8Seq &q) { return blocks(q) * slices(q); }, &before))
+    return;
+  const int ns = slices(s), ro = rb * cut.R + rr;
+  if (ns < 2 || ro >= s.n * G) return;
+  const size_t pu = (size_t)(before + rb * ns) * a.KV + kv, step = (size_t)a.KV;
+  const float4 *sc = reinterpret_cast<const float4 *>(part + sums) + pu * cut.R + rr;
+  const float4 *v = reinterpret_cast<const float4 *>(part) + (pu * cut.R + rr) * LPR + e4;
+  float M = -INFINITY;
+  Kv8Unit2 u = {-INFINITY, 0.0f};
+  const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+  float4 my = none;
+  for (int s0 = 0; s0 < ns; s0 += kWave)
+    if (s0 + lane < ns) {
+      my = sc[(size_t)(s0 + lane) * step * cut.R];
+      M = fmaxf(M, my.x);
+      u = kv8_larger(u, {my.y, my.z});
+    }
+  M = wave_max(M);
+  const float at = u.m - u.mid;
+  const int best = __ffsll((unsigned long long)__ballot(at == wave_max(at))) - 1;
+  u.m = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(u.m), best));
+  u.mid = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(u.mid), best));
+  const float Mr = M == -INFINITY ? 0.0f : M;
+  if (u.m == -INFINITY) u.m = 0.0f;
+  float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+  float den = 0.0f;
+  for (int s0 = 0; s0 < ns; s0 += kWave) {
+    const int n = min(ns - s0, kWave);
+    if (ns > kWave) my = lane < n ? sc[(size_t)(s0 + lane) * step * cut.R] : none;
+    const float f = __builtin_amdgcn_exp2f(my.x - Mr);  // 0 for a slice without keys, and past the last
+    den = __builtin_fmaf(my.w, __builtin_amdgcn_exp2f((my.y - u.m) - (my.z - u.mid)), den);
+#pragma unroll 4
+    for (int i = 0; i < n; i += SP) {
+      const int k = i + lane / LPR;
+      const float fk = __shfl(f, k & (kWave - 1));
+      if (k < n) {
+        const float4 x = v[(size_t)(s0 + k) * step * cut.R * LPR];
+        num.x = __builtin_fmaf(x.x, fk, num.x);
+        num.y = __builtin_fmaf(x.y, fk, num.y);
+        num.z = __builtin_fmaf(x.z, fk, num.z);
+        num.w = __builtin_fmaf(x.w, fk, num.w);
+      }
+    }
+  }
+  den = wave_sum(den);
+#pragma unroll
+  for (int o = LPR; o < kWave; o <<= 1) {
+    num.x += __shfl_xor(num.x, o);
+    num.y += __shfl_xor(num.y, o);
+    num.z += __shfl_xor(num.z, o);
+    num.w += __shfl_xor(num.w, o);
+  }
+  if (lane >= LPR) return;
+  const float f = den == 0.0f ? 0.0f : 1.0f / den;
+  const int e = (int)((Mr - u.m) + u.mid), t = ro / G;
+  *reinterpret_cast<float4 *>(out + (size_t)(s.row0 + t) * out_stride + (kv * G + ro - t * G) * D + 4 * e4) =
+      make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
+}
 
 // One wave a row and head: a key per lane and round, the round's weights in LDS, then the
 // lanes own output elements.
 template <int D>
 __global__ __launch_bounds__(kWave) void kv8_attend_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
-                                                           int H, float *__restrict__ out, int out_stride) {
+                                                           int H, float *__restrict__ out, int out_stride,
+                                                           int rows_min) {
   constexpr int DPL = (D + kWave - 1) / kWave;
   __shared__ float qs[D], ps[kWave];
   __shared__ size_t rows[kWave];
   const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kv = h / (H / a.KV);
   Kv8Seq s;
-  if (!kv8_find_row(a, row, s)) return;
+  if (!kv8_find_row(a, row, s) || s.n * (H / a.KV) < rows_min) return;
   const int cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
   const int S = min(s.past + row - s.row0 + 1, cap);
   for (int e = lane; e < D; e += kWave) qs[e] = q[(size_t)row * q_stride + h * D + e];
@@ -346,18 +855,63 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
   return hipErrorInvalidValue;
 }
 
-hipError_t launch_kv8_attention(const Kv8Args &a, int D, const float *q, int q_stride, int H, float *out,
-                                int out_stride, void *work, hipStream_t s) {
-  const auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(a.T, H), dim3(kWave), 0, s, a, q, q_stride, H, out, out_stride);
-    return hipGetLastError();
-  };
-  if (D == 32) return go(kv8_attend_kernel<32>);
-  if (D == 64) return go(kv8_attend_kernel<64>);
-  if (D == 128) return go(kv8_attend_kernel<128>);
-  return hipErrorInvalidValue;
+// ---- how a call's attention is cut
+
+struct Kv8Plan {
+  Kv8Cut step;
+  long long step_blocks, step_units;  // most row blocks, and slices of them
+  size_t step_sums;                   // floats of the step slices' sums, their scalars behind them
+};
+
+constexpr int kKv8StepRows = 32;  // rows of a sequence and KV head that the step kernel takes
+
+static Kv8Plan kv8_plan(const Kv8Args &a, int D, int H) {
+  Kv8Plan p;
+  const int G = H / a.KV;
+  const long long most = (long long)a.max_new * G;
+  const int R = most <= 8 ? 8 : 16;
+  p.step = {G, R, 1, kKv8StepRows, std::max(1, 1024 / a.KV), 256};
+  p.step_blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
+  p.step_units = p.step_blocks + p.step.slots;
+  p.step_sums = (size_t)p.step_units * a.KV * R * D;
+  return p;
 }
 
-size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H) { return 0; }
+size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H) {
+  const Kv8Plan p = kv8_plan(a, D, H);
+  return (p.step_sums + (size_t)p.step_units * a.KV * p.step.R * 4) * sizeof(float);
+}
+
+template <int D>
+static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, int H, float *out, int out_stride,
+                                float *work, hipStream_t s) {
+  const Kv8Plan p = kv8_plan(a, D, H);
+  const long long grid = p.step_units * a.KV, merge = (p.step_blocks * a.KV * p.step.R + 3) / 4;
+  if (grid > 0x7FFFFFFF || merge > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const auto go = [&](auto kern, int nw) {
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(nw * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
+                       p.step);
+  };
+  if (p.step.R == 8)
+    go(kv8_step_kernel<D, false, 4>, 4);
+  else
+    go(kv8_step_kernel<D, true, 4>, 4);
+  if ((a.max_pages << a.page_shift) > p.step.min_keys)
+    hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3((unsigned)merge), dim3(256), 0, s, a, p.step, work, p.step_sums,
+                       H / a.KV, out, out_stride);
+  if ((long long)a.max_new * (H / a.KV) > kKv8StepRows)
+    hipLaunchKernelGGL(kv8_attend_kernel<D>, dim3(a.T, H), dim3(kWave), 0, s, a, q, q_stride, H, out, out_stride,
+                       kKv8StepRows + 1);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv8_attention(const Kv8Args &a, int D, const float *q, int q_stride, int H, float *out,
+                                int out_stride, void *work, hipStream_t s) {
+  float *w = static_cast<float *>(work);
+  if (D == 32) return kv8_attention<32>(a, q, q_stride, H, out, out_stride, w, s);
+  if (D == 64) return kv8_attention<64>(a, q, q_stride, H, out, out_stride, w, s);
+  if (D == 128) return kv8_attention<128>(a, q, q_stride, H, out, out_stride, w, s);
+  return hipErrorInvalidValue;
+}
 
 }  // namespace lbk
