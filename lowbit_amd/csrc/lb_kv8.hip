@@ -67,18 +67,18 @@ __device__ __forceinline__ Kv8Seq kv8_lane(const Kv8Seq &s, int lane) {
 
 // Unit u of the batch's units (sequence b has units(its Kv8Seq) of them, in order): its
 // sequence in s, its index there in `at` and, where asked, the sum of weight(..) over the
-// sequences before it. False past the last. By the whole wave: 64 sequences a step, one round
-// trip of loads each.
+// sequences before it. False past the last. By the whole wave, 64 sequences a step, the first
+// of them in `first` already.
 struct Kv8None {
   __device__ int operator()(const Kv8Seq &) const { return 0; }
 };
 template <class F, class W = Kv8None>
-__device__ __forceinline__ bool kv8_locate(const Kv8Args &a, int u, F units, Kv8Seq &s, int &at, W weight = W(),
-                                           int *before = nullptr) {
+__device__ __forceinline__ bool kv8_locate(const Kv8Args &a, const Kv8Seq &first, int u, F units, Kv8Seq &s, int &at,
+                                           W weight = W(), int *before = nullptr) {
   const int lane = threadIdx.x & (kWave - 1);
   int base = 0, sum = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const Kv8Seq q = kv8_seq(a, b0 + lane);
+    const Kv8Seq q = b0 ? kv8_seq(a, b0 + lane) : first;
     const int c = units(q), inc = wave_scan(c), all = __builtin_amdgcn_readlane(inc, 63);
     const int wt = before ? weight(q) : 0, winc = before ? wave_scan(wt) : 0;
     if (u < base + all) {
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
     const int end = min(q.past + q.n, cap);
     return end > q.past ? ((end - 1) >> a.page_shift) - (q.past >> a.page_shift) + 1 : 0;
   };
-  if (!kv8_locate(a, unit, pages_of, s, at)) return;
+  if (!kv8_locate(a, kv8_seq(a, tid & (kWave - 1)), unit, pages_of, s, at)) return;
   const int pi = (s.past >> a.page_shift) + at;
   const int t0 = max(s.past, pi << a.page_shift), t1 = min(min(s.past + s.n, cap), (pi + 1) << a.page_shift);
   const int lo = t0 & (page - 1), items = (t1 - t0) * PER;
@@ -292,14 +292,17 @@ __device__ __forceinline__ int kv8_keys(const Kv8Args &a, const Kv8Seq &s) {
   return min(s.past + s.n, a.max_pages << a.page_shift);
 }
 
+// Rows of a row block, by the column blocks of 16 a wave takes (0: 8 rows, both terms in one).
+__host__ __device__ constexpr int kv8_rows(int nc) { return nc ? 16 * nc : 8; }
+
 __device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-// Keys a slice: the batch's row blocks times keys over the slots, so that however the lengths
-// differ the slices are alike, in steps of 256. (The sum in float, 1 % up: never more slices
-// than slots and row blocks together.)
-__device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c) {
-  float sum = 0.0f;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+// How many keys a slice has: the batch's row blocks times keys over the slots, so that however
+// the lengths differ the slices are alike, in steps of 256. (The sum in float, 1 % up: never
+// more slices than slots and row blocks together.) `first`: sequences 0 .. 63 by lane.
+__device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first) {
+  float sum = (float)kv8_row_blocks(c, first) * (float)kv8_keys(a, first);
+  for (int b0 = kWave; b0 < a.B; b0 += kWave) {
     const Kv8Seq s = kv8_seq(a, b0 + (int)(threadIdx.x & (kWave - 1)));
     sum += (float)kv8_row_blocks(c, s) * (float)kv8_keys(a, s);
   }
@@ -307,19 +310,30 @@ __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c)
   return max(c.min_keys, round_up((int)per + 1, 256));
 }
 
-// Row block and slice of unit u.
+// Row block and slice of unit u; or, u a row block, that row block and the units before its
+// sequence's.
 struct Kv8Unit {
   Kv8Seq s;
-  int rb, slice, slices, slice_keys;
+  int rb, slice, slices, slice_keys, before, at;
 };
+template <bool BLOCK>
 __device__ __forceinline__ bool kv8_unit(const Kv8Args &a, const Kv8Cut &c, int u, Kv8Unit &w) {
-  w.slice_keys = kv8_slice_keys(a, c);
+  const Kv8Seq first = kv8_seq(a, threadIdx.x & (kWave - 1));
+  w.slice_keys = kv8_slice_keys(a, c, first);
+  const auto blocks = [&](const Kv8Seq &s) { return kv8_row_blocks(c, s); };
   const auto slices = [&](const Kv8Seq &s) { return (kv8_keys(a, s) + w.slice_keys - 1) / w.slice_keys; };
-  int at;
-  if (!kv8_locate(a, u, [&](const Kv8Seq &s) { return kv8_row_blocks(c, s) * slices(s); }, w.s, at)) return false;
-  w.slices = slices(w.s);
-  w.rb = at / w.slices;
-  w.slice = at - w.rb * w.slices;
+  const auto units = [&](const Kv8Seq &s) { return blocks(s) * slices(s); };
+  if constexpr (BLOCK) {
+    if (!kv8_locate(a, first, u, blocks, w.s, w.at, units, &w.before)) return false;
+    w.slices = slices(w.s);
+    w.rb = w.at;
+  } else {  // the last row blocks, which see the most keys, first
+    if (!kv8_locate(a, first, u, units, w.s, w.at)) return false;
+    w.slices = slices(w.s);
+    const int back = w.at / w.slices;
+    w.rb = blocks(w.s) - 1 - back;
+    w.slice = w.at - back * w.slices;
+  }
   return true;
 }
 
@@ -362,12 +376,12 @@ struct Kv8Unit2 {
 };
 __device__ __forceinline__ Kv8Unit2 kv8_larger(Kv8Unit2 a, Kv8Unit2 b) { return b.m - b.mid > a.m - a.mid ? b : a; }
 
-// A tile of 16 keys as a wave holds it: page 0 stands in where there is none.
+// A tile of 16 keys as a wave holds it.
 struct Kv8Tile {
-  size_t at;       // first code row
-  bool held;       // some of its keys count
-  float kscale;    // 2^ke of K
-  float ev;        // V's exponent
+  bool held;     // there is such a page
+  bool unused;   // its V codes are not to be used
+  float kscale;  // 2^ke of K
+  float ev;      // V's exponent
 };
 
 // Few query rows a sequence (steps): R = 8 rows a block, or 16 (SEP). NW waves share a slice
@@ -382,25 +396,32 @@ struct Kv8Tile {
 // that V needs, and its output elements come out contiguous. The next chunk's K is requested
 // once the scores are made, its V once the outputs are: loads are always in flight, and no
 // LDS lies between them and the matrix cores.
-template <int D, bool SEP, int NW>
-__global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
+template <int D, int NC, int NW>
+__global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 4) void kv8_attend_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
                                                                int H, float *__restrict__ out, int out_stride,
                                                                float *__restrict__ part, Kv8Cut cut) {
-  constexpr int R = SEP ? 16 : 8, KS = D / 32, CK = 32;
+  constexpr bool SEP = NC > 0;
+  constexpr int NB = SEP ? NC : 1, R = kv8_rows(NC), KS = D / 32, CK = 32;
   constexpr int KB = D >= 64 ? 16 : 8, KL = D / (4 * KB);  // bytes of a K load, loads per lane and tile
-  constexpr int VB = D / 16, VW = VB > 4 ? 2 : 1;           // bytes of a V load (a key's), words of it
+  constexpr int VB = D / 16;                               // bytes of a V load (a key's)
   constexpr int PS = D + 4;
   __shared__ float sh[NW][R][PS];
   __shared__ float sm[NW][R], sl[NW][R], smid[NW];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int c = lane & 15, g = lane >> 4, row_c = SEP ? c : c & 7;
+  const int c = lane & 15, g = lane >> 4;
   const int kv = (int)blockIdx.x % a.KV, unit = (int)blockIdx.x / a.KV;
   Kv8Unit w;
-  if (!kv8_unit(a, cut, unit, w)) return;
+  if (!kv8_unit<false>(a, cut, unit, w)) return;
   const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
-  // this lane's query row, and the keys that it and the block's last row see
-  const int r = w.rb * R + row_c, tok = min(r, rows - 1) / G, head = kv * G + min(r, rows - 1) - tok * G;
-  const int lim = r < rows ? min(w.s.past + tok + 1, cap) : 0;
+  // this lane's query rows, the keys they see, and those that the block's last row sees
+  int lim[NB];
+  const float *qr[NB];
+#pragma unroll
+  for (int y = 0; y < NB; y++) {
+    const int r = w.rb * R + (SEP ? 16 * y + c : c & 7), rc = min(r, rows - 1), tok = rc / G;
+    lim[y] = r < rows ? min(w.s.past + tok + 1, cap) : 0;
+    qr[y] = q + (size_t)(w.s.row0 + tok) * q_stride + (kv * G + rc - tok * G) * D;
+  }
   const int tok_last = (min(w.rb * R + R, rows) - 1) / G, tok_first = w.rb * R / G;
   const int k_begin = w.slice * w.slice_keys;
   const int k_end = min(min(w.s.past + tok_last + 1, cap), k_begin + w.slice_keys);
@@ -408,77 +429,45 @@ __global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_k
   const int chunks = max(0, (k_end - k_begin - CK * wave + CK * NW - 1) / (CK * NW));
   const int32_t *table = a.table + (size_t)w.s.b * a.max_pages;
 
-  // ---- tiles of the wave's next 32 chunks, one a lane; `biggest`: their largest V exponent
+  // ---- tiles of the wave's next 32 chunks, one a lane (t_ve -1: no such page)
   int t_page = 0, t_ke = 0, t_ve = 0;
   const auto tile_key = [&](int i) { return k_begin + CK * (wave + NW * (i >> 1)) + 16 * (i & 1); };
   const auto load_tiles = [&](int i0) {
     const int key = tile_key(i0 + lane);
     const int pg = key < k_end ? table[key >> a.page_shift] : -1;
     const bool in = (unsigned)pg < (unsigned)a.pages;
-    const size_t block = (size_t)(in ? pg : 0) * a.KV + kv;
-    t_page = in ? pg : -1;
+    t_page = in ? pg : 0;
+    const size_t block = (size_t)t_page * a.KV + kv;
     t_ke = a.ke[block];
-    t_ve = in ? a.ve[block] : -1;
-    return wave_max_i32(t_ve == 255 ? -1 : t_ve);
+    t_ve = a.ve[block];
+    t_ve = in ? t_ve : -1;
   };
-  const float *qr = q + (size_t)(w.s.row0 + tok) * q_stride + head * D;
-  v8h qh[KS], ql[SEP ? KS : 1];
-  float4 qf[KS][2];
+  v8h qh[NB][KS], ql[NB][SEP ? KS : 1];
+  float4 qf[NB][KS][2];
 #pragma unroll
-  for (int s = 0; s < KS; s++) {
-    const int d = D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-    qf[s][0] = *reinterpret_cast<const float4 *>(qr + d);
-    qf[s][1] = *reinterpret_cast<const float4 *>(qr + d + 4);
-  }
-  int biggest = load_tiles(0);
-  for (int i = kWave; i < 2 * chunks; i += kWave) biggest = max(biggest, load_tiles(i));
-  if (2 * chunks > kWave) load_tiles(0);
-  const int least = max(biggest - kKv8Spread, 0);  // E8M0 exponents of V below count as zeros
-  const float mid = (float)(max(biggest, 0) - kKv8Spread / 2 - 127);
-
-  // ---- the query row in two terms
-  int big = 0;
+  for (int y = 0; y < NB; y++)
 #pragma unroll
-  for (int s = 0; s < KS; s++) big = max(big, max(abs_bits(qf[s][0]), abs_bits(qf[s][1])));
-  big = max(big, __shfl_xor(big, 16));
-  big = max(big, __shfl_xor(big, 32));
-  float up, down;
-  kv8_q_scale(big, up, down);
-  const float cx = down * (kKv8Log2e / sqrtf((float)D));
-#pragma unroll
-  for (int s = 0; s < KS; s++) {
-    const float x[8] = {qf[s][0].x * up, qf[s][0].y * up, qf[s][0].z * up, qf[s][0].w * up,
-                        qf[s][1].x * up, qf[s][1].y * up, qf[s][1].z * up, qf[s][1].w * up};
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const _Float16 hi = (_Float16)x[e], lo = (_Float16)half_rest(x[e], hi);
-      if constexpr (SEP) {
-        qh[s][e] = hi;
-        ql[s][e] = lo;
-      } else {
-        qh[s][e] = c < 8 ? hi : lo;
-      }
+    for (int s = 0; s < KS; s++) {
+      const int d = D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+      qf[y][s][0] = *reinterpret_cast<const float4 *>(qr[y] + d);
+      qf[y][s][1] = *reinterpret_cast<const float4 *>(qr[y] + d + 4);
     }
-  }
+  load_tiles(0);
 
+  // ---- codes of a chunk's two tiles (no page: page 0's, not used)
   uint4 kf[2][KL];
   uint2 vf[2][4];
-  Kv8Tile now[2], next[2];
-  const auto tile = [&](int i, Kv8Tile &t) {
-    const int l = i & (kWave - 1), key = tile_key(i);
-    const int pg = __builtin_amdgcn_readlane(t_page, l), ke = __builtin_amdgcn_readlane(t_ke, l);
-    const int ve = __builtin_amdgcn_readlane(t_ve, l);
-    t.held = pg >= 0;
-    t.at = (((size_t)max(pg, 0) * a.KV + kv) << a.page_shift) + (key & (page - 1));
-    t.kscale = e8m0_to_f32((uint32_t)ke);
-    t.ev = ve == 255 ? __builtin_nanf("") : (float)(max(ve, least) - 127);
-    return !t.held || (ve < least) || ve == 0;  // its codes are not to be used
+  size_t at[2];  // first code row of the tiles requested last
+  const auto locate = [&](int i) {
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+      at[x] = (((size_t)__builtin_amdgcn_readlane(t_page, (i + x) & (kWave - 1)) * a.KV + kv) << a.page_shift) +
+              (tile_key(i + x) & (page - 1));
   };
-  bool mask_v[2], mask_n[2];
-  const auto load_k = [&](const Kv8Tile *t) {
+  const auto load_k = [&]() {
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      const uint8_t *p = a.k + t[x].at * D + c * D + KB * g;
+      const uint8_t *p = a.k + at[x] * D + c * D + KB * g;
       if constexpr (D == 32) {
         const uint2 v = *reinterpret_cast<const uint2 *>(p);
         kf[x][0] = make_uint4(v.x, v.y, 0, 0);
@@ -488,109 +477,173 @@ __global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_k
       }
     }
   };
-  const auto load_v = [&](const Kv8Tile *t) {
+  const auto load_v = [&]() {
 #pragma unroll
     for (int x = 0; x < 2; x++)
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const uint8_t *p = a.v + t[x].at * D + (4 * g + e) * D + VB * c;
+        const uint8_t *p = a.v + at[x] * D + (4 * g + e) * D + VB * c;
         if constexpr (VB == 8) vf[x][e] = *reinterpret_cast<const uint2 *>(p);
         if constexpr (VB == 4) vf[x][e].x = *reinterpret_cast<const uint32_t *>(p);
         if constexpr (VB == 2) vf[x][e].x = *reinterpret_cast<const uint16_t *>(p);
       }
   };
-  float m = -INFINITY, l = 0.0f;
-  bool huge = false;  // |m| with few bits left for fractions: x has to be rounded as it was for m
-  v4f acc[VB];
-#pragma unroll
-  for (int j = 0; j < VB; j++) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
   if (chunks) {
-#pragma unroll
-    for (int x = 0; x < 2; x++) mask_v[x] = tile(x, now[x]);
-    load_k(now);
-    load_v(now);
+    locate(0);
+    load_k();
+    load_v();
   }
+
+  // ---- the wave's largest V exponent
+  int biggest = wave_max_i32(t_ve == 255 ? -1 : t_ve);
+  if (2 * chunks > kWave) {
+    for (int i = kWave; i < 2 * chunks; i += kWave) {
+      load_tiles(i);
+      biggest = max(biggest, wave_max_i32(t_ve == 255 ? -1 : t_ve));
+    }
+    load_tiles(0);
+  }
+  const int least = max(biggest - kKv8Spread, 0);  // E8M0 exponents of V below count as zeros
+  const float mid = (float)(max(biggest, 0) - kKv8Spread / 2 - 127);
+
+  // ---- the query rows in two terms
+  float cx[NB];
+#pragma unroll
+  for (int y = 0; y < NB; y++) {
+    int big = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++) big = max(big, max(abs_bits(qf[y][s][0]), abs_bits(qf[y][s][1])));
+    big = max(big, __shfl_xor(big, 16));
+    big = max(big, __shfl_xor(big, 32));
+    float up, down;
+    kv8_q_scale(big, up, down);
+    cx[y] = down * (kKv8Log2e / sqrtf((float)D));
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const float4 a0 = qf[y][s][0], a1 = qf[y][s][1];
+      const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const _Float16 hi = (_Float16)x[e], lo = (_Float16)half_rest(x[e], hi);
+        if constexpr (SEP) {
+          qh[y][s][e] = hi;
+          ql[y][s][e] = lo;
+        } else {
+          qh[y][s][e] = c < 8 ? hi : lo;
+        }
+      }
+    }
+  }
+
+  float m[NB], l[NB];
+  v4f acc[NB][VB];
+#pragma unroll
+  for (int y = 0; y < NB; y++) {
+    m[y] = -INFINITY, l[y] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VB; j++) acc[y][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  bool huge = false;  // |m| with few bits left for fractions: x has to be rounded as it was for m
   for (int i = 0; i < chunks; i++) {
     const int key0 = tile_key(2 * i);
-    // ---- scores of 32 keys
-    v4f s[2];
+    Kv8Tile now[2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      s[x] = v4f{0.f, 0.f, 0.f, 0.f};
+      const int o = (2 * i + x) & (kWave - 1);
+      const int ke = __builtin_amdgcn_readlane(t_ke, o), ve = __builtin_amdgcn_readlane(t_ve, o);
+      now[x].held = ve >= 0;
+      now[x].unused = ve < max(least, 1);
+      now[x].kscale = e8m0_to_f32((uint32_t)ke);
+      now[x].ev = ve == 255 ? __builtin_nanf("") : (float)(max(ve, least) - 127);
+    }
+    // ---- scores of 32 keys
+    v4f s[NB][2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+#pragma unroll
+      for (int y = 0; y < NB; y++) s[y][x] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < KS; k++) {
         const uint4 kw = kf[x][k >> 1];
         const v8h kk = k & 1 ? e4m3x8_h(kw.z, kw.w) : e4m3x8_h(kw.x, kw.y);
-        s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[k], s[x], 0, 0, 0);
-        if constexpr (SEP) s[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[k], s[x], 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < NB; y++) {
+          s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[y][k], s[y][x], 0, 0, 0);
+          if constexpr (SEP) s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[y][k], s[y][x], 0, 0, 0);
+        }
       }
     }
     const bool more = i + 1 < chunks;
     if (more) {
       if (((2 * i + 2) & (kWave - 1)) == 0) load_tiles(2 * i + 2);
-#pragma unroll
-      for (int x = 0; x < 2; x++) mask_n[x] = tile(2 * i + 2 + x, next[x]);
-      load_k(next);
+      locate(2 * i + 2);
+      load_k();
     }
     if constexpr (!SEP) {
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[x][e] += dpp_f<0x128>(s[x][e], 0.0f);  // row_ror:8
+        for (int e = 0; e < 4; e++) s[0][x][e] += dpp_f<0x128>(s[0][x][e], 0.0f);  // row_ror:8
     }
     // ---- what some row does not see: scores -inf, and V's codes, which may be anything, 0
-    const bool edge = key0 + CK > k_full || mask_v[0] || mask_v[1];
+    const bool edge = key0 + CK > k_full || now[0].unused || now[1].unused;
     if (edge) {
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int key = key0 + 16 * x + 4 * g + e;
-          s[x][e] = key < lim && now[x].held ? s[x][e] : -INFINITY;
-          if (key >= k_end || mask_v[x]) vf[x][e] = make_uint2(0, 0);
+#pragma unroll
+          for (int y = 0; y < NB; y++) s[y][x][e] = key < lim[y] && now[x].held ? s[y][x][e] : -INFINITY;
+          if (key >= k_end || now[x].unused) vf[x][e] = make_uint2(0, 0);
         }
     }
-    // ---- the running reference
-    const float c0 = cx * now[0].kscale, c1 = cx * now[1].kscale;
-    const float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
-    const float t1 = fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]));
-    const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
-    if (__any(top > m)) {
-      const float mnew = fmaxf(m, ceilf(quarters_max(top)));
-      const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mnew);
-      m = mnew;
-      huge = __any(fabsf(m) > 0x1p22f);
-      l *= alpha;
+    v8h ph[NB], pl[NB];
 #pragma unroll
-      for (int j = 0; j < VB; j++)
+    for (int y = 0; y < NB; y++) {
+      // ---- the running reference
+      const float c0 = cx[y] * now[0].kscale, c1 = cx[y] * now[1].kscale;
+      const v4f s0 = s[y][0], s1 = s[y][1];
+      const float t0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3]));
+      const float t1 = fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]));
+      const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
+      if (__any(top > m[y])) {
+        const float mnew = fmaxf(m[y], ceilf(quarters_max(top)));
+        const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[y] - mnew);
+        m[y] = mnew;
+        huge = huge || __any(fabsf(mnew) > 0x1p22f && mnew != -INFINITY);
+        l[y] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[j][e] *= alpha;
-    }
-    // ---- weights, their sum, and their two terms
-    v8h ph, pl;
+        for (int j = 0; j < VB; j++)
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-      const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - (m == -INFINITY ? 0.0f : m);
-      const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
-      float p[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        p[e] = __builtin_fmaf(s[x][e], cc, off);
-        if (huge) p[e] = (__builtin_fmaf(s[x][e], cc, now[x].ev) - m) + kKv8WUp;
-        p[e] = __builtin_amdgcn_exp2f(p[e]);
-        // a block whose exponent is NaN counts where it is seen
-        if (edge) p[e] = s[x][e] == -INFINITY ? 0.0f : p[e];
-        l = __builtin_fmaf(p[e], edge && p[e] == 0.0f ? 0.0f : unit_l, l);
+          for (int e = 0; e < 4; e++) acc[y][j][e] *= alpha;
       }
+      // ---- weights, their sum, and their two terms
+      const float ref = m[y] == -INFINITY ? 0.0f : m[y];
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const h2v hi = pk_half(p[e], p[e + 1]);
-        const h2v lo = pk_half(half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y));
-        if constexpr (SEP) {
-          ph[4 * x + e] = hi.x, ph[4 * x + e + 1] = hi.y;
-          pl[4 * x + e] = lo.x, pl[4 * x + e + 1] = lo.y;
-        } else {
-          ph[4 * x + e] = c < 8 ? hi.x : lo.x, ph[4 * x + e + 1] = c < 8 ? hi.y : lo.y;
+      for (int x = 0; x < 2; x++) {
+        const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - ref;
+        const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          p[e] = __builtin_fmaf(s[y][x][e], cc, off);
+          if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - ref) + kKv8WUp;
+          p[e] = __builtin_amdgcn_exp2f(p[e]);
+          // a block whose exponent is NaN counts where it is seen
+          if (edge) p[e] = s[y][x][e] == -INFINITY ? 0.0f : p[e];
+          l[y] = __builtin_fmaf(p[e], edge && p[e] == 0.0f ? 0.0f : unit_l, l[y]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const h2v hi = pk_half(p[e], p[e + 1]);
+          const h2v lo = pk_half(half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y));
+          if constexpr (SEP) {
+            ph[y][4 * x + e] = hi.x, ph[y][4 * x + e + 1] = hi.y;
+            pl[y][4 * x + e] = lo.x, pl[y][4 * x + e + 1] = lo.y;
+          } else {
+            ph[y][4 * x + e] = c < 8 ? hi.x : lo.x, ph[y][4 * x + e + 1] = c < 8 ? hi.y : lo.y;
+          }
         }
       }
     }
@@ -614,39 +667,41 @@ __global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_k
         };
         const h2v e0 = two(z[0][0]), e1 = two(z[0][1]), e2 = two(z[1][0]), e3 = two(z[1][1]);
         const v8h vv = {e0.x, e0.y, e1.x, e1.y, e2.x, e2.y, e3.x, e3.y};
-        v4f &o = acc[2 * b + y];
-        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o, 0, 0, 0);
-        if constexpr (SEP) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o, 0, 0, 0);
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+          v4f &o = acc[n][2 * b + y];
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[n], o, 0, 0, 0);
+          if constexpr (SEP) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[n], o, 0, 0, 0);
+        }
       }
     }
-    if (more) {
-      load_v(next);
-#pragma unroll
-      for (int x = 0; x < 2; x++) now[x] = next[x], mask_v[x] = mask_n[x];
-    }
+    if (more) load_v();
   }
 
-  // ---- the waves' sums, merged; element 4 VB g + VB e + j of row c is acc[j][e]
-  l = quarters_sum(l);
-  if constexpr (!SEP) {
+  // ---- the waves' sums, merged; element 4 VB g + VB e + j of row c is acc[.][j][e]
 #pragma unroll
-    for (int j = 0; j < VB; j++)
+  for (int y = 0; y < NB; y++) {
+    l[y] = quarters_sum(l[y]);
+    if constexpr (!SEP) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) acc[j][e] += dpp_f<0x128>(acc[j][e], 0.0f);
-  }
-  if (c < R) {
+      for (int j = 0; j < VB; j++)
 #pragma unroll
-    for (int e = 0; e < 4; e++)
+        for (int e = 0; e < 4; e++) acc[y][j][e] += dpp_f<0x128>(acc[y][j][e], 0.0f);
+    }
+    if (SEP || c < 8) {
 #pragma unroll
-      for (int j = 0; j < VB; j++) sh[wave][c][4 * VB * g + VB * e + j] = acc[j][e];
-    if (g == 0) {
-      sm[wave][c] = m;
-      sl[wave][c] = l;
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int j = 0; j < VB; j++) sh[wave][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
+      if (g == 0) {
+        sm[wave][16 * y + c] = m[y];
+        sl[wave][16 * y + c] = l[y];
+      }
     }
   }
   if (lane == 0) smid[wave] = mid;
   __syncthreads();
-  const size_t pu = (size_t)unit * a.KV + kv;
+  const size_t pu = (size_t)(unit - w.at + w.rb * w.slices + w.slice) * a.KV + kv;
   float *po = part + pu * R * D;
   float4 *ps = reinterpret_cast<float4 *>(part + (size_t)gridDim.x * R * D) + pu * R;
   for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
@@ -685,37 +740,42 @@ __global__ __launch_bounds__(NW *kWave, SEP && D == 128 ? 3 : 4) void kv8_step_k
   }
 }
 
-// Partial sums of a row block's slices -> out, a wave a row: lane s holds slice s's scalars (m, the
-// denominator's unit and it), then the lanes share the slices' D-element sums, 256 / D slices at a time.
-template <int D>
+// Partial sums of a row block's slices -> out. W waves share a row: lane s of each holds slice
+// s's scalars (m, the denominator's unit and it), and the row's D-element sums, 256 / D slices
+// to a wave load, go round the waves, eight loads requested before the scalars are waited for.
+// Four waves where there are few rows: 118 slices of 32 rows took a wave a row 22.8 us.
+template <int D, int W>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
-                                                       size_t sums, int G, float *__restrict__ out, int out_stride) {
-  constexpr int LPR = D / 4, SP = kWave / LPR;
+                                                       size_t sums, float *__restrict__ out, int out_stride) {
+  constexpr int LPR = D / 4, SP = kWave / LPR, U = 8;
+  __shared__ float4 sh[W > 1 ? W : 1][LPR];
   const int lane = threadIdx.x & (kWave - 1), e4 = lane % LPR;
-  const int idx = (int)blockIdx.x * 4 + (int)(threadIdx.x / kWave);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wr = wave % W;
+  const int idx = (int)blockIdx.x * (4 / W) + wave / W;
   const int rr = idx % cut.R, kv = idx / cut.R % a.KV;
-  Kv8Seq s;
-  int rb, before;
-  const int keys = kv8_slice_keys(a, cut);
-  const auto slices = [&](const Kv8Seq &q) { return (kv8_keys(a, q) + keys - 1) / keys; };
-  const auto blocks = [&](const Kv8Seq &q) { return kv8_row_blocks(cut, q); };
-  if (!kv8_locate(a, idx / cut.R / a.KV, blocks, s, rb, [&](const Kv8Seq &q) { return blocks(q) * slices(q); }, &before))
-    return;
-  const int ns = slices(s), ro = rb * cut.R + rr;
-  if (ns < 2 || ro >= s.n * G) return;
-  const size_t pu = (size_t)(before + rb * ns) * a.KV + kv, step = (size_t)a.KV;
+  Kv8Unit w;
+  if (!kv8_unit<true>(a, cut, idx / cut.R / a.KV, w)) return;
+  const int ns = w.slices, ro = w.rb * cut.R + rr;
+  if (ns < 2 || ro >= w.s.n * cut.G) return;
+  const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(part + sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(part) + (pu * cut.R + rr) * LPR + e4;
+  const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+  float4 x[U];
+  const auto load = [&](int i0) {  // this wave's next slices, past the last the last again
+#pragma unroll
+    for (int i = 0; i < U; i++) x[i] = v[(size_t)min(i0 + SP * W * i + lane / LPR, ns - 1) * step * LPR];
+  };
   float M = -INFINITY;
   Kv8Unit2 u = {-INFINITY, 0.0f};
-  const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-  float4 my = none;
-  for (int s0 = 0; s0 < ns; s0 += kWave)
-    if (s0 + lane < ns) {
-      my = sc[(size_t)(s0 + lane) * step * cut.R];
-      M = fmaxf(M, my.x);
-      u = kv8_larger(u, {my.y, my.z});
-    }
+  float4 my = lane < ns ? sc[(size_t)lane * step] : none;
+  load(SP * wr);
+  const float4 head = my;
+  for (int s0 = 0; s0 < ns; s0 += kWave) {
+    if (s0) my = s0 + lane < ns ? sc[(size_t)(s0 + lane) * step] : none;
+    M = fmaxf(M, my.x);
+    u = kv8_larger(u, {my.y, my.z});
+  }
   M = wave_max(M);
   const float at = u.m - u.mid;
   const int best = __ffsll((unsigned long long)__ballot(at == wave_max(at))) - 1;
@@ -725,21 +785,24 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, c
   if (u.m == -INFINITY) u.m = 0.0f;
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.0f;
-  for (int s0 = 0; s0 < ns; s0 += kWave) {
-    const int n = min(ns - s0, kWave);
-    if (ns > kWave) my = lane < n ? sc[(size_t)(s0 + lane) * step * cut.R] : none;
+  my = head;
+  for (int s0 = 0; s0 < ns; s0 += kWave) {  // 64 slices' scalars in the lanes
+    if (s0) my = s0 + lane < ns ? sc[(size_t)(s0 + lane) * step] : none;
     const float f = __builtin_amdgcn_exp2f(my.x - Mr);  // 0 for a slice without keys, and past the last
     den = __builtin_fmaf(my.w, __builtin_amdgcn_exp2f((my.y - u.m) - (my.z - u.mid)), den);
-#pragma unroll 4
-    for (int i = 0; i < n; i += SP) {
-      const int k = i + lane / LPR;
-      const float fk = __shfl(f, k & (kWave - 1));
-      if (k < n) {
-        const float4 x = v[(size_t)(s0 + k) * step * cut.R * LPR];
-        num.x = __builtin_fmaf(x.x, fk, num.x);
-        num.y = __builtin_fmaf(x.y, fk, num.y);
-        num.z = __builtin_fmaf(x.z, fk, num.z);
-        num.w = __builtin_fmaf(x.w, fk, num.w);
+    const int n = min(ns - s0, kWave);
+    for (int i0 = SP * wr; i0 < n; i0 += SP * W * U) {
+      if (s0 || i0 > SP * wr) load(s0 + i0);
+#pragma unroll
+      for (int i = 0; i < U; i++) {
+        const int k = i0 + SP * W * i + lane / LPR;
+        const float fk = __shfl(f, k & (kWave - 1));
+        if (k < n) {
+          num.x = __builtin_fmaf(x[i].x, fk, num.x);
+          num.y = __builtin_fmaf(x[i].y, fk, num.y);
+          num.z = __builtin_fmaf(x[i].z, fk, num.z);
+          num.w = __builtin_fmaf(x[i].w, fk, num.w);
+        }
       }
     }
   }
@@ -751,75 +814,19 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, c
     num.z += __shfl_xor(num.z, o);
     num.w += __shfl_xor(num.w, o);
   }
+  if constexpr (W > 1) {  // (a workgroup of W = 4 is one row: its waves stay or leave together)
+    if (lane < LPR) sh[wr][lane] = num;
+    __syncthreads();
+    if (wr) return;
+    num = sh[0][e4];
+#pragma unroll
+    for (int k = 1; k < W; k++) num = add4(num, sh[k][e4]);
+  }
   if (lane >= LPR) return;
   const float f = den == 0.0f ? 0.0f : 1.0f / den;
-  const int e = (int)((Mr - u.m) + u.mid), t = ro / G;
-  *reinterpret_cast<float4 *>(out + (size_t)(s.row0 + t) * out_stride + (kv * G + ro - t * G) * D + 4 * e4) =
+  const int e = (int)((Mr - u.m) + u.mid), t = ro / cut.G;
+  *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * cut.G + ro - t * cut.G) * D + 4 * e4) =
       make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
-}
-
-// One wave a row and head: a key per lane and round, the round's weights in LDS, then the
-// lanes own output elements.
-template <int D>
-__global__ __launch_bounds__(kWave) void kv8_attend_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
-                                                           int H, float *__restrict__ out, int out_stride,
-                                                           int rows_min) {
-  constexpr int DPL = (D + kWave - 1) / kWave;
-  __shared__ float qs[D], ps[kWave];
-  __shared__ size_t rows[kWave];
-  const int row = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, kv = h / (H / a.KV);
-  Kv8Seq s;
-  if (!kv8_find_row(a, row, s) || s.n * (H / a.KV) < rows_min) return;
-  const int cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
-  const int S = min(s.past + row - s.row0 + 1, cap);
-  for (int e = lane; e < D; e += kWave) qs[e] = q[(size_t)row * q_stride + h * D + e];
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, acc[DPL];
-#pragma unroll
-  for (int j = 0; j < DPL; j++) acc[j] = 0.0f;
-  for (int k0 = 0; k0 < S; k0 += kWave) {
-    const int key = k0 + lane;
-    const int pg = key < S ? a.table[(size_t)s.b * a.max_pages + (key >> a.page_shift)] : -1;
-    const bool in = (unsigned)pg < (unsigned)a.pages;
-    const size_t block = (size_t)(in ? pg : 0) * a.KV + kv, at = (block << a.page_shift) + (key & (page - 1));
-    float sc = -INFINITY, vs = 0.0f;
-    if (in) {
-      float d = 0.0f;
-      for (int e = 0; e < D; e += 4) {
-        const float4 k4 = e4m3x4_f32(*reinterpret_cast<const uint32_t *>(a.k + at * D + e));
-        d = __builtin_fmaf(qs[e], k4.x, d);
-        d = __builtin_fmaf(qs[e + 1], k4.y, d);
-        d = __builtin_fmaf(qs[e + 2], k4.z, d);
-        d = __builtin_fmaf(qs[e + 3], k4.w, d);
-      }
-      sc = d * e8m0_to_f32(a.ke[block]) / sqrtf((float)D);
-      vs = e8m0_to_f32(a.ve[block]);
-    }
-    const float mnew = fmaxf(m, wave_max(sc)), ref = mnew == -INFINITY ? 0.0f : mnew;
-    const float alpha = expf(m - ref), p = in ? expf(sc - ref) : 0.0f;
-    m = mnew;
-    l = __builtin_fmaf(l, alpha, wave_sum(p));
-    __syncthreads();
-    ps[lane] = in ? p * vs : 0.0f;
-    rows[lane] = in ? at : ~(size_t)0;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < DPL; j++) acc[j] *= alpha;
-    for (int i = 0; i < kWave; i++) {
-      if (rows[i] == ~(size_t)0) continue;
-#pragma unroll
-      for (int j = 0; j < DPL; j++) {
-        const int e = lane + kWave * j;
-        if (e < D)
-          acc[j] = __builtin_fmaf(ps[i], __builtin_amdgcn_cvt_f32_fp8((int)a.v[rows[i] * D + e], 0), acc[j]);
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < DPL; j++) {
-    const int e = lane + kWave * j;
-    if (e < D) out[(size_t)row * out_stride + h * D + e] = l == 0.0f ? 0.0f : acc[j] / l;
-  }
 }
 
 // ---------------------------------------------------------------- launchers
@@ -857,51 +864,83 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
 
 // ---- how a call's attention is cut
 
+// Sequences of more rows a KV head than this take row blocks of 32.
+constexpr int kKv8FewRows = 16;
+
+// One class of a call's sequences, by their rows: a launch of kv8_attend_kernel and its merge.
+struct Kv8Part {
+  Kv8Cut cut;
+  int nc = -1;  // column blocks of the kernel, -1: no such sequences
+  long long blocks = 0, units = 0;  // most row blocks a KV head, and slices of them
+  size_t sums = 0, floats = 0;      // the slices' sums, their scalars behind them
+};
 struct Kv8Plan {
-  Kv8Cut step;
-  long long step_blocks, step_units;  // most row blocks, and slices of them
-  size_t step_sums;                   // floats of the step slices' sums, their scalars behind them
+  Kv8Part few, many;
 };
 
-constexpr int kKv8StepRows = 32;  // rows of a sequence and KV head that the step kernel takes
-
+#ifndef KNW
+#define KNW 4
+#endif
+#ifndef KMIN
+#define KMIN 256
+#endif
+#ifndef KROWS
+#define KROWS 2048
+#endif
 static Kv8Plan kv8_plan(const Kv8Args &a, int D, int H) {
-  Kv8Plan p;
   const int G = H / a.KV;
   const long long most = (long long)a.max_new * G;
-  const int R = most <= 8 ? 8 : 16;
-  p.step = {G, R, 1, kKv8StepRows, std::max(1, 1024 / a.KV), 256};
-  p.step_blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
-  p.step_units = p.step_blocks + p.step.slots;
-  p.step_sums = (size_t)p.step_units * a.KV * R * D;
+  const auto part = [&](int nc, int rows_min, int rows_max, int groups) {
+    Kv8Part p;
+    const int R = kv8_rows(nc);
+    p.nc = nc;
+    p.cut = {G, R, rows_min, rows_max, std::max(1, groups / a.KV), KMIN};
+    p.blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
+    p.units = p.blocks + p.cut.slots;
+    p.sums = (size_t)p.units * a.KV * R * D;
+    p.floats = p.sums + (size_t)p.units * a.KV * R * 4;
+    return p;
+  };
+  Kv8Plan p;
+  const bool many = most > kKv8FewRows;
+  // a batch of one sequence is taken whole by the launch that its largest size calls for
+  if (!many || a.B > 1) p.few = part(most <= 8 ? 0 : 1, 1, kKv8FewRows, 1024);
+  if (many) p.many = part(2, a.B > 1 ? kKv8FewRows + 1 : 1, 0x7FFFFFFF, 512);
   return p;
 }
 
 size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H) {
   const Kv8Plan p = kv8_plan(a, D, H);
-  return (p.step_sums + (size_t)p.step_units * a.KV * p.step.R * 4) * sizeof(float);
+  return (p.few.floats + p.many.floats) * sizeof(float);
 }
 
 template <int D>
 static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, int H, float *out, int out_stride,
                                 float *work, hipStream_t s) {
-  const Kv8Plan p = kv8_plan(a, D, H);
-  const long long grid = p.step_units * a.KV, merge = (p.step_blocks * a.KV * p.step.R + 3) / 4;
-  if (grid > 0x7FFFFFFF || merge > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const auto go = [&](auto kern, int nw) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(nw * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
-                       p.step);
-  };
-  if (p.step.R == 8)
-    go(kv8_step_kernel<D, false, 4>, 4);
-  else
-    go(kv8_step_kernel<D, true, 4>, 4);
-  if ((a.max_pages << a.page_shift) > p.step.min_keys)
-    hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3((unsigned)merge), dim3(256), 0, s, a, p.step, work, p.step_sums,
-                       H / a.KV, out, out_stride);
-  if ((long long)a.max_new * (H / a.KV) > kKv8StepRows)
-    hipLaunchKernelGGL(kv8_attend_kernel<D>, dim3(a.T, H), dim3(kWave), 0, s, a, q, q_stride, H, out, out_stride,
-                       kKv8StepRows + 1);
+  const Kv8Plan plan = kv8_plan(a, D, H);
+  for (const Kv8Part *p : {&plan.many, &plan.few}) {
+    if (p->nc < 0) continue;
+    const long long grid = p->units * a.KV, rows = p->blocks * a.KV * p->cut.R;
+    if (grid > 0x7FFFFFFF || rows > 0x7FFFFFFF) return hipErrorInvalidValue;
+    const auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(KNW * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
+                         p->cut);
+    };
+    const auto merge = [&](auto kern, int w) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)((rows * w + 3) / 4)), dim3(256), 0, s, a, p->cut, work, p->sums, out,
+                         out_stride);
+    };
+    if (p->nc == 0) go(kv8_attend_kernel<D, 0, KNW>);
+    if (p->nc == 1) go(kv8_attend_kernel<D, 1, KNW>);
+    if (p->nc == 2) go(kv8_attend_kernel<D, 2, KNW>);
+    if ((a.max_pages << a.page_shift) > p->cut.min_keys) {
+      if (rows <= KROWS)
+        merge(kv8_merge_kernel<D, 4>, 4);
+      else
+        merge(kv8_merge_kernel<D, 1>, 1);
+    }
+    work += p->floats;
+  }
   return hipGetLastError();
 }
 
