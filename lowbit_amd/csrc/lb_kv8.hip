@@ -348,8 +348,10 @@ __device__ __forceinline__ v8h e4m3x8_h(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ h2v pk_half(float a, float b) {  // toward zero: lo keeps what is left
   return __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-// The other term's share of x: x - hi (exact).
-__device__ __forceinline__ float half_rest(float x, _Float16 hi) { return x - (float)hi; }
+// The other term: x - hi (exact), rounded.
+__device__ __forceinline__ _Float16 half_rest(float x, _Float16 hi) {
+  return (_Float16)__builtin_fmaf((float)hi, -1.0f, x);
+}
 
 // 2^(13 - exponent of a row's largest |q|), which brings it into [2^13, 2^14), and the inverse;
 // NaN where the row is not finite.
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const _Float16 hi = (_Float16)x[e], lo = (_Float16)half_rest(x[e], hi);
+        const _Float16 hi = (_Float16)x[e], lo = half_rest(x[e], hi);
         if constexpr (SEP) {
           qh[y][s][e] = hi;
           ql[y][s][e] = lo;
@@ -620,32 +622,46 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       }
       // ---- weights, their sum, and their two terms
       const float ref = m[y] == -INFINITY ? 0.0f : m[y];
+      const auto weights = [&](auto slow) {
 #pragma unroll
-      for (int x = 0; x < 2; x++) {
-        const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - ref;
-        const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
-        float p[4];
+        for (int x = 0; x < 2; x++) {
+          const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - ref;
+          const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
+          float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          p[e] = __builtin_fmaf(s[y][x][e], cc, off);
-          if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - ref) + kKv8WUp;
-          p[e] = __builtin_amdgcn_exp2f(p[e]);
-          // a block whose exponent is NaN counts where it is seen
-          if (edge) p[e] = s[y][x][e] == -INFINITY ? 0.0f : p[e];
-          l[y] = __builtin_fmaf(p[e], edge && p[e] == 0.0f ? 0.0f : unit_l, l[y]);
-        }
+          for (int e = 0; e < 4; e++) {
+            p[e] = __builtin_fmaf(s[y][x][e], cc, off);
+            if constexpr (slow) {
+              if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - ref) + kKv8WUp;
+              p[e] = __builtin_amdgcn_exp2f(p[e]);
+              // a block whose exponent is NaN counts where it is seen
+              const bool seen = s[y][x][e] != -INFINITY;
+              p[e] = seen ? p[e] : 0.0f;
+              l[y] = __builtin_fmaf(p[e], seen ? unit_l : 0.0f, l[y]);
+            } else {
+              p[e] = __builtin_amdgcn_exp2f(p[e]);
+              l[y] = __builtin_fmaf(p[e], unit_l, l[y]);
+            }
+          }
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const h2v hi = pk_half(p[e], p[e + 1]);
-          const h2v lo = pk_half(half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y));
-          if constexpr (SEP) {
-            ph[y][4 * x + e] = hi.x, ph[y][4 * x + e + 1] = hi.y;
-            pl[y][4 * x + e] = lo.x, pl[y][4 * x + e + 1] = lo.y;
-          } else {
-            ph[y][4 * x + e] = c < 8 ? hi.x : lo.x, ph[y][4 * x + e + 1] = c < 8 ? hi.y : lo.y;
+          for (int e = 0; e < 4; e += 2) {
+            const h2v hi = pk_half(p[e], p[e + 1]);
+            const h2v lo = {half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y)};
+            if constexpr (SEP) {
+              ph[y][4 * x + e] = hi.x, ph[y][4 * x + e + 1] = hi.y;
+              pl[y][4 * x + e] = lo.x, pl[y][4 * x + e + 1] = lo.y;
+            } else {
+              const h2v two = __builtin_bit_cast(
+                  h2v, c < 8 ? __builtin_bit_cast(uint32_t, hi) : __builtin_bit_cast(uint32_t, lo));
+              ph[y][4 * x + e] = two.x, ph[y][4 * x + e + 1] = two.y;
+            }
           }
         }
-      }
+      };
+      if (!SEP || edge || huge)
+        weights(std::true_type());
+      else
+        weights(std::false_type());
     }
     // ---- out^T += V^T W^T, two output tiles (bytes 2 b, 2 b + 1 of a V load) at a time
 #pragma unroll
@@ -745,18 +761,12 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
 // to a wave load, go round the waves, eight loads requested before the scalars are waited for.
 // Four waves where there are few rows: 118 slices of 32 rows took a wave a row 22.8 us.
 template <int D, int W>
-__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
-                                                       size_t sums, float *__restrict__ out, int out_stride) {
+__device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Cut &cut, const Kv8Unit &w, int kv, int rr,
+                                              int wr, const float *__restrict__ part, size_t sums,
+                                              float4 (*sh)[D / 4], float *__restrict__ out, int out_stride) {
   constexpr int LPR = D / 4, SP = kWave / LPR, U = 8;
-  __shared__ float4 sh[W > 1 ? W : 1][LPR];
   const int lane = threadIdx.x & (kWave - 1), e4 = lane % LPR;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wr = wave % W;
-  const int idx = (int)blockIdx.x * (4 / W) + wave / W;
-  const int rr = idx % cut.R, kv = idx / cut.R % a.KV;
-  Kv8Unit w;
-  if (!kv8_unit<true>(a, cut, idx / cut.R / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
-  if (ns < 2 || ro >= w.s.n * cut.G) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(part + sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(part) + (pu * cut.R + rr) * LPR + e4;
@@ -814,7 +824,7 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, c
     num.z += __shfl_xor(num.z, o);
     num.w += __shfl_xor(num.w, o);
   }
-  if constexpr (W > 1) {  // (a workgroup of W = 4 is one row: its waves stay or leave together)
+  if constexpr (W > 1) {  // (the workgroup is one row's)
     if (lane < LPR) sh[wr][lane] = num;
     __syncthreads();
     if (wr) return;
@@ -827,6 +837,24 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, c
   const int e = (int)((Mr - u.m) + u.mid), t = ro / cut.G;
   *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * cut.G + ro - t * cut.G) * D + 4 * e4) =
       make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
+}
+
+template <int D, int W>
+__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
+                                                       size_t sums, float *__restrict__ out, int out_stride) {
+  __shared__ float4 sh[W > 1 ? W : 1][D / 4];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int rows = W > 1 ? cut.R : 1;  // workgroups of a row block
+  const int idx = (int)blockIdx.x / rows, kv = idx % a.KV;
+  Kv8Unit w;
+  if (!kv8_unit<true>(a, cut, idx / a.KV, w) || w.slices < 2) return;
+  const int last = min(cut.R, w.s.n * cut.G - w.rb * cut.R);
+  if constexpr (W > 1) {
+    if ((int)blockIdx.x % rows < last) kv8_merge_row<D, W>(a, cut, w, kv, (int)blockIdx.x % rows, wave, part, sums, sh, out, out_stride);
+  } else {
+    for (int rr = wave; rr < last; rr += 4)
+      kv8_merge_row<D, W>(a, cut, w, kv, rr, 0, part, sums, sh, out, out_stride);
+  }
 }
 
 // ---------------------------------------------------------------- launchers
@@ -927,8 +955,8 @@ static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, 
                          p->cut);
     };
     const auto merge = [&](auto kern, int w) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)((rows * w + 3) / 4)), dim3(256), 0, s, a, p->cut, work, p->sums, out,
-                         out_stride);
+      hipLaunchKernelGGL(kern, dim3((unsigned)(w > 1 ? rows : rows / p->cut.R)), dim3(256), 0, s, a, p->cut, work,
+                         p->sums, out, out_stride);
     };
     if (p->nc == 0) go(kv8_attend_kernel<D, 0, KNW>);
     if (p->nc == 1) go(kv8_attend_kernel<D, 1, KNW>);
