@@ -275,13 +275,20 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 // the subnormals that the matrix cores flush lie 2^-28 below).
 
 constexpr float kKv8WUp = 14.0f;   // weights are scaled by 2^14
+#ifndef KHEAD
+#define KHEAD 3
+#endif
+constexpr float kKv8Head = KHEAD;
 constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
 constexpr float kKv8Log2e = 1.4426950408889634f;
 
-// How a launch cuts its rows and keys: the sequences of rows_min .. rows_max rows a KV head,
-// row blocks of R rows, about `slots` slices a KV head of at least min_keys keys.
+// How a launch cuts its rows and keys: the sequences of rows_min .. rows_max rows a KV head, row
+// blocks of R rows, their keys in slices of at least min_keys, about `slots` of them a KV head
+// where there are at most few_blocks row blocks, slots_many where there are more, and then no
+// shorter than `keep` times the mean row block's keys.
 struct Kv8Cut {
-  int G, R, rows_min, rows_max, slots, min_keys;
+  int G, R, rows_min, rows_max, min_keys, few_blocks, slots, slots_many;
+  float keep;
 };
 
 __device__ __forceinline__ int kv8_row_blocks(const Kv8Cut &c, const Kv8Seq &s) {
@@ -301,13 +308,17 @@ __device__ __forceinline__ int round_up(int v, int to) { return (v + to - 1) / t
 // the lengths differ the slices are alike, in steps of 256. (The sum in float, 1 % up: never
 // more slices than slots and row blocks together.) `first`: sequences 0 .. 63 by lane.
 __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first) {
-  float sum = (float)kv8_row_blocks(c, first) * (float)kv8_keys(a, first);
+  float blocks = (float)kv8_row_blocks(c, first), sum = blocks * (float)kv8_keys(a, first);
   for (int b0 = kWave; b0 < a.B; b0 += kWave) {
     const Kv8Seq s = kv8_seq(a, b0 + (int)(threadIdx.x & (kWave - 1)));
-    sum += (float)kv8_row_blocks(c, s) * (float)kv8_keys(a, s);
+    const float n = (float)kv8_row_blocks(c, s);
+    blocks += n;
+    sum += n * (float)kv8_keys(a, s);
   }
-  const float per = fminf(wave_sum(sum) * 1.01f / (float)c.slots, (float)kKv8MaxPos);
-  return max(c.min_keys, round_up((int)per + 1, 256));
+  blocks = fmaxf(wave_sum(blocks), 1.0f), sum = wave_sum(sum);
+  const float even = sum * 1.01f / (float)(blocks <= (float)c.few_blocks ? c.slots : c.slots_many);
+  const float per = fmaxf(even, blocks <= (float)c.few_blocks ? 0.0f : c.keep * sum / blocks);
+  return max(c.min_keys, round_up((int)fminf(per, (float)kKv8MaxPos) + 1, 256));
 }
 
 // Row block and slice of unit u; or, u a row block, that row block and the units before its
@@ -348,16 +359,18 @@ __device__ __forceinline__ v8h e4m3x8_h(uint32_t lo, uint32_t hi) {
 __device__ __forceinline__ h2v pk_half(float a, float b) {  // toward zero: lo keeps what is left
   return __builtin_bit_cast(h2v, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-// The other term: x - hi (exact), rounded.
-__device__ __forceinline__ _Float16 half_rest(float x, _Float16 hi) {
-  return (_Float16)__builtin_fmaf((float)hi, -1.0f, x);
+// The other term: x - hi (exact), rounded, in one instruction (v_fma_mixlo_f16); minus1 is -1
+// in a register that the compiler cannot see through, or it makes a conversion and two more.
+__device__ __forceinline__ _Float16 half_rest(float x, _Float16 hi, float minus1) {
+  return (_Float16)__builtin_fmaf((float)hi, minus1, x);
 }
+__device__ __forceinline__ float minus_one() { return __uint_as_float(opaque(0xBF800000u)); }
 
-// 2^(13 - exponent of a row's largest |q|), which brings it into [2^13, 2^14), and the inverse;
-// NaN where the row is not finite.
+// 2^(13 - exponent of a row's largest |q|), which brings it into [2^13, 2^14), and the inverse.
+// (An element that is not finite has a lo term of NaN, so its row's scores are NaN.)
 __device__ __forceinline__ void kv8_q_scale(int big, float &up, float &down) {
   const int e = min(267 - (big >> 23), 253);
-  up = big >= 0x7F800000 ? __builtin_nanf("") : __int_as_float(e << 23);
+  up = __int_as_float(e << 23);
   down = __int_as_float((254 - e) << 23);
 }
 
@@ -378,12 +391,17 @@ struct Kv8Unit2 {
 };
 __device__ __forceinline__ Kv8Unit2 kv8_larger(Kv8Unit2 a, Kv8Unit2 b) { return b.m - b.mid > a.m - a.mid ? b : a; }
 
+// Waits for every load of the wave. After loads on a path that is seldom taken: without it the
+// compiler waits for all loads wherever the paths have joined, the common one included.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
+
 // A tile of 16 keys as a wave holds it.
 struct Kv8Tile {
   bool held;     // there is such a page
   bool unused;   // its V codes are not to be used
   float kscale;  // 2^ke of K
   float ev;      // V's exponent
+  float unit;    // 2^(mid - ev), what a weight counts in the denominator
 };
 
 // Few query rows a sequence (steps): R = 8 rows a block, or 16 (SEP). NW waves share a slice
@@ -504,11 +522,14 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       biggest = max(biggest, wave_max_i32(t_ve == 255 ? -1 : t_ve));
     }
     load_tiles(0);
+    wait_loads();
   }
   const int least = max(biggest - kKv8Spread, 0);  // E8M0 exponents of V below count as zeros
-  const float mid = (float)(max(biggest, 0) - kKv8Spread / 2 - 127);
+  const int imid = max(biggest, 0) - kKv8Spread / 2;
+  const float mid = (float)(imid - 127);
 
   // ---- the query rows in two terms
+  const float minus1 = minus_one();
   float cx[NB];
 #pragma unroll
   for (int y = 0; y < NB; y++) {
@@ -525,13 +546,16 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       const float4 a0 = qf[y][s][0], a1 = qf[y][s][1];
       const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const _Float16 hi = (_Float16)x[e], lo = half_rest(x[e], hi);
+      for (int e = 0; e < 8; e += 2) {
+        const h2v hi = pk_half(x[e], x[e + 1]);
+        const h2v lo = {half_rest(x[e], hi.x, minus1), half_rest(x[e + 1], hi.y, minus1)};
         if constexpr (SEP) {
-          qh[y][s][e] = hi;
-          ql[y][s][e] = lo;
+          qh[y][s][e] = hi.x, qh[y][s][e + 1] = hi.y;
+          ql[y][s][e] = lo.x, ql[y][s][e + 1] = lo.y;
         } else {
-          qh[y][s][e] = c < 8 ? hi : lo;
+          const h2v two =
+              __builtin_bit_cast(h2v, c < 8 ? __builtin_bit_cast(uint32_t, hi) : __builtin_bit_cast(uint32_t, lo));
+          qh[y][s][e] = two.x, qh[y][s][e + 1] = two.y;
         }
       }
     }
@@ -546,7 +570,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
     for (int j = 0; j < VB; j++) acc[y][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   bool huge = false;  // |m| with few bits left for fractions: x has to be rounded as it was for m
-  for (int i = 0; i < chunks; i++) {
+  const auto chunk = [&](int i, auto more) {
     const int key0 = tile_key(2 * i);
     Kv8Tile now[2];
 #pragma unroll
@@ -557,27 +581,39 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       now[x].unused = ve < max(least, 1);
       now[x].kscale = e8m0_to_f32((uint32_t)ke);
       now[x].ev = ve == 255 ? __builtin_nanf("") : (float)(max(ve, least) - 127);
+      now[x].unit = __int_as_float(ve == 255 ? 0x7FC00000 : (127 + imid - max(ve, least)) << 23);
     }
     // ---- scores of 32 keys
     v4f s[NB][2];
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
+    for (int y = 0; y < NB; y++)
 #pragma unroll
-      for (int y = 0; y < NB; y++) s[y][x] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < 2; x++) s[y][x] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
+    for (int k = 0; k < KS; k++) {
+      v8h kk[2];
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
         const uint4 kw = kf[x][k >> 1];
-        const v8h kk = k & 1 ? e4m3x8_h(kw.z, kw.w) : e4m3x8_h(kw.x, kw.y);
+        kk[x] = k & 1 ? e4m3x8_h(kw.z, kw.w) : e4m3x8_h(kw.x, kw.y);
+      }
 #pragma unroll
-        for (int y = 0; y < NB; y++) {
-          s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[y][k], s[y][x], 0, 0, 0);
-          if constexpr (SEP) s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[y][k], s[y][x], 0, 0, 0);
-        }
+      for (int x = 0; x < 2; x++)
+#pragma unroll
+        for (int y = 0; y < NB; y++) s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], qh[y][k], s[y][x], 0, 0, 0);
+      if constexpr (SEP) {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int y = 0; y < NB; y++)
+            s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], ql[y][k], s[y][x], 0, 0, 0);
       }
     }
-    const bool more = i + 1 < chunks;
-    if (more) {
-      if (((2 * i + 2) & (kWave - 1)) == 0) load_tiles(2 * i + 2);
+    if constexpr (more) {
+      if (((2 * i + 2) & (kWave - 1)) == 0) {
+        load_tiles(2 * i + 2);
+        wait_loads();
+      }
       locate(2 * i + 2);
       load_k();
     }
@@ -610,7 +646,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       const float t1 = fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]));
       const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
       if (__any(top > m[y])) {
-        const float mnew = fmaxf(m[y], ceilf(quarters_max(top)));
+        const float mnew = fmaxf(m[y], ceilf(quarters_max(top)) + kKv8Head);
         const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[y] - mnew);
         m[y] = mnew;
         huge = huge || __any(fabsf(mnew) > 0x1p22f && mnew != -INFINITY);
@@ -625,8 +661,7 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
       const auto weights = [&](auto slow) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-          const float cc = x ? c1 : c0, off = now[x].ev + kKv8WUp - ref;
-          const float unit_l = __builtin_amdgcn_exp2f(mid - now[x].ev);
+          const float cc = x ? c1 : c0, off = (now[x].ev + kKv8WUp) - ref;
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
@@ -637,16 +672,16 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
               // a block whose exponent is NaN counts where it is seen
               const bool seen = s[y][x][e] != -INFINITY;
               p[e] = seen ? p[e] : 0.0f;
-              l[y] = __builtin_fmaf(p[e], seen ? unit_l : 0.0f, l[y]);
+              l[y] = __builtin_fmaf(p[e], seen ? now[x].unit : 0.0f, l[y]);
             } else {
               p[e] = __builtin_amdgcn_exp2f(p[e]);
-              l[y] = __builtin_fmaf(p[e], unit_l, l[y]);
+              l[y] = __builtin_fmaf(p[e], now[x].unit, l[y]);
             }
           }
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
             const h2v hi = pk_half(p[e], p[e + 1]);
-            const h2v lo = {half_rest(p[e], hi.x), half_rest(p[e + 1], hi.y)};
+            const h2v lo = {half_rest(p[e], hi.x, minus1), half_rest(p[e + 1], hi.y, minus1)};
             if constexpr (SEP) {
               ph[y][4 * x + e] = hi.x, ph[y][4 * x + e + 1] = hi.y;
               pl[y][4 * x + e] = lo.x, pl[y][4 * x + e + 1] = lo.y;
@@ -683,16 +718,21 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
         };
         const h2v e0 = two(z[0][0]), e1 = two(z[0][1]), e2 = two(z[1][0]), e3 = two(z[1][1]);
         const v8h vv = {e0.x, e0.y, e1.x, e1.y, e2.x, e2.y, e3.x, e3.y};
+        const int o = 2 * b + y;
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-          v4f &o = acc[n][2 * b + y];
-          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[n], o, 0, 0, 0);
-          if constexpr (SEP) o = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[n], o, 0, 0, 0);
+        for (int n = 0; n < NB; n++) acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[n], acc[n][o], 0, 0, 0);
+        if constexpr (SEP) {
+#pragma unroll
+          for (int n = 0; n < NB; n++)
+            acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[n], acc[n][o], 0, 0, 0);
         }
       }
     }
-    if (more) load_v();
-  }
+    if constexpr (more) load_v();
+  };
+  // the last chunk apart, so that every wait in the loop counts the same loads behind it
+  for (int i = 0; i + 1 < chunks; i++) chunk(i, std::true_type());
+  if (chunks) chunk(chunks - 1, std::false_type());
 
   // ---- the waves' sums, merged; element 4 VB g + VB e + j of row c is acc[.][j][e]
 #pragma unroll
@@ -719,12 +759,10 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
   __syncthreads();
   const size_t pu = (size_t)(unit - w.at + w.rb * w.slices + w.slice) * a.KV + kv;
   float *po = part + pu * R * D;
-  float4 *ps = reinterpret_cast<float4 *>(part + (size_t)gridDim.x * R * D) + pu * R;
-  for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
-    const int rr = i / (D / 4), d = 4 * (i % (D / 4)), ro = w.rb * R + rr;
-    if (ro >= rows) break;
-    float M = sm[0][rr];
-    Kv8Unit2 u = {sm[0][rr], smid[0]};
+  // a thread a row: the waves' factors, and the sums' common unit
+  for (int rr = threadIdx.x; rr < R; rr += NW * kWave) {
+    float M = sm[0][rr], den = 0.0f, f[NW];
+    Kv8Unit2 u = {M, smid[0]};
 #pragma unroll
     for (int x = 1; x < NW; x++) {
       M = fmaxf(M, sm[x][rr]);
@@ -732,26 +770,43 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : NC == 1 && D == 128 ? 3 : 
     }
     const float Mr = M == -INFINITY ? 0.0f : M;
     if (u.m == -INFINITY) u.m = 0.0f;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.0f;
 #pragma unroll
     for (int x = 0; x < NW; x++) {
-      const float f = __builtin_amdgcn_exp2f(sm[x][rr] - Mr);  // 0 for a wave without keys
+      f[x] = __builtin_amdgcn_exp2f(sm[x][rr] - Mr);  // 0 for a wave without keys
+      den = __builtin_fmaf(sl[x][rr], __builtin_amdgcn_exp2f((sm[x][rr] - u.m) - (smid[x] - u.mid)), den);
+    }
+    if (w.slices > 1) {
+      reinterpret_cast<float4 *>(part + (size_t)gridDim.x * R * D)[pu * R + rr] =
+          make_float4(M, M == -INFINITY ? M : u.m, u.mid, den);
+    } else {
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+      for (int x = 0; x < NW; x++) f[x] *= inv;
+    }
+#pragma unroll
+    for (int x = 0; x < NW; x++) sm[x][rr] = f[x];
+    sl[0][rr] = (Mr - u.m) + u.mid;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
+    const int rr = i / (D / 4), d = 4 * (i % (D / 4)), ro = w.rb * R + rr;
+    if (ro >= rows) break;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int x = 0; x < NW; x++) {
+      const float f = sm[x][rr];
       const float4 v = *reinterpret_cast<const float4 *>(&sh[x][rr][d]);
       num.x = __builtin_fmaf(v.x, f, num.x);
       num.y = __builtin_fmaf(v.y, f, num.y);
       num.z = __builtin_fmaf(v.z, f, num.z);
       num.w = __builtin_fmaf(v.w, f, num.w);
-      den = __builtin_fmaf(sl[x][rr], __builtin_amdgcn_exp2f((sm[x][rr] - u.m) - (smid[x] - u.mid)), den);
     }
     if (w.slices > 1) {
       *reinterpret_cast<float4 *>(po + rr * D + d) = num;
-      if (d == 0) ps[rr] = make_float4(M, M == -INFINITY ? M : u.m, u.mid, den);
     } else {
-      const float f = den == 0.0f ? 0.0f : 1.0f / den;
-      const int e = (int)((Mr - u.m) + u.mid), t = ro / G;
+      const int e = (int)sl[0][rr], t = ro / G;
       *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * G + ro - t * G) * D + d) =
-          make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
+          make_float4(ldexpf(num.x, e), ldexpf(num.y, e), ldexpf(num.z, e), ldexpf(num.w, e));
     }
   }
 }
@@ -899,6 +954,7 @@ constexpr int kKv8FewRows = 16;
 struct Kv8Part {
   Kv8Cut cut;
   int nc = -1;  // column blocks of the kernel, -1: no such sequences
+  int waves = 0;  // of a workgroup
   long long blocks = 0, units = 0;  // most row blocks a KV head, and slices of them
   size_t sums = 0, floats = 0;      // the slices' sums, their scalars behind them
 };
@@ -906,8 +962,26 @@ struct Kv8Plan {
   Kv8Part few, many;
 };
 
-#ifndef KNW
-#define KNW 4
+#ifndef KFB
+#define KFB 256
+#endif
+#ifndef KS1
+#define KS1 512
+#endif
+#ifndef KS2
+#define KS2 2048
+#endif
+#ifndef KFB2
+#define KFB2 384
+#endif
+#ifndef KS3
+#define KS3 1024
+#endif
+#ifndef KKEEP
+#define KKEEP 1.25f
+#endif
+#ifndef KBIG
+#define KBIG 1024
 #endif
 #ifndef KMIN
 #define KMIN 256
@@ -918,13 +992,20 @@ struct Kv8Plan {
 static Kv8Plan kv8_plan(const Kv8Args &a, int D, int H) {
   const int G = H / a.KV;
   const long long most = (long long)a.max_new * G;
-  const auto part = [&](int nc, int rows_min, int rows_max, int groups) {
+  const auto part = [&](int nc, int rows_min, int rows_max) {
     Kv8Part p;
     const int R = kv8_rows(nc);
+    const auto each = [&](int groups) { return std::max(1, groups / a.KV); };
     p.nc = nc;
-    p.cut = {G, R, rows_min, rows_max, std::max(1, groups / a.KV), KMIN};
     p.blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
-    p.units = p.blocks + p.cut.slots;
+    if (nc < 2) {
+      p.waves = 4;
+      p.cut = {G, R, rows_min, rows_max, KMIN, each(KFB), each(KS1), each(KS2), 0.0f};
+    } else {
+      p.waves = p.blocks * a.KV >= KBIG ? 2 : 4;
+      p.cut = {G, R, rows_min, rows_max, KMIN, each(KFB2), each(KS3), each(KS3), KKEEP};
+    }
+    p.units = p.blocks + std::max(p.cut.slots, p.cut.slots_many);
     p.sums = (size_t)p.units * a.KV * R * D;
     p.floats = p.sums + (size_t)p.units * a.KV * R * 4;
     return p;
@@ -932,8 +1013,8 @@ static Kv8Plan kv8_plan(const Kv8Args &a, int D, int H) {
   Kv8Plan p;
   const bool many = most > kKv8FewRows;
   // a batch of one sequence is taken whole by the launch that its largest size calls for
-  if (!many || a.B > 1) p.few = part(most <= 8 ? 0 : 1, 1, kKv8FewRows, 1024);
-  if (many) p.many = part(2, a.B > 1 ? kKv8FewRows + 1 : 1, 0x7FFFFFFF, 512);
+  if (!many || a.B > 1) p.few = part(most <= 8 ? 0 : 1, 1, kKv8FewRows);
+  if (many) p.many = part(2, a.B > 1 ? kKv8FewRows + 1 : 1, 0x7FFFFFFF);
   return p;
 }
 
@@ -950,17 +1031,18 @@ static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, 
     if (p->nc < 0) continue;
     const long long grid = p->units * a.KV, rows = p->blocks * a.KV * p->cut.R;
     if (grid > 0x7FFFFFFF || rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const auto go = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(KNW * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
+    const auto go = [&](auto kern, int nw) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(nw * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
                          p->cut);
     };
     const auto merge = [&](auto kern, int w) {
       hipLaunchKernelGGL(kern, dim3((unsigned)(w > 1 ? rows : rows / p->cut.R)), dim3(256), 0, s, a, p->cut, work,
                          p->sums, out, out_stride);
     };
-    if (p->nc == 0) go(kv8_attend_kernel<D, 0, KNW>);
-    if (p->nc == 1) go(kv8_attend_kernel<D, 1, KNW>);
-    if (p->nc == 2) go(kv8_attend_kernel<D, 2, KNW>);
+    if (p->nc == 0) go(kv8_attend_kernel<D, 0, 4>, 4);
+    if (p->nc == 1) go(kv8_attend_kernel<D, 1, 4>, 4);
+    if (p->nc == 2 && p->waves == 4) go(kv8_attend_kernel<D, 2, 4>, 4);
+    if (p->nc == 2 && p->waves == 2) go(kv8_attend_kernel<D, 2, 2>, 2);
     if ((a.max_pages << a.page_shift) > p->cut.min_keys) {
       if (rows <= KROWS)
         merge(kv8_merge_kernel<D, 4>, 4);
