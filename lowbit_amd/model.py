@@ -26,6 +26,11 @@ launch of its own); the LM head's epilogue folds the greedy argmax into a
 64-bit key that `lbd_argmax_finalize` turns into the next token. Prompts (T > 1)
 run the unfused sequence on the matrix-core GEMMs.
 
+With a paged 8-bit cache (`new_cache(.., kv="e4m3")`, KV8Cache) the rotary embedding and
+the cache write are `lbd_kv8_append` and the attention `lbd_kv8_attention`, in prompts
+and steps alike; such a cache may hold several sequences, which `forward_batch` and
+`generate_batch` run together.
+
 Same architecture and arithmetic as the reference model: RMSNorm in fp32, q/k/v
 projections concatenated along N and gate/up rows interleaved in (gate i, up i)
 pairs (quantization is per output row, so no quantized value changes), rotary embedding in the "rotate_half"
@@ -156,6 +161,93 @@ class KVCache:
         self.fused_merge = slices <= 8 and cfg.num_heads * cfg.head_dim <= 2048
 
 
+class KV8Cache:
+    """K and V of one or more sequences in pages of a shared pool, 8 bits an element (E4M3
+    codes, an E8M0 exponent for each page and KV head; lbd_kv8_* of include/lowbit_hip.h):
+    a quarter of KVCache's bytes, no bound of 16000 positions, and sequences take pages as
+    they grow. `lengths[s]` tokens of sequence s are valid. `capacity` positions a sequence;
+    `pages` in the pool (default: enough for every sequence at its capacity)."""
+
+    def __init__(self, cfg: ModelConfig, capacity: int, sequences: int = 1, page: int = 32, pages: int | None = None):
+        if capacity <= 0 or sequences <= 0 or (pages is not None and pages <= 0):
+            raise ValueError("capacity, sequences and pages must be positive")
+        if page not in (16, 32, 64, 128):
+            raise ValueError("pages hold 16, 32, 64 or 128 tokens")
+        if cfg.head_dim not in (32, 64, 128):
+            raise ValueError("the 8-bit cache takes heads of 32, 64 or 128")
+        self.capacity, self.page = int(capacity), int(page)
+        self.max_pages = -(-self.capacity // self.page)
+        self.pages = int(sequences * self.max_pages if pages is None else pages)
+        kv, d = cfg.num_kv_heads, cfg.head_dim
+        codes, exps = self.pages * kv * self.page * d, self.pages * kv
+        self.layers = []  # (lbd_kv8_pool, its buffers) of each layer; the layers share the page table
+        for _ in range(cfg.num_layers):
+            b = [_buf(codes), _buf(codes), _buf(exps), _buf(exps)]
+            self.layers.append((K.LbdKv8Pool(*(x.ptr for x in b), self.pages, self.page, kv, d), b))
+        self.lengths = np.zeros(sequences, np.int64)
+        self._held = np.zeros(sequences, np.int64)  # pages of each sequence
+        self._free = list(range(self.pages - 1, -1, -1))
+        self._table = np.full((sequences, self.max_pages), -1, np.int32)
+        self._dirty = True
+        self.table = _buf(self._table.nbytes)
+        self.past, self.q_start = _buf(4 * sequences), _buf(4 * (sequences + 1))
+        self.one = K.DeviceBuffer.from_array(np.array([0, 1], np.int32))  # q_start of a one-token step
+        self.work = _buf(16)
+
+    @property
+    def length(self) -> int:
+        """Valid tokens of a cache of one sequence."""
+        if len(self.lengths) != 1:
+            raise ValueError("a cache of several sequences has lengths, not one length")
+        return int(self.lengths[0])
+
+    @length.setter
+    def length(self, n: int):
+        if len(self.lengths) != 1:
+            raise ValueError("a cache of several sequences has lengths, not one length")
+        self.truncate(0, n)
+
+    def truncate(self, seq: int, n: int = 0):
+        """Sequence `seq` keeps its first n tokens (pages past them return to the pool)."""
+        keep = -(-int(n) // self.page)
+        if n < 0 or keep > self._held[seq]:
+            raise ValueError(f"sequence {seq} does not hold {n} tokens")
+        gone = self._table[seq, keep:self._held[seq]]
+        self._free.extend(int(p) for p in gone[::-1])
+        if len(gone):
+            gone[:] = -1
+            self._dirty = True
+        self._held[seq], self.lengths[seq] = keep, n
+
+    def reserve(self, seq: int, n: int):
+        """Pages for the first n positions of sequence `seq`."""
+        if n > self.capacity:
+            raise ValueError(f"KV cache full ({n} > {self.capacity})")
+        need, has = -(-int(n) // self.page), int(self._held[seq])
+        if need - has > len(self._free):
+            raise ValueError(f"KV cache full (no {need - has} pages left for sequence {seq})")
+        for i in range(has, need):
+            self._table[seq, i] = self._free.pop()
+            self._dirty = True
+        self._held[seq] = max(need, has)
+
+    def upload(self):
+        """The page table to the device, where it changed."""
+        if self._dirty:
+            _check(K.lib().lb_memcpy_h2d(self.table.ptr, self._table.ctypes.data, self._table.nbytes), "table upload")
+            self._dirty = False
+
+    def batch(self, q_start: int, past: int, seqs: int, max_new: int, rows: int) -> K.LbdKv8Batch:
+        """The lbd_kv8_batch of the first `seqs` sequences, with room for its attention in `work`."""
+        return K.LbdKv8Batch(q_start, past, self.table.ptr, seqs, self.max_pages, max_new, rows)
+
+    def room(self, b: K.LbdKv8Batch, heads: int):
+        """Grow `work` to what the attention of this batch takes (no call may be in flight)."""
+        need = K.lib().lbd_kv8_attention_work_bytes(C.byref(self.layers[0][0]), C.byref(b), heads)
+        if need > self.work.nbytes:
+            self.work = _buf(need)
+
+
 @dataclass
 class _Layer:
     ln1: K.DeviceBuffer
@@ -267,8 +359,17 @@ class Model:
     def linear_weight_bytes(self) -> int:
         return sum(x.nbytes for L in self.layers for x in (L.qkv, L.o, L.gate_up, L.down)) + self.lm_head.nbytes
 
-    def new_cache(self, max_len: int) -> KVCache:
-        return KVCache(self.cfg, max_len)
+    def new_cache(self, max_len: int, kv: str = "fp32", sequences: int = 1, page: int = 32,
+                  pages: int | None = None) -> "KVCache | KV8Cache":
+        """A cache of max_len positions: kv="fp32" (one sequence), or kv="e4m3", the paged 8-bit
+        cache of `sequences` sequences (KV8Cache)."""
+        if kv == "fp32":
+            if sequences != 1 or pages is not None:
+                raise ValueError("the fp32 cache holds one sequence, without pages")
+            return KVCache(self.cfg, max_len)
+        if kv != "e4m3":
+            raise ValueError(f"kv must be 'fp32' or 'e4m3', not {kv!r}")
+        return KV8Cache(self.cfg, max_len, sequences, page, pages)
 
     # ------------------------------------------------------------ one step
 
@@ -330,7 +431,10 @@ class Model:
         for li, ly in enumerate(self.layers):
             self._fused_linear(ly.qkv, x, self.qkv.ptr, norm=ly.ln1.ptr,
                                bias=None if ly.qkv_bias is None else ly.qkv_bias.ptr)
-            if cache.fused_merge:
+            if isinstance(cache, KV8Cache):
+                self._attend_kv8(cache, li, None)
+                self._fused_linear(ly.o, self.att.ptr, x, res=x)
+            elif cache.fused_merge:
                 # key slices, merged in the o projection's prologue
                 _check(L.lbd_attention_slices(self.qkv.ptr, H, KV, D, self.cos.ptr, self.sin.ptr, self.pos.ptr,
                                               cfg.max_position, cache.k[li].ptr, cache.v[li].ptr, cache.capacity,
@@ -357,10 +461,30 @@ class Model:
         else:
             self._fused_linear(self.lm_head, x, self.all_logits.ptr, norm=self.norm.ptr)
 
-    def _step(self, T: int, cache: KVCache, logits: str, argmax_hist: bool):
-        """Enqueue one forward of the T tokens in self.tok at position *pos."""
-        if T == 1 and self.fused:
-            return self._step_fused(cache, logits, argmax_hist)
+    def _attend_kv8(self, cache: KV8Cache, li: int, bias: int | None):
+        """Layer li's append of the rows in self.qkv (rotated in place) and their attention, by the
+        batch that _plan_kv8 or forward_batch left in self.batch."""
+        cfg, L, s = self.cfg, self.L, self.stream
+        H, D = cfg.num_heads, cfg.head_dim
+        width, pool, b = (H + 2 * cfg.num_kv_heads) * D, C.byref(cache.layers[li][0]), C.byref(self.batch)
+        _check(L.lbd_kv8_append(pool, b, self.qkv.ptr, width, bias, H, self.cos.ptr, self.sin.ptr, cfg.max_position,
+                                self.qkv.ptr, width, s), "kv8 append")
+        _check(L.lbd_kv8_attention(pool, b, self.qkv.ptr, width, H, self.att.ptr, H * D, cache.work.ptr,
+                                   cache.work.nbytes, s), "kv8 attention")
+
+    def _plan_kv8(self, cache, T: int):
+        """The batch of T tokens of a one-sequence 8-bit cache at position *pos."""
+        if not isinstance(cache, KV8Cache):
+            return
+        q_start = cache.one
+        if T > 1:
+            a, q_start = np.array([0, T], np.int32), cache.q_start
+            _check(self.L.lb_memcpy_h2d(q_start.ptr, a.ctypes.data, 8), "q_start upload")
+        self.batch = cache.batch(q_start.ptr, self.pos.ptr, 1, T, T)
+        cache.room(self.batch, self.cfg.num_heads)
+
+    def _layers(self, T: int, cache):
+        """The T tokens in self.tok through every layer and the last norm, into self.h."""
         cfg, L, s = self.cfg, self.L, self.stream
         h, I, H, KV, D = cfg.hidden_size, cfg.intermediate_size, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         qkvw = (H + 2 * KV) * D
@@ -368,11 +492,15 @@ class Model:
         for li, ly in enumerate(self.layers):
             _check(L.lbd_rmsnorm(self.x.ptr, ly.ln1.ptr, T, h, cfg.rms_norm_eps, self.h.ptr, s), "rmsnorm")
             self._linear(ly.qkv, self.h.ptr, T, self.qkv.ptr)
-            _check(L.lbd_qkv_rope(self.qkv.ptr, None if ly.qkv_bias is None else ly.qkv_bias.ptr, T, H, KV, D,
-                                  self.cos.ptr, self.sin.ptr, self.pos.ptr, cfg.max_position,
-                                  cache.k[li].ptr, cache.v[li].ptr, cache.capacity, s), "qkv rope")
-            _check(L.lbd_attention(self.qkv.ptr, qkvw, cache.k[li].ptr, cache.v[li].ptr, T, H, KV, D,
-                                   self.pos.ptr, cache.capacity, self.att.ptr, s), "attention")
+            bias = None if ly.qkv_bias is None else ly.qkv_bias.ptr
+            if isinstance(cache, KV8Cache):
+                self._attend_kv8(cache, li, bias)
+            else:
+                _check(L.lbd_qkv_rope(self.qkv.ptr, bias, T, H, KV, D, self.cos.ptr, self.sin.ptr, self.pos.ptr,
+                                      cfg.max_position, cache.k[li].ptr, cache.v[li].ptr, cache.capacity, s),
+                       "qkv rope")
+                _check(L.lbd_attention(self.qkv.ptr, qkvw, cache.k[li].ptr, cache.v[li].ptr, T, H, KV, D,
+                                       self.pos.ptr, cache.capacity, self.att.ptr, s), "attention")
             self._linear(ly.o, self.att.ptr, T, self.o.ptr)
             _check(L.lbd_add(self.x.ptr, self.o.ptr, T * h, s), "add")
             _check(L.lbd_rmsnorm(self.x.ptr, ly.ln2.ptr, T, h, cfg.rms_norm_eps, self.h.ptr, s), "rmsnorm")
@@ -381,6 +509,14 @@ class Model:
             self._linear(ly.down, self.m.ptr, T, self.o.ptr)
             _check(L.lbd_add(self.x.ptr, self.o.ptr, T * h, s), "add")
         _check(L.lbd_rmsnorm(self.x.ptr, self.norm.ptr, T, h, cfg.rms_norm_eps, self.h.ptr, s), "rmsnorm")
+
+    def _step(self, T: int, cache: KVCache, logits: str, argmax_hist: bool):
+        """Enqueue one forward of the T tokens in self.tok at position *pos."""
+        if T == 1 and self.fused:
+            return self._step_fused(cache, logits, argmax_hist)
+        cfg, L, s = self.cfg, self.L, self.stream
+        h = cfg.hidden_size
+        self._layers(T, cache)
         if logits == "none":
             return
         if logits == "last":
@@ -429,6 +565,10 @@ class Model:
             self._alloc(T)
             self.tok = _buf(4 * T)
         self._sync()
+        if isinstance(cache, KV8Cache):
+            cache.reserve(0, pos + T)
+            cache.upload()
+            self._plan_kv8(cache, T)
         _check(self.L.lb_memcpy_h2d(self.tok.ptr, tokens.ctypes.data, 4 * T), "token upload")
         self._set_pos(pos)
         if logits == "all":
@@ -465,12 +605,18 @@ class Model:
         self.hist = _buf(4 * (cache.capacity + 1))
         L = self.L
         self._sync()
+        if isinstance(cache, KV8Cache):  # the whole answer's pages, so that the recorded step never changes
+            cache.reserve(0, start + T + steps)
+            cache.upload()
+            self._plan_kv8(cache, T)
         _check(L.lb_memcpy_h2d(self.tok.ptr, prompt.ctypes.data, 4 * T), "token upload")
         self._set_pos(start)
         t0 = time.perf_counter()
         self._step(T, cache, "last", argmax_hist=True)
         self._sync()
         t1 = time.perf_counter()
+        if steps:
+            self._plan_kv8(cache, 1)
         if steps and graph:
             # every linear of a one-token step takes the decode kernels (M = 1),
             # which allocate nothing, so the step can be recorded
@@ -498,3 +644,68 @@ class Model:
             timings["decode_s"] = t2 - t1
             timings["decode_forwards"] = steps
         return [int(v) for v in out]
+
+    # ------------------------------------------------------------ several sequences
+
+    def forward_batch(self, tokens: list, cache: KV8Cache) -> np.ndarray:
+        """Run tokens[s] (possibly none) of each sequence s of an 8-bit cache behind what it holds:
+        prompts, chunks of prompts and single tokens in one pass. Returns the logits [S, V] of each
+        sequence's last token; rows of sequences without tokens are NaN."""
+        cfg, L = self.cfg, self.L
+        S = len(cache.lengths)
+        if not isinstance(cache, KV8Cache) or len(tokens) != S:
+            raise ValueError("forward_batch takes a KV8Cache and a list of tokens for each of its sequences")
+        rows = [self._tokens(t) if len(t) else np.zeros(0, np.int32) for t in tokens]
+        news = np.array([len(r) for r in rows])
+        T, last = int(news.sum()), int(news.max(initial=0))
+        if T == 0:
+            raise ValueError("no tokens")
+        try:
+            for i in range(S):
+                cache.reserve(i, int(cache.lengths[i] + news[i]))
+        except ValueError:
+            for i in range(S):  # what the others had taken goes back
+                cache.truncate(i, int(cache.lengths[i]))
+            raise
+        self._sync()
+        if max(T, S) > self.tmax:
+            self._alloc(max(T, S))
+            self.tok = _buf(4 * max(T, S))
+        cache.upload()
+        starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+        ends = np.where(news > 0, starts[1:] - 1, 0).astype(np.int32)
+        past, tok = cache.lengths.astype(np.int32), np.concatenate(rows).astype(np.int32)
+        for buf, a in ((cache.q_start, starts), (cache.past, past), (self.tok, tok)):
+            _check(L.lb_memcpy_h2d(buf.ptr, a.ctypes.data, a.nbytes), "batch upload")
+        self.batch = cache.batch(cache.q_start.ptr, cache.past.ptr, S, last, T)
+        cache.room(self.batch, cfg.num_heads)
+        self._layers(T, cache)
+        # the sequences' last rows, gathered, through the LM head
+        index, rows_h = K.DeviceBuffer.from_array(ends), _buf(S * cfg.hidden_size * 4)
+        out = _buf(S * cfg.vocab_size * 4)
+        _check(L.lbd_embed(self.h.ptr, T, cfg.hidden_size, index.ptr, S, rows_h.ptr, self.stream), "row gather")
+        self._linear(self.lm_head, rows_h.ptr, S, out.ptr)
+        self._sync()
+        cache.lengths += news
+        y = out.to_array((S, cfg.vocab_size), np.float32)
+        y[news == 0] = np.nan
+        return y
+
+    def generate_batch(self, prompts: list, n_new: int, cache: KV8Cache | None = None) -> list[list[int]]:
+        """Greedy decoding of several prompts together: all prompts in one pass, then one token of
+        every sequence a pass (the argmax on the host)."""
+        if not len(prompts) or not all(len(p) for p in prompts):
+            raise ValueError("no tokens")
+        if n_new <= 0:
+            return [[] for _ in prompts]
+        if cache is None:
+            cache = self.new_cache(max(len(p) for p in prompts) + n_new, kv="e4m3", sequences=len(prompts))
+        out = [[] for _ in prompts]
+        y = self.forward_batch(list(prompts), cache)
+        for i in range(n_new):
+            tok = y.argmax(1)
+            for o, v in zip(out, tok):
+                o.append(int(v))
+            if i + 1 < n_new:
+                y = self.forward_batch([[int(v)] for v in tok], cache)
+        return out

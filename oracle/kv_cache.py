@@ -122,20 +122,23 @@ class Pool:
             safe = np.where((pgs >= 0) & (pgs < self.pages), pgs, 0)
             k, v = (np.moveaxis(self.values(c[safe], e[safe]), 1, 0).reshape(kv, -1, d)[:, :last]
                     for c, e in ((self.k, self.ke), (self.v, self.ve)))
-            for i in range(n):
-                row = int(q_start[b]) + i
-                see = np.flatnonzero(held & (np.arange(last) <= past[b] + i))
-                for h in range(heads):
-                    o = out[row, h * d:(h + 1) * d]
-                    if not len(see):
-                        o[:] = 0
-                        continue
-                    x = q[row, h * d:(h + 1) * d].astype(np.float64)
-                    kk, vv = k[h // g][see], v[h // g][see]
-                    with np.errstate(invalid="ignore"):
-                        s = kk @ x / np.sqrt(d)
-                        p = np.exp(s - s.max())
-                        p /= p.sum()
-                        o[:] = p @ vv
-                        mags[row, h] = (np.abs(kk) @ np.abs(x)).max() / np.sqrt(d), (p @ np.abs(vv)).max(), len(see)
+            rows = slice(int(q_start[b]), int(q_start[b]) + n)
+            see = held & (np.arange(last) <= past[b] + np.arange(n)[:, None])
+            some = see.any(1)
+            for h in range(heads):
+                x = q[rows, h * d:(h + 1) * d].astype(np.float64)
+                kk, vv = k[h // g], v[h // g]
+                # what no row of the sequence sees, or one of them only, must not reach the others
+                kk, vv = (np.where(see.any(0)[:, None], a, 0) for a in (kk, vv))
+                bad = np.isnan(vv).any(1)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    s = np.where(see, x @ kk.T / np.sqrt(d), -np.inf)
+                    p = np.exp(s - np.where(some, np.where(np.isnan(s), -np.inf, s).max(1), 0)[:, None])
+                    p /= np.where(some, p.sum(1), 1)[:, None]
+                    w = p @ np.where(bad[:, None], 0, vv)
+                    w[(see & bad).any(1)] = np.nan
+                    size = np.where(see, np.abs(x) @ np.abs(np.where(np.isnan(kk), 0, kk)).T, 0).max(1) / np.sqrt(d)
+                    mean = (p @ np.abs(np.where(bad[:, None], 0, vv))).max(1)
+                out[rows, h * d:(h + 1) * d] = np.where(some[:, None], w, 0)
+                mags[rows, h] = np.stack([size, mean, see.sum(1)], 1)
         return mags

@@ -326,6 +326,21 @@ def test_attention_many_sequences(rng):
     run_attention(rng, 32, 16, 2, 4, [(p, min(n, 1)) for p, n in seqs])
 
 
+@pytest.mark.parametrize("D,KV,H,seqs", [
+    # few rows: 157 slices of a row, merged a workgroup a row (more slices than lanes)
+    (32, 1, 2, [(40000, 1)]), (128, 1, 5, [(40000, 1)]),
+    # and 40 sequences of several slices, merged a row to D / 4 lanes
+    (32, 8, 16, [(300 + 27 * i, 1) for i in range(40)]), (64, 8, 8, [(300 + 27 * i, 1) for i in range(40)]),
+    (128, 8, 8, [(1100 - 20 * i, 1) for i in range(40)]),
+    # many rows: 68 row blocks in 9 and more slices; row blocks enough for workgroups of two waves,
+    # with a sequence long enough to be cut beside them
+    (64, 1, 24, [(4000, 90)]), (32, 1, 24, [(4000, 90)]),
+    (128, 8, 56, [(0, 500), (3000, 20)]), (64, 8, 64, [(0, 700), (2500, 20), (5, 90)]),
+    (32, 8, 64, [(0, 950), (2500, 80)])], ids=str)
+def test_attention_slices(rng, D, KV, H, seqs):
+    run_attention(rng, D, 32, KV, H, seqs)
+
+
 def test_attention_prompts_and_steps(rng):
     run_attention(rng, 64, 32, 2, 8, [(700, 1), (0, 90), (1300, 1), (33, 2), (0, 1), (250, 40), (64, 0)])
 
@@ -405,6 +420,77 @@ def test_attention_query_sizes(rng, scale, n):
         check(got, ref, mags, D, H)
     else:
         assert np.abs(got - ref).max() <= 2.0 ** -19 * np.abs(ref).max()
+
+
+def test_rows_before_the_first_sequence_and_positions_past_the_table(rng):
+    """q_start may begin behind row 0; a token past the table's last position is not written and
+    attends over all of it."""
+    D, page, KV, H = 64, 16, 2, 6
+    q_start, past, T = np.array([3, 8, 8, 30]), np.array([44, 3, 40]), 33
+    table = np.array([[5, 1, 7], [2, -1, -1], [0, 3, 6]], np.int32)
+    pool = cached(rng, 8, page, KV, D, table, [(44, 4), (3, 0), (40, 8)])
+    qkv = rng.standard_normal((T, (H + 2 * KV) * D)).astype(np.float32)
+    cos, sin = angles(rng, 50, D)
+    dev, want, q = Device(pool, q_start, past, table, 22, T), pool.copy(), np.full((T, H * D), FILL)
+    got = dev.append(qkv, None, H, cos, sin, q)
+    want.append(q_start, past, table, 22, qkv, None, H, cos, sin, q)
+    assert np.array_equal(got, q)
+    same_pool(dev.held(), want)
+    out, ref = dev.attention(got, H, H * D), np.full((T, H * D), FILL, np.float64)
+    mags = want.attention(q_start, past, table, 22, got, H, ref)
+    check(out, ref, mags, D, H)
+
+
+def test_pool_past_four_gib(rng):
+    """Pages whose codes lie past 2^32 bytes: the same as in a small pool."""
+    D, page, KV, H, far = 128, 128, 8, 16, 33000  # 131072 code bytes a page
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    seqs = [(0, 140), (0, 3)]
+    small = np.array([[1, 3], [0, -1]], np.int32)
+    big = np.where(small >= 0, far - 4 + small, -1).astype(np.int32)
+    q_start, past, T = np.array([0, 140, 143]), np.array([0, 0]), 143
+    qkv = rng.standard_normal((T, (H + 2 * KV) * D)).astype(np.float32)
+    cos, sin = angles(rng, 140, D)
+    pool = O.Pool(rng, 4, page, KV, D)
+    near = Device(pool, q_start, past, small, 140, T)
+    q = near.append(qkv, None, H, cos, sin, np.full((T, H * D), FILL))
+    want = near.attention(q, H, H * D)
+    buf = [K.DeviceBuffer(far * KV * n) for n in (page * D, page * D, 1, 1)]
+    assert buf[0].nbytes > 1 << 32
+    dev = Device(pool, q_start, past, big, 140, T)
+    dev.pool = K.LbdKv8Pool(*(b.ptr for b in buf), far, page, KV, D)
+    assert np.array_equal(dev.append(qkv, None, H, cos, sin, np.full((T, H * D), FILL)), q)
+    assert np.array_equal(dev.attention(q, H, H * D), want)
+    # one more token each, few rows
+    for d in (near, dev):
+        d.arrays[:2] = [up(np.array(a, np.int32)) for a in ([0, 1, 2], [140, 3])]
+        d.batch = K.LbdKv8Batch(*(a.ptr for a in d.arrays), 2, 2, 1, 2)
+    step = qkv[:2].copy()
+    q1, q2 = (d.append(step, None, H, cos, sin, np.full((2, H * D), FILL)) for d in (near, dev))
+    assert np.array_equal(q1, q2) and np.array_equal(near.attention(q1, H, H * D), dev.attention(q1, H, H * D))
+    ok(L.lb_dev_synchronize())
+
+
+def test_one_workspace_for_calls_of_all_sizes(rng):
+    """Calls in stream order share a workspace that is the largest of theirs."""
+    D, page, KV, H = 64, 32, 2, 8
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    runs = []
+    for seqs in ([(3000, 1), (5, 1)], [(700, 90), (0, 40)], [(1200, 1)] * 9, [(4000, 3)]):
+        pages, q_start, past, table, T = batch_of(rng, page, seqs)
+        pool = cached(rng, pages, page, KV, D, table, seqs)
+        q = rng.standard_normal((T, H * D)).astype(np.float32)
+        dev = Device(pool, q_start, past, table, max(n for _, n in seqs), T)
+        runs.append((dev, up(q), up(np.full((T, H * D), FILL)), dev.attention(q, H, H * D), T))
+    need = max(L.lbd_kv8_attention_work_bytes(C.byref(d.pool), C.byref(d.batch), H) for d, *_ in runs)
+    ws = K.DeviceBuffer(need)
+    for _ in range(2):
+        for dev, dq, do, _, T in runs:
+            ok(L.lbd_kv8_attention(C.byref(dev.pool), C.byref(dev.batch), dq.ptr, H * D, H, do.ptr, H * D, ws.ptr, need,
+                                   None))
+    ok(L.lb_dev_synchronize())
+    for _, _, do, want, T in runs:
+        assert np.array_equal(do.to_array((T, H * D), np.float32), want)
 
 
 def test_runs_of_append_and_attention(rng):
