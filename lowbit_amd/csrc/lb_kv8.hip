@@ -290,6 +290,15 @@ struct Kv8Cut {
   float fits;                        // many rows: workgroups a KV head that the device holds at once, else 0
 };
 
+// One class of a call's sequences, by their rows, and where its slices' sums lie in the workspace:
+// `sums` floats of them from `at` on, their scalars behind. Of a KV head at most `blocks` row
+// blocks and `units` slices. merge: workgroups a row block of the second launch, 0: one a row.
+struct Kv8Part {
+  Kv8Cut cut;
+  int blocks, units, merge;
+  size_t at, sums;
+};
+
 // r / G for 0 <= r < 2^32 / 2: the product is at most one too large.
 __device__ __forceinline__ int kv8_token(const Kv8Cut &c, int r) {
   if (c.G == 1) return r;
@@ -455,19 +464,23 @@ struct Kv8Tile {
 // once the scores are made, its V once the outputs are: loads are always in flight, and no
 // LDS lies between them and the matrix cores.
 template <int D, int NC, int NW>
-__global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 4) void kv8_attend_kernel(Kv8Args a, const float *__restrict__ q, int q_stride,
-                                                               int H, float *__restrict__ out, int out_stride,
-                                                               float *__restrict__ part, size_t sums, Kv8Cut cut) {
+struct Kv8Lds {
+  float sh[NW][kv8_rows(NC)][D + 4];
+  float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
+};
+
+template <int D, int NC, int NW>
+__device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, int kv, int unit,
+                                           const float *__restrict__ q, int q_stride, float *__restrict__ out,
+                                           int out_stride, float *__restrict__ work, Kv8Lds<D, NC, NW> &lds) {
   constexpr bool SEP = NC > 0;
   constexpr int NB = SEP ? NC : 1, R = kv8_rows(NC), KS = D / 32, CK = 32;
   constexpr int KB = D >= 64 ? 16 : 8, KL = D / (4 * KB);  // bytes of a K load, loads per lane and tile
   constexpr int VB = D / 16;                               // bytes of a V load (a key's)
-  constexpr int PS = D + 4;
-  __shared__ float sh[NW][R][PS];
-  __shared__ float sm[NW][R], sl[NW][R], smid[NW];
+  const Kv8Cut &cut = pt.cut;
+  float *part = work + pt.at;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;
-  const int kv = blockIdx.x, unit = (int)(blockIdx.y + blockIdx.z * kKv8GridY);
   Kv8Unit w;
   if (!kv8_unit<false>(a, cut, unit, w)) return;
   const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
@@ -786,35 +799,35 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 
 #pragma unroll
       for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int j = 0; j < VB; j++) sh[wave][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
+        for (int j = 0; j < VB; j++) lds.sh[wave][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
       if (g == 0) {
-        sm[wave][16 * y + c] = m[y];
-        sl[wave][16 * y + c] = l[y];
+        lds.sm[wave][16 * y + c] = m[y];
+        lds.sl[wave][16 * y + c] = l[y];
       }
     }
   }
-  if (lane == 0) smid[wave] = mid;
+  if (lane == 0) lds.smid[wave] = mid;
   __syncthreads();
   const size_t pu = (size_t)(unit - w.at + w.rb * w.slices + w.slice) * a.KV + kv;
   float *po = part + pu * R * D;
   // a thread a row: the waves' factors, and the sums' common unit
   for (int rr = threadIdx.x; rr < R; rr += NW * kWave) {
-    float M = sm[0][rr], den = 0.0f, f[NW];
-    Kv8Unit2 u = {M, smid[0]};
+    float M = lds.sm[0][rr], den = 0.0f, f[NW];
+    Kv8Unit2 u = {M, lds.smid[0]};
 #pragma unroll
     for (int x = 1; x < NW; x++) {
-      M = fmaxf(M, sm[x][rr]);
-      u = kv8_larger(u, {sm[x][rr], smid[x]});
+      M = fmaxf(M, lds.sm[x][rr]);
+      u = kv8_larger(u, {lds.sm[x][rr], lds.smid[x]});
     }
     const float Mr = M == -INFINITY ? 0.0f : M;
     if (u.m == -INFINITY) u.m = 0.0f;
 #pragma unroll
     for (int x = 0; x < NW; x++) {
-      f[x] = __builtin_amdgcn_exp2f(sm[x][rr] - Mr);  // 0 for a wave without keys
-      den = __builtin_fmaf(sl[x][rr], __builtin_amdgcn_exp2f((sm[x][rr] - u.m) - (smid[x] - u.mid)), den);
+      f[x] = __builtin_amdgcn_exp2f(lds.sm[x][rr] - Mr);  // 0 for a wave without keys
+      den = __builtin_fmaf(lds.sl[x][rr], __builtin_amdgcn_exp2f((lds.sm[x][rr] - u.m) - (lds.smid[x] - u.mid)), den);
     }
     if (w.slices > 1) {
-      reinterpret_cast<float4 *>(part + sums)[pu * R + rr] =
+      reinterpret_cast<float4 *>(part + pt.sums)[pu * R + rr] =
           make_float4(M, M == -INFINITY ? M : u.m, u.mid, den);
     } else {
       const float inv = den == 0.0f ? 0.0f : 1.0f / den;
@@ -822,8 +835,8 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 
       for (int x = 0; x < NW; x++) f[x] *= inv;
     }
 #pragma unroll
-    for (int x = 0; x < NW; x++) sm[x][rr] = f[x];
-    sl[0][rr] = (Mr - u.m) + u.mid;
+    for (int x = 0; x < NW; x++) lds.sm[x][rr] = f[x];
+    lds.sl[0][rr] = (Mr - u.m) + u.mid;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
@@ -832,8 +845,8 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int x = 0; x < NW; x++) {
-      const float f = sm[x][rr];
-      const float4 v = *reinterpret_cast<const float4 *>(&sh[x][rr][d]);
+      const float f = lds.sm[x][rr];
+      const float4 v = *reinterpret_cast<const float4 *>(&lds.sh[x][rr][d]);
       num.x = __builtin_fmaf(v.x, f, num.x);
       num.y = __builtin_fmaf(v.y, f, num.y);
       num.z = __builtin_fmaf(v.z, f, num.z);
@@ -842,11 +855,35 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 
     if (w.slices > 1) {
       *reinterpret_cast<float4 *>(po + rr * D + d) = num;
     } else {
-      const int e = (int)sl[0][rr], t = kv8_token(cut, ro);
+      const int e = (int)lds.sl[0][rr], t = kv8_token(cut, ro);
       *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * G + ro - t * G) * D + d) =
           make_float4(ldexpf(num.x, e), ldexpf(num.y, e), ldexpf(num.z, e), ldexpf(num.w, e));
     }
   }
+}
+
+// One class of sequences, or (MIXED) two in one launch, of many rows (NC = 2) and then of few
+// (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
+// (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
+// other 57 us, one of each 45; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
+template <int D, int NC, int NW, bool MIXED>
+__global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 ? 3 : 4) void kv8_attend_kernel(
+    Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
+    int out_stride, float *__restrict__ work) {
+  union Lds {
+    Kv8Lds<D, NC, NW> one;
+    Kv8Lds<D, 1, NW> few;
+  };
+  __shared__ Lds lds;
+  const int kv = blockIdx.x;
+  const int unit = (int)(blockIdx.y + blockIdx.z * kKv8GridY);
+  if constexpr (MIXED) {
+    if (unit >= p0.units) {
+      kv8_attend<D, 1, NW>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
+      return;
+    }
+  }
+  kv8_attend<D, NC, NW>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
 }
 
 // Partial sums of a row block's slices -> out, two ways: few rows of many slices, many rows of few.
@@ -856,20 +893,21 @@ __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 && NW == 4 ? 3 : 
 // eight loads requested before the scalars are waited for (118 slices of 32 rows: a wave a row
 // took 22.8 us, this 6.4).
 template <int D>
-__global__ __launch_bounds__(256) void kv8_merge_long_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
-                                                            size_t sums, float *__restrict__ out, int out_stride) {
+__device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &pt, int block,
+                                               const float *__restrict__ work, float4 (*sh)[D / 4],
+                                               float *__restrict__ out, int out_stride) {
   constexpr int W = 4, LPR = D / 4, SP = kWave / LPR, U = 8;
-  __shared__ float4 sh[W][LPR];
+  const Kv8Cut &cut = pt.cut;
   const int lane = threadIdx.x & (kWave - 1), e4 = lane % LPR;
   const int wr = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int rr = (int)blockIdx.x % cut.R, idx = (int)blockIdx.x / cut.R, kv = idx % a.KV;
+  const int rr = block % cut.R, idx = block / cut.R, kv = idx % a.KV;
   Kv8Unit w;
   if (!kv8_unit<true>(a, cut, idx / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
   if (ns < 2 || ro >= w.s.n * cut.G) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
-  const float4 *sc = reinterpret_cast<const float4 *>(part + sums) + pu * cut.R + rr;
-  const float4 *v = reinterpret_cast<const float4 *>(part) + (pu * cut.R + rr) * LPR + e4;
+  const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
+  const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
   const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
   float4 x[U];
   const auto load = [&](int i0) {  // this wave's next slices, past the last the last again
@@ -941,14 +979,15 @@ __global__ __launch_bounds__(256) void kv8_merge_long_kernel(Kv8Args a, Kv8Cut c
 // block. Eight slices at a time, all of their loads in flight together and nothing exchanged
 // between lanes (200 rows of 8200 keys in five slices, 32 heads: 13.9 us a wave a row, 6.3 so).
 template <int D>
-__device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Cut &cut, const Kv8Unit &w, int kv, int rr,
-                                              const float *__restrict__ part, size_t sums, float *__restrict__ out,
+__device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &pt, const Kv8Unit &w, int kv, int rr,
+                                              const float *__restrict__ work, float *__restrict__ out,
                                               int out_stride) {
+  const Kv8Cut &cut = pt.cut;
   constexpr int LPR = D / 4, U = 8;
   const int e4 = threadIdx.x % LPR, ns = w.slices, ro = w.rb * cut.R + rr;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
-  const float4 *sc = reinterpret_cast<const float4 *>(part + sums) + pu * cut.R + rr;
-  const float4 *v = reinterpret_cast<const float4 *>(part) + (pu * cut.R + rr) * LPR + e4;
+  const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
+  const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
   float M = -INFINITY, den = 0.0f;
   Kv8Unit2 u = {-INFINITY, 0.0f};
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -990,16 +1029,35 @@ __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Cut &cu
 }
 
 template <int D>
-__global__ __launch_bounds__(256) void kv8_merge_wide_kernel(Kv8Args a, Kv8Cut cut, const float *__restrict__ part,
-                                                            size_t sums, int groups, float *__restrict__ out,
-                                                            int out_stride) {
-  constexpr int LPR = D / 4, ROWS = 256 / LPR;
-  const int idx = (int)blockIdx.x / groups, kv = idx % a.KV;
+__device__ __forceinline__ void kv8_merge(const Kv8Args &a, const Kv8Part &pt, int block,
+                                          const float *__restrict__ work, float4 (*sh)[D / 4],
+                                          float *__restrict__ out, int out_stride) {
+  constexpr int ROWS = 1024 / D;
+  if (!pt.merge) {
+    kv8_merge_long<D>(a, pt, block, work, sh, out, out_stride);
+    return;
+  }
+  const int idx = block / pt.merge, kv = idx % a.KV;
   Kv8Unit w;
-  if (!kv8_unit<true>(a, cut, idx / a.KV, w) || w.slices < 2) return;
-  const int rows = min(cut.R, w.s.n * cut.G - w.rb * cut.R);
-  for (int rr = (int)blockIdx.x % groups * ROWS + threadIdx.x / LPR; rr < rows; rr += groups * ROWS)
-    kv8_merge_row<D>(a, cut, w, kv, rr, part, sums, out, out_stride);
+  if (!kv8_unit<true>(a, pt.cut, idx / a.KV, w) || w.slices < 2) return;
+  const int rows = min(pt.cut.R, w.s.n * pt.cut.G - w.rb * pt.cut.R);
+  for (int rr = block % pt.merge * ROWS + threadIdx.x / (D / 4); rr < rows; rr += pt.merge * ROWS)
+    kv8_merge_row<D>(a, pt, w, kv, rr, work, out, out_stride);
+}
+
+template <int D, bool MIXED>
+__global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Part p0, Kv8Part p1, int blocks0,
+                                                        const float *__restrict__ work, float *__restrict__ out,
+                                                        int out_stride) {
+  __shared__ float4 sh[4][D / 4];
+  const int block = blockIdx.x;
+  if constexpr (MIXED) {
+    if (block >= blocks0) {
+      kv8_merge<D>(a, p1, block - blocks0, work, sh, out, out_stride);
+      return;
+    }
+  }
+  kv8_merge<D>(a, p0, block, work, sh, out, out_stride);
 }
 
 // ---------------------------------------------------------------- launchers
@@ -1040,86 +1098,85 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
 // Sequences of more rows a KV head than this take row blocks of 32.
 constexpr int kKv8FewRows = 16;
 
-// One class of a call's sequences, by their rows: a launch of kv8_attend_kernel and its merge.
-struct Kv8Part {
-  Kv8Cut cut;
-  int nc = -1;  // column blocks of the kernel, -1: no such sequences
-  int waves = 0;  // of a workgroup
-  long long blocks = 0, units = 0;  // most row blocks a KV head, and slices of them
-  size_t sums = 0, floats = 0;      // the slices' sums, their scalars behind them
-};
 struct Kv8Plan {
-  Kv8Part few, many;
+  Kv8Part p[2];  // the call's classes: with both, many rows first
+  int parts, nc, waves;  // column blocks of the first one's kernel, waves of a workgroup
+  size_t floats;         // of the workspace
 };
 
-static Kv8Plan kv8_plan(const Kv8Args &a, int D, int H) {
+// false: the grid would not hold it.
+static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
   const int G = H / a.KV, cap = a.max_pages << a.page_shift;
   const long long most = (long long)a.max_new * G;
   const unsigned g_inv = (unsigned)(((1ull << 32) + G - 1) / G);  // (G = 1: not used)
-  const auto part = [&](int nc, int rows_min, int rows_max) {
-    Kv8Part p;
+  const auto each = [&](int groups) { return std::max(1, groups / a.KV); };
+  const bool many = most > kKv8FewRows;
+  plan = {};
+  const auto add = [&](int nc, int rows_min, int rows_max) {
+    Kv8Part &p = plan.p[plan.parts];
     const int R = kv8_rows(nc);
-    const auto each = [&](int groups) { return std::max(1, groups / a.KV); };
-    p.nc = nc;
-    p.blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
+    long long blocks;
     if (nc < 2) {
-      p.blocks = std::min(a.B, a.T);  // a row block each
-      p.waves = 4;
-      p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(2048), 0.0f};
+      blocks = std::min(a.B, a.T);  // a row block each
+      p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f};
     } else {
+      blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
       const int res = 256 * (D == 128 ? 2 : D == 64 ? 3 : 4);  // workgroups of four waves that the device holds
-      p.waves = p.blocks * a.KV >= 2 * res ? 2 : 4;
-      const int fits = res * 4 / p.waves;
+      // two waves a workgroup where there are enough of them: a row's query is laid out by half as
+      // many waves, and each sees more keys (2048 tokens of 32 heads on 8 98 -> 91 us)
+      if (blocks * a.KV >= 2 * res) plan.waves = 2;
+      const int fits = plan.waves == 2 ? 2 * res : res;
       p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), (float)fits / (float)a.KV};
     }
-    p.units = p.blocks + p.cut.slots;
-    p.sums = (size_t)p.units * a.KV * R * D;
-    p.floats = p.sums + (size_t)p.units * a.KV * R * 4;
-    return p;
+    const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
+    if (units > 1 << 29 || rows > 1 << 29) return false;
+    p.blocks = (int)blocks;
+    p.units = (int)units;
+    // few rows of many slices: a workgroup a row; many: 1024 / D rows at a time
+    p.merge = rows <= 2048 ? 0 : blocks * a.KV >= 1024 ? 1 : std::max(1, R * D / 1024);
+    p.at = plan.floats;
+    p.sums = (size_t)units * a.KV * R * D;
+    plan.floats += p.sums + (size_t)units * a.KV * R * 4;
+    plan.parts++;
+    return true;
   };
-  Kv8Plan p;
-  const bool many = most > kKv8FewRows;
-  // a batch of one sequence is taken whole by the launch that its largest size calls for
-  if (!many || a.B > 1) p.few = part(most <= 8 ? 0 : 1, 1, kKv8FewRows);
-  if (many) p.many = part(2, a.B > 1 ? kKv8FewRows + 1 : 1, 0x7FFFFFFF);
-  return p;
+  plan.waves = 4;
+  plan.nc = many ? 2 : most > 8 ? 1 : 0;
+  // a batch of one sequence is taken whole by the kernel that its largest size calls for
+  if (!many) return add(plan.nc, 1, kKv8FewRows);
+  return add(2, a.B > 1 ? kKv8FewRows + 1 : 1, 0x7FFFFFFF) && (a.B == 1 || add(1, 1, kKv8FewRows));
 }
 
 size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H) {
-  const Kv8Plan p = kv8_plan(a, D, H);
-  return (p.few.floats + p.many.floats) * sizeof(float);
+  Kv8Plan p;
+  return kv8_plan(a, D, H, p) ? p.floats * sizeof(float) : 0;
 }
 
 template <int D>
 static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, int H, float *out, int out_stride,
                                 float *work, hipStream_t s) {
-  const Kv8Plan plan = kv8_plan(a, D, H);
-  for (const Kv8Part *p : {&plan.many, &plan.few}) {
-    if (p->nc < 0) continue;
-    const long long rows = p->blocks * a.KV * p->cut.R, deep = (p->units + kKv8GridY - 1) / kKv8GridY;
-    if (deep > 65535 || rows > 0x7FFFFFFF) return hipErrorInvalidValue;
-    const dim3 grid(a.KV, (unsigned)std::min<long long>(p->units, kKv8GridY), (unsigned)deep);
-    const auto go = [&](auto kern, int nw) {
-      hipLaunchKernelGGL(kern, grid, dim3(nw * kWave), 0, s, a, q, q_stride, H, out, out_stride, work,
-                         p->sums, p->cut);
-    };
-    if (p->nc == 0) go(kv8_attend_kernel<D, 0, 4>, 4);
-    if (p->nc == 1) go(kv8_attend_kernel<D, 1, 4>, 4);
-    if (p->nc == 2 && p->waves == 4) go(kv8_attend_kernel<D, 2, 4>, 4);
-    if (p->nc == 2 && p->waves == 2) go(kv8_attend_kernel<D, 2, 2>, 2);
-    if ((a.max_pages << a.page_shift) > p->cut.min_keys) {
-      if (rows <= 2048) {
-        hipLaunchKernelGGL(kv8_merge_long_kernel<D>, dim3((unsigned)rows), dim3(256), 0, s, a, p->cut, work, p->sums,
-                           out, out_stride);
-      } else {
-        const long long blocks = p->blocks * a.KV;
-        const int per = 1024 / D, groups = blocks >= 1024 ? 1 : (p->cut.R + per - 1) / per;
-        hipLaunchKernelGGL(kv8_merge_wide_kernel<D>, dim3((unsigned)(blocks * groups)), dim3(256), 0, s, a, p->cut,
-                           work, p->sums, groups, out, out_stride);
-      }
-    }
-    work += p->floats;
-  }
+  Kv8Plan plan;
+  if (!kv8_plan(a, D, H, plan)) return hipErrorInvalidValue;
+  const Kv8Part &p0 = plan.p[0], &p1 = plan.p[1];
+  const int units = p0.units + p1.units;
+  const dim3 grid(a.KV, std::min(units, kKv8GridY), (units + kKv8GridY - 1) / kKv8GridY);
+  const auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, grid, dim3(plan.waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
+  };
+  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, 4, false>);
+  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, 4, false>);
+  if (plan.nc == 2 && plan.waves == 4)
+    plan.parts == 1 ? go(kv8_attend_kernel<D, 2, 4, false>) : go(kv8_attend_kernel<D, 2, 4, true>);
+  if (plan.nc == 2 && plan.waves == 2)
+    plan.parts == 1 ? go(kv8_attend_kernel<D, 2, 2, false>) : go(kv8_attend_kernel<D, 2, 2, true>);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || (a.max_pages << a.page_shift) <= p0.cut.min_keys) return e;
+  const auto groups = [&](const Kv8Part &p) { return p.blocks * a.KV * (p.merge ? p.merge : p.cut.R); };
+  const auto merge = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(groups(p0) + groups(p1)), dim3(256), 0, s, a, p0, p1, groups(p0), work, out,
+                       out_stride);
+  };
+  plan.parts == 1 ? merge(kv8_merge_kernel<D, false>) : merge(kv8_merge_kernel<D, true>);
   return hipGetLastError();
 }
 
