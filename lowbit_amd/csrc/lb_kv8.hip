@@ -916,11 +916,15 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   };
   float M = -INFINITY;
   Kv8Unit2 u = {-INFINITY, 0.0f};
-  float4 my = lane < ns ? sc[(size_t)lane * step] : none;
+  float4 my = none;  // (conditional loads, not a choice between addresses)
+  if (lane < ns) my = sc[(size_t)lane * step];
   load(SP * wr);
   const float4 head = my;
   for (int s0 = 0; s0 < ns; s0 += kWave) {
-    if (s0) my = s0 + lane < ns ? sc[(size_t)(s0 + lane) * step] : none;
+    if (s0) {
+      my = none;
+      if (s0 + lane < ns) my = sc[(size_t)(s0 + lane) * step];
+    }
     M = fmaxf(M, my.x);
     u = kv8_larger(u, {my.y, my.z});
   }
@@ -935,7 +939,10 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   float den = 0.0f;
   my = head;
   for (int s0 = 0; s0 < ns; s0 += kWave) {  // 64 slices' scalars in the lanes
-    if (s0) my = s0 + lane < ns ? sc[(size_t)(s0 + lane) * step] : none;
+    if (s0) {
+      my = none;
+      if (s0 + lane < ns) my = sc[(size_t)(s0 + lane) * step];
+    }
     const float f = __builtin_amdgcn_exp2f(my.x - Mr);  // 0 for a slice without keys, and past the last
     den = __builtin_fmaf(my.w, __builtin_amdgcn_exp2f((my.y - u.m) - (my.z - u.mid)), den);
     const int n = min(ns - s0, kWave);
@@ -995,9 +1002,12 @@ __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &p
     float4 my[U], x[U];
 #pragma unroll
     for (int i = 0; i < U; i++) {
-      const bool in = s0 + i < ns;
-      my[i] = in ? sc[(size_t)(s0 + i) * step] : make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-      x[i] = in ? v[(size_t)(s0 + i) * step * LPR] : make_float4(0.f, 0.f, 0.f, 0.f);
+      my[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+      x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s0 + i < ns) {
+        my[i] = sc[(size_t)(s0 + i) * step];
+        x[i] = v[(size_t)(s0 + i) * step * LPR];
+      }
     }
     float Mn = M;
     Kv8Unit2 un = u;
