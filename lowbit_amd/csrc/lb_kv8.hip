@@ -278,6 +278,8 @@ constexpr int kKv8GridY = 1 << 15;  // units of a call in the grid's second dime
 constexpr float kKv8WUp = 14.0f;   // weights are scaled by 2^14
 constexpr float kKv8Head = 3.0f;  // a new reference lies this far above the largest x + ev: fewer follow
 constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
+// The reference before any key: finite, so that masked scores of -inf weigh exp2(-inf) = 0 under it.
+constexpr float kKv8None = -3.4028234663852886e38f;
 constexpr float kKv8Log2e = 1.4426950408889634f;
 
 // How a launch cuts its rows and keys: the sequences of rows_min .. rows_max rows a KV head, in
@@ -438,6 +440,10 @@ struct Kv8Unit2 {
 };
 __device__ __forceinline__ Kv8Unit2 kv8_larger(Kv8Unit2 a, Kv8Unit2 b) { return b.m - b.mid > a.m - a.mid ? b : a; }
 
+// The larger of two matrix-core results (NaN never wins): the median with +inf, one instruction,
+// where fmaxf would first make both canonical.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+
 // Waits for every load of the wave. After loads on a path that is seldom taken: without it the
 // compiler waits for all loads wherever the paths have joined, the common one included.
 __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
@@ -448,6 +454,7 @@ struct Kv8Tile {
   bool unused;   // its V codes are not to be used
   float kscale;  // 2^ke of K
   float ev;      // V's exponent
+  float ev_up;   // and that of the weights' scale
   float unit;    // 2^(mid - ev), what a weight counts in the denominator
 };
 
@@ -616,7 +623,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   v4f acc[NB][VB];
 #pragma unroll
   for (int y = 0; y < NB; y++) {
-    m[y] = -INFINITY, l[y] = 0.0f;
+    m[y] = kKv8None, l[y] = 0.0f;
 #pragma unroll
     for (int j = 0; j < VB; j++) acc[y][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
@@ -632,6 +639,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       now[x].unused = ve < max(least, 1);
       now[x].kscale = e8m0_to_f32((uint32_t)ke);
       now[x].ev = ve == 255 ? __builtin_nanf("") : (float)(max(ve, least) - 127);
+      now[x].ev_up = now[x].ev + kKv8WUp;
       now[x].unit = __int_as_float(ve == 255 ? 0x7FC00000 : (127 + imid - max(ve, least)) << 23);
     }
     // ---- scores of 32 keys
@@ -693,14 +701,14 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       // ---- the running reference
       const float c0 = cx[y] * now[0].kscale, c1 = cx[y] * now[1].kscale;
       const v4f s0 = s[y][0], s1 = s[y][1];
-      const float t0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3]));
-      const float t1 = fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]));
+      const float t0 = fmaxf(larger(s0[0], s0[1]), larger(s0[2], s0[3]));
+      const float t1 = fmaxf(larger(s1[0], s1[1]), larger(s1[2], s1[3]));
       const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
       if (__any(top > m[y])) {
         const float mnew = fmaxf(m[y], ceilf(quarters_max(top)) + kKv8Head);
-        const float alpha = mnew == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[y] - mnew);
+        const float alpha = __builtin_amdgcn_exp2f(m[y] - mnew);
         m[y] = mnew;
-        huge = huge || __any(fabsf(mnew) > 0x1p22f && mnew != -INFINITY);
+        huge = huge || __any(fabsf(mnew) > 0x1p22f && mnew != kKv8None);
         l[y] *= alpha;
 #pragma unroll
         for (int j = 0; j < VB; j++)
@@ -708,17 +716,16 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           for (int e = 0; e < 4; e++) acc[y][j][e] *= alpha;
       }
       // ---- weights, their sum, and their two terms
-      const float ref = m[y] == -INFINITY ? 0.0f : m[y];
       const auto weights = [&](auto slow) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-          const float cc = x ? c1 : c0, off = (now[x].ev + kKv8WUp) - ref;
+          const float cc = x ? c1 : c0, off = now[x].ev_up - m[y];
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             p[e] = __builtin_fmaf(s[y][x][e], cc, off);
             if constexpr (slow) {
-              if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - ref) + kKv8WUp;
+              if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - m[y]) + kKv8WUp;
               p[e] = __builtin_amdgcn_exp2f(p[e]);
               // a block whose exponent is NaN counts where it is seen
               const bool seen = s[y][x][e] != -INFINITY;
@@ -819,16 +826,14 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       M = fmaxf(M, lds.sm[x][rr]);
       u = kv8_larger(u, {lds.sm[x][rr], lds.smid[x]});
     }
-    const float Mr = M == -INFINITY ? 0.0f : M;
-    if (u.m == -INFINITY) u.m = 0.0f;
 #pragma unroll
     for (int x = 0; x < NW; x++) {
-      f[x] = __builtin_amdgcn_exp2f(lds.sm[x][rr] - Mr);  // 0 for a wave without keys
+      f[x] = __builtin_amdgcn_exp2f(lds.sm[x][rr] - M);  // 0 for a wave without keys
       den = __builtin_fmaf(lds.sl[x][rr], __builtin_amdgcn_exp2f((lds.sm[x][rr] - u.m) - (lds.smid[x] - u.mid)), den);
     }
     if (w.slices > 1) {
       reinterpret_cast<float4 *>(part + pt.sums)[pu * R + rr] =
-          make_float4(M, M == -INFINITY ? M : u.m, u.mid, den);
+          make_float4(M, u.m, u.mid, den);
     } else {
       const float inv = den == 0.0f ? 0.0f : 1.0f / den;
 #pragma unroll
@@ -836,7 +841,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     }
 #pragma unroll
     for (int x = 0; x < NW; x++) lds.sm[x][rr] = f[x];
-    lds.sl[0][rr] = (Mr - u.m) + u.mid;
+    lds.sl[0][rr] = (M - u.m) + u.mid;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
@@ -908,14 +913,14 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
-  const float4 none = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+  const float4 none = make_float4(kKv8None, kKv8None, 0.f, 0.f);
   float4 x[U];
   const auto load = [&](int i0) {  // this wave's next slices, past the last the last again
 #pragma unroll
     for (int i = 0; i < U; i++) x[i] = v[(size_t)min(i0 + SP * W * i + lane / LPR, ns - 1) * step * LPR];
   };
-  float M = -INFINITY;
-  Kv8Unit2 u = {-INFINITY, 0.0f};
+  float M = kKv8None;
+  Kv8Unit2 u = {kKv8None, 0.0f};
   float4 my = none;  // (conditional loads, not a choice between addresses)
   if (lane < ns) my = sc[(size_t)lane * step];
   load(SP * wr);
@@ -933,8 +938,6 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   const int best = __ffsll((unsigned long long)__ballot(at == wave_max(at))) - 1;
   u.m = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(u.m), best));
   u.mid = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(u.mid), best));
-  const float Mr = M == -INFINITY ? 0.0f : M;
-  if (u.m == -INFINITY) u.m = 0.0f;
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
   float den = 0.0f;
   my = head;
@@ -943,7 +946,7 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
       my = none;
       if (s0 + lane < ns) my = sc[(size_t)(s0 + lane) * step];
     }
-    const float f = __builtin_amdgcn_exp2f(my.x - Mr);  // 0 for a slice without keys, and past the last
+    const float f = __builtin_amdgcn_exp2f(my.x - M);  // 0 for a slice without keys, and past the last
     den = __builtin_fmaf(my.w, __builtin_amdgcn_exp2f((my.y - u.m) - (my.z - u.mid)), den);
     const int n = min(ns - s0, kWave);
     for (int i0 = SP * wr; i0 < n; i0 += SP * W * U) {
@@ -977,7 +980,7 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   for (int k = 1; k < W; k++) num = add4(num, sh[k][e4]);
   if (lane >= LPR) return;
   const float f = den == 0.0f ? 0.0f : 1.0f / den;
-  const int e = (int)((Mr - u.m) + u.mid), t = kv8_token(cut, ro);
+  const int e = (int)((M - u.m) + u.mid), t = kv8_token(cut, ro);
   *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * cut.G + ro - t * cut.G) * D + 4 * e4) =
       make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
 }
@@ -995,14 +998,14 @@ __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &p
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
-  float M = -INFINITY, den = 0.0f;
-  Kv8Unit2 u = {-INFINITY, 0.0f};
+  float M = kKv8None, den = 0.0f;
+  Kv8Unit2 u = {kKv8None, 0.0f};
   float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int s0 = 0; s0 < ns; s0 += U) {
     float4 my[U], x[U];
 #pragma unroll
     for (int i = 0; i < U; i++) {
-      my[i] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+      my[i] = make_float4(kKv8None, kKv8None, 0.f, 0.f);
       x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (s0 + i < ns) {
         my[i] = sc[(size_t)(s0 + i) * step];
@@ -1016,24 +1019,22 @@ __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &p
       Mn = fmaxf(Mn, my[i].x);
       un = kv8_larger(un, {my[i].y, my[i].z});
     }
-    const float Mr = Mn == -INFINITY ? 0.0f : Mn, um = un.m == -INFINITY ? 0.0f : un.m;
-    const float fm = __builtin_amdgcn_exp2f(M - Mr), fd = __builtin_amdgcn_exp2f((u.m - um) - (u.mid - un.mid));
+    const float fm = __builtin_amdgcn_exp2f(M - Mn), fd = __builtin_amdgcn_exp2f((u.m - un.m) - (u.mid - un.mid));
     num = make_float4(num.x * fm, num.y * fm, num.z * fm, num.w * fm);
     den *= fd;
 #pragma unroll
     for (int i = 0; i < U; i++) {
-      const float f = __builtin_amdgcn_exp2f(my[i].x - Mr);  // 0 for a slice without keys, and past the last
+      const float f = __builtin_amdgcn_exp2f(my[i].x - Mn);  // 0 for a slice without keys, and past the last
       num.x = __builtin_fmaf(x[i].x, f, num.x);
       num.y = __builtin_fmaf(x[i].y, f, num.y);
       num.z = __builtin_fmaf(x[i].z, f, num.z);
       num.w = __builtin_fmaf(x[i].w, f, num.w);
-      den = __builtin_fmaf(my[i].w, __builtin_amdgcn_exp2f((my[i].y - um) - (my[i].z - un.mid)), den);
+      den = __builtin_fmaf(my[i].w, __builtin_amdgcn_exp2f((my[i].y - un.m) - (my[i].z - un.mid)), den);
     }
     M = Mn, u = un;
   }
-  if (u.m == -INFINITY) u.m = 0.0f;
   const float f = den == 0.0f ? 0.0f : 1.0f / den;
-  const int e = (int)(((M == -INFINITY ? 0.0f : M) - u.m) + u.mid), t = kv8_token(cut, ro);
+  const int e = (int)((M - u.m) + u.mid), t = kv8_token(cut, ro);
   *reinterpret_cast<float4 *>(out + (size_t)(w.s.row0 + t) * out_stride + (kv * cut.G + ro - t * cut.G) * D + 4 * e4) =
       make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
 }
@@ -1134,7 +1135,7 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
       const int res = 256 * (D == 128 ? 2 : D == 64 ? 3 : 4);  // workgroups of four waves that the device holds
       // two waves a workgroup where there are enough of them: a row's query is laid out by half as
       // many waves, and each sees more keys (2048 tokens of 32 heads on 8 98 -> 91 us)
-      if (blocks * a.KV >= 2 * res) plan.waves = 2;
+      if (4 * blocks * a.KV >= 5 * res) plan.waves = 2;
       const int fits = plan.waves == 2 ? 2 * res : res;
       p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), (float)fits / (float)a.KV};
     }
