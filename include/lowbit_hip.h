@@ -490,8 +490,10 @@ int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const f
  * .. their own, which the cache must hold: lbd_kv8_append first. A row whose positions are
  * on no page at all gets zeros. Rows of no sequence are left as they are. out must not
  * overlap q. Strides multiples of 4, q and out 16-byte aligned. work:
- * lbd_kv8_attention_work_bytes of the same arguments, 16-byte aligned (NULL where that is
- * 0); it needs no clearing, and calls that share it must be ordered (one stream). */
+ * lbd_kv8_attention_work_bytes of the same arguments (0: they are refused), 16-byte aligned;
+ * it needs no clearing, and calls that share it must be ordered (one stream, or graphs that
+ * are not replayed at once). A code of NaN in a page written by other means counts as NaN
+ * where it is seen. */
 size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch,
                                     int H);
 int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q,

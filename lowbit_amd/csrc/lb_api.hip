@@ -1582,8 +1582,9 @@ int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, cons
   if ((rc = kv8_pointers(a)) < 0) return rc;
   if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ARG, "q and out must be 16-byte aligned");
   const size_t need = lbk::kv8_attention_work_bytes(a, pool->D, H);
-  if (need && (!work || work_bytes < need)) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
-  if (need && !aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
+  if (!need) return fail(LB_ERR_SHAPE, "too many rows of heads for a launch");
+  if (!work || work_bytes < need) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
+  if (!aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
   LB_LAUNCH(lbk::launch_kv8_attention(a, pool->D, q, q_stride, H, out, out_stride, work,
                                       static_cast<hipStream_t>(stream)),
             "kv8 attention launch");

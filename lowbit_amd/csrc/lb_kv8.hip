@@ -486,6 +486,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const int c = lane & 15, g = lane >> 4;
   Kv8Unit w;
   if (!kv8_unit<false>(a, cut, unit, w)) return;
+  const int place = unit - w.at + w.rb * w.slices + w.slice;  // in the workspace
+  if (place >= pt.units) return;  // (rows of several sequences at once, which is not allowed)
   const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
   // this lane's query rows, the keys they see, and those that the block's last row sees
   int lim[NB];
@@ -827,7 +829,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   }
   if (lane == 0) lds.smid[wave] = mid;
   __syncthreads();
-  const size_t pu = (size_t)(unit - w.at + w.rb * w.slices + w.slice) * a.KV + kv;
+  const size_t pu = (size_t)place * a.KV + kv;
   float *po = part + pu * R * D;
   // a thread a row: the waves' factors, and the sums' common unit
   for (int rr = threadIdx.x; rr < R; rr += NW * kWave) {
@@ -921,7 +923,7 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   Kv8Unit w;
   if (!kv8_unit<true>(a, cut, idx / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
-  if (ns < 2 || ro >= w.s.n * cut.G) return;
+  if (ns < 2 || ro >= w.s.n * cut.G || w.before + (w.rb + 1) * ns > pt.units) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
@@ -1063,6 +1065,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8Args &a, const Kv8Part &pt, i
   const int idx = block / pt.merge, kv = idx % a.KV;
   Kv8Unit w;
   if (!kv8_unit<true>(a, pt.cut, idx / a.KV, w) || w.slices < 2) return;
+  if (w.before + (w.rb + 1) * w.slices > pt.units) return;
   const int rows = min(pt.cut.R, w.s.n * pt.cut.G - w.rb * pt.cut.R);
   for (int rr = block % pt.merge * ROWS + threadIdx.x / (D / 4); rr < rows; rr += pt.merge * ROWS)
     kv8_merge_row<D>(a, pt, w, kv, rr, work, out, out_stride);
@@ -1094,7 +1097,7 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
   const auto go = [&](auto kern, int nt) {
     const long long chunks = ((long long)H * (D / 8) + nt - 1) / nt;
     const long long grid = nkv * 2 * a.KV + chunks * a.T;
-    if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+    if (grid > 0xFFFFFFFFll / nt) return hipErrorInvalidValue;  // threads of a launch are counted in 32 bits
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(nt), 0, s, a, qkv, stride, bias, H, cosT, sinT, max_pos, q_out,
                        q_stride, (int)nkv);
     return hipGetLastError();
@@ -1152,7 +1155,7 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
       p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), (float)fits / (float)a.KV};
     }
     const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
-    if (units > 1 << 29 || rows > 1 << 29) return false;
+    if (blocks * a.KV >= 1 << 23) return false;  // threads of a launch are counted in 32 bits
     p.blocks = (int)blocks;
     p.units = (int)units;
     // few rows of many slices: a workgroup a row; many: 1024 / D rows at a time

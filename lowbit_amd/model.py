@@ -652,8 +652,8 @@ class Model:
         prompts, chunks of prompts and single tokens in one pass. Returns the logits [S, V] of each
         sequence's last token; rows of sequences without tokens are NaN."""
         cfg, L = self.cfg, self.L
-        S = len(cache.lengths)
-        if not isinstance(cache, KV8Cache) or len(tokens) != S:
+        S = len(cache.lengths) if isinstance(cache, KV8Cache) else -1
+        if len(tokens) != S:
             raise ValueError("forward_batch takes a KV8Cache and a list of tokens for each of its sequences")
         rows = [self._tokens(t) if len(t) else np.zeros(0, np.int32) for t in tokens]
         news = np.array([len(r) for r in rows])

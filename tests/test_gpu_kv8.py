@@ -253,6 +253,21 @@ def test_batches_that_make_no_sense(rng):
     assert got.shape == (T, H * D)
 
 
+@pytest.mark.parametrize("rows,G", [(1, 8), (2000, 1)])
+def test_rows_of_several_sequences_at_once(rng, rows, G):
+    """q_start that goes back and forth, so that far more rows take part than there are: the long
+    sequence's slices, which lie about the workspace's end, stay inside it (its guard stays)."""
+    D, page, B, past = 64, 128, 2001 if rows > 1 else 3000, 20000
+    pool = O.Pool(rng, 2, page, 1, D)
+    q_start = np.arange(B + 1) % 2 * rows
+    pasts = np.zeros(B, np.int64)
+    pasts[96 if rows > 1 else 1000:][:8] = past
+    table = rng.integers(0, 2, (B, -(-(past + rows) // page))).astype(np.int32)
+    q = rng.standard_normal((rows, G * D)).astype(np.float32)
+    got = Device(pool, q_start, pasts, table, rows, rows).attention(q, G, G * D)
+    assert got.shape == q.shape
+
+
 # ---------------------------------------------------------------- attention
 
 def cached(rng, pages, page, KV, D, table, seqs, spread=2):
@@ -570,3 +585,28 @@ def test_same_bits_twice(rng):
     q = rng.standard_normal((T, H * D)).astype(np.float32)
     dev = Device(pool, q_start, past, table, 1, T)
     assert np.array_equal(dev.attention(q, H, H * D), dev.attention(q, H, H * D))
+
+
+def test_two_streams_at_once(rng):
+    """Calls on two streams, each with a workspace of its own, over one pool."""
+    D, page, KV, H = 64, 32, 2, 8
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    runs = []
+    for seqs in ([(3000, 1)] * 6, [(700, 90), (0, 200), (2000, 1)]):
+        pages, q_start, past, table, T = batch_of(rng, page, seqs)
+        pool = cached(rng, pages, page, KV, D, table, seqs)
+        q = rng.standard_normal((T, H * D)).astype(np.float32)
+        dev = Device(pool, q_start, past, table, max(n for _, n in seqs), T)
+        need = L.lbd_kv8_attention_work_bytes(C.byref(dev.pool), C.byref(dev.batch), H)
+        s = C.c_void_p()
+        ok(L.lb_stream_create(C.byref(s)))
+        runs.append((dev, up(q), up(np.full((T, H * D), FILL)), K.DeviceBuffer(need), need, s,
+                     dev.attention(q, H, H * D)))
+    for _ in range(20):
+        for dev, dq, do, ws, need, s, _ in runs:
+            ok(L.lbd_kv8_attention(C.byref(dev.pool), C.byref(dev.batch), dq.ptr, H * D, H, do.ptr, H * D, ws.ptr, need,
+                                   s.value))
+    ok(L.lb_dev_synchronize())
+    for _, _, do, _, _, s, want in runs:
+        assert np.array_equal(do.to_array(want.shape, np.float32), want)
+        ok(L.lb_stream_destroy(s.value))

@@ -149,3 +149,10 @@ def test_pages_come_and_go():
                 lambda: model.new_cache(0, kv="e4m3")):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_batches_take_an_8_bit_cache():
+    cfg, W = small()
+    model = M.Model(cfg, W, "w4a16")
+    with pytest.raises(ValueError):
+        model.forward_batch([[1]], model.new_cache(10))
