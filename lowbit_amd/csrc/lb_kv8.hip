@@ -415,6 +415,13 @@ __device__ __forceinline__ _Float16 half_rest(float x, _Float16 hi, float minus1
 }
 __device__ __forceinline__ float minus_one() { return __uint_as_float(opaque(0xBF800000u)); }
 
+// max(a, |x|, |y|), in one instruction (NaN never wins).
+__device__ __forceinline__ float max3_abs(float a, float x, float y) {
+  float r;
+  asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(x), "v"(y));
+  return r;
+}
+
 // 2^(13 - exponent of a row's largest |q|), which brings it into [2^13, 2^14), and the inverse.
 // (An element that is not finite has a lo term of NaN, so its row's scores are NaN.)
 __device__ __forceinline__ void kv8_q_scale(int big, float &up, float &down) {
@@ -448,6 +455,7 @@ __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70
 struct Kv8Tile {
   bool held;     // there is such a page
   bool unused;   // its V codes are not to be used
+  bool nan;      // K's or V's block is NaN
   float kscale;  // 2^ke of K
   float ev;      // V's exponent
   float ev_up;   // and that of the weights' scale
@@ -510,7 +518,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   int t_ke = 0, t_ve = 0;
   size_t t_at = 0;  // the tile's first code row, in bytes
   float t_kscale = 0.f, t_ev = 0.f, t_unit = 0.f;
-  uint64_t t_held = 0, t_unused = 0;  // a bit a tile
+  uint64_t t_held = 0, t_unused = 0, t_nan = 0;  // a bit a tile
   const auto tile_key = [&](int i) { return k_begin + CK * (wave + NW * (i >> 1)) + 16 * (i & 1); };
   const auto load_tiles = [&](int i0) {
     const int key = tile_key(i0 + lane);
@@ -592,6 +600,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const auto weigh_tiles = [&]() {
     const int ve = max(t_ve, least);
     t_held = __ballot(t_ve >= 0);
+    t_nan = __ballot(t_ke == 255 || t_ve == 255);
     t_unused = __ballot(t_ve < max(least, 1));
     t_kscale = e8m0_to_f32((uint32_t)t_ke);
     t_ev = t_ve == 255 ? __builtin_nanf("") : (float)(ve - 127);
@@ -604,9 +613,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   float cx[NB];
 #pragma unroll
   for (int y = 0; y < NB; y++) {
-    int big = 0;
+    float top = 0.0f;
 #pragma unroll
-    for (int s = 0; s < KS; s++) big = max(big, max(abs_bits(qf[y][s][0]), abs_bits(qf[y][s][1])));
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) top = max3_abs(max3_abs(top, qf[y][s][e].x, qf[y][s][e].y), qf[y][s][e].z, qf[y][s][e].w);
+    int big = __float_as_int(top);
     big = max(big, __shfl_xor(big, 16));
     big = max(big, __shfl_xor(big, 32));
     float up, down;
@@ -650,6 +662,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       const auto of = [&](float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), o)); };
       now[x].held = t_held >> o & 1;
       now[x].unused = t_unused >> o & 1;
+      now[x].nan = t_nan >> o & 1;
       now[x].kscale = of(t_kscale);
       now[x].ev = of(t_ev);
       now[x].ev_up = now[x].ev + kKv8WUp;
@@ -698,7 +711,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     }
     // ---- what some row does not see: scores -inf, and V's codes, which may be anything, 0
     const bool edge = key0 + CK > k_full || now[0].unused || now[1].unused;
+    bool careful = false;  // a score of -inf may meet a factor of NaN or 0
     if (edge) {
+      bool zero = false;
+#pragma unroll
+      for (int y = 0; y < NB; y++) zero = zero || cx[y] * fminf(now[0].kscale, now[1].kscale) == 0.0f;
+      careful = careful || now[0].nan || now[1].nan || __any(zero);
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
@@ -765,7 +783,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           }
         }
       };
-      if (edge || huge)
+      if (careful || huge)
         weights(std::true_type());
       else
         weights(std::false_type());

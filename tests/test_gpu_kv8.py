@@ -437,6 +437,18 @@ def test_attention_query_sizes(rng, scale, n):
         assert np.abs(got - ref).max() <= 2.0 ** -19 * np.abs(ref).max()
 
 
+@pytest.mark.parametrize("n", [1, 20, 100])
+def test_attention_of_zeros(rng, n):
+    """Rows of zeros over blocks of the least exponent: every key counts alike, those behind a row not."""
+    D, page, KV, H, seqs = 64, 16, 1, 3, [(37, n), (0, n)]
+    pages, q_start, past, table, T = batch_of(rng, page, seqs)
+    pool = cached(rng, pages, page, KV, D, table, seqs)
+    pool.ke[:] = 0
+    q = np.zeros((T, H * D + 4), np.float32)
+    q[::3] = 1e-30
+    run_attention(rng, D, page, KV, H, seqs, pad=0, extra=0, pool=pool, table=table, q=q)
+
+
 def test_rows_before_the_first_sequence_and_positions_past_the_table(rng):
     """q_start may begin behind row 0; a token past the table's last position is not written and
     attends over all of it."""
