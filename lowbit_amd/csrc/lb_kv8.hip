@@ -150,6 +150,15 @@ __device__ __forceinline__ void rope4_pair(float4 &a, float4 &b, float4 c, float
 //     and nobody else writes it. A thread takes IT items of 8 elements: 4 of each half of a
 //     token's head row, a rotation's partners (page D / 8 items at most).
 //   the others: 8 NT elements of a row's query heads, rotated into q_out.
+//
+// What bounds it: a step, the launch and three loads one after the other (the batch, the page, the
+// block's exponent): one token of 14 heads on 2 2.6 us, 64 sequences of 32 heads on 8 3.4 us.
+// Prompts, the bytes: 4 sequences of up to 1000 tokens, 32 heads on 8, 45.8 MB in 10.7 us = 4.3
+// TB/s (a large copy reaches 5.2). A block is one workgroup's so that its largest element costs no
+// second pass over the rows and no atomic, and codes leave as whole words.
+//
+// Rounding: rotation as lbd_qkv_rope's, every product and sum to float32; a code to the nearest
+// E4M3, ties to even, once, and once more for each later growth of its block's exponent.
 template <int D, int NT, int IT>
 __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *qkv, int stride,
                                                         const float *__restrict__ bias, int H,
@@ -462,18 +471,32 @@ struct Kv8Tile {
   float unit;    // 2^(mid - ev), what a weight counts in the denominator
 };
 
-// Few query rows a sequence (steps): R = 8 rows a block, or 16 (SEP). NW waves share a slice
-// in chunks of 32 keys, two 16-key tiles, each wave with its own running reference and sums,
-// merged in LDS. Everything is transposed, scores^T = K Q^T and out^T = V^T W^T, so a lane
-// keeps one query row (lane % 16) and what it gets from the first product (keys 4 (lane / 16)
-// + r of either tile) is the operand of the second as it is. R = 8: columns 8..15 hold the lo
-// terms of the rows in 0..7, one matrix instruction for both, and a row rotation by 8 adds
-// them; SEP: hi and lo one after the other.
+// A row block's slice of keys. NW waves share it in chunks of 32 keys, two 16-key tiles, each
+// wave with its own running reference and sums, merged in LDS. Everything is transposed,
+// scores^T = K Q^T and out^T = V^T W^T, so a lane keeps one query row (lane % 16) of each column
+// block and what it gets from the first product (keys 4 (lane / 16) + r of either tile) is the
+// operand of the second as it is.
+//   NC 0: 8 rows; columns 8 .. 15 hold the lo terms of the rows in 0 .. 7, one matrix instruction
+//     for both, and a row rotation by 8 adds them.
+//   NC 1: 16 rows, hi and lo one after the other.
+//   NC 2: 32 rows, two column blocks of 16, for which K and V are made float16 once.
 // K is read 16 bytes a lane (8 at D = 32), V D / 16 bytes a lane of eight keys: a lane's bytes
 // of two keys are interleaved by v_perm on their way to float16, which is all the transposing
 // that V needs, and its output elements come out contiguous. The next chunk's K is requested
 // once the scores are made, its V once the outputs are: loads are always in flight, and no
 // LDS lies between them and the matrix cores.
+//
+// What bounds it. Few rows, the cache's bytes: 61 sequences of 50 to 4096 keys, 32 heads on 8 of
+// 128, 254 MB in 52 us and 5 for the merge, 4.5 TB/s; one of 60000 keys 25 us and 5. (Three waves a
+// SIMD at D = 128: with registers for four the loop spills, 72 us against 59.) Short ones, the
+// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.6 us.
+// Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 87 us, 397 TFLOP/s of the
+// formula, twice that in products of two terms (a large float16 product reaches 1180). The matrix
+// cores are busy for a third of the time and the vector units for nearly half, and at two waves a
+// SIMD the two hardly overlap; loads cost 5 %. Tried and slower or alike: products of 32 x 32 x 16
+// (0 to 6 %), the next chunk's scores beside this one's weights (0 to 40 %, it spills at D = 128),
+// matrix and vector instructions alternated by scheduling barriers, both column blocks' weights in
+// one stretch (3 %).
 template <int D, int NC, int NW>
 struct Kv8Lds {
   float sh[NW][kv8_rows(NC)][D + 4];
@@ -1176,8 +1199,11 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     if (blocks * a.KV >= 1 << 23) return false;  // threads of a launch are counted in 32 bits
     p.blocks = (int)blocks;
     p.units = (int)units;
-    // few rows of many slices: a workgroup a row; many: 1024 / D rows at a time
-    p.merge = rows <= 2048 ? 0 : blocks * a.KV >= 1024 ? 1 : std::max(1, R * D / 1024);
+    // Few rows (of many slices): a workgroup a row (but 16 sequences of up to 2000
+    // keys and 4 tokens, 32 heads on 8, 2048 rows: 16.2 us, a workgroup a row 21.1). Many: 1024 / D rows at
+    // a time, and where there are workgroups enough a whole row block one after the other, as each
+    // finds its place anew (1000 tokens, 32 heads on 8: 39.6 us, with four a row block 44.3).
+    p.merge = rows <= 512 ? 0 : blocks * a.KV >= 256 ? 1 : std::max(1, R * D / 1024);
     p.at = plan.floats;
     p.sums = (size_t)units * a.KV * R * D;
     plan.floats += p.sums + (size_t)units * a.KV * R * 4;
