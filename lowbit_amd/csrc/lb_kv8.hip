@@ -487,9 +487,9 @@ struct Kv8Tile {
 // LDS lies between them and the matrix cores.
 //
 // What bounds it. Few rows, the cache's bytes: 61 sequences of 50 to 4096 keys, 32 heads on 8 of
-// 128, 254 MB in 52 us and 5 for the merge, 4.5 TB/s; one of 60000 keys 25 us and 5. (Three waves a
+// 128, 254 MB in 52 us and 5 for the merge, 4.3 to 4.5 TB/s; one of 60000 keys 25 us and 5. (Three waves a
 // SIMD at D = 128: with registers for four the loop spills, 72 us against 59.) Short ones, the
-// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.6 us.
+// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.8 us.
 // Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 87 us, 397 TFLOP/s of the
 // formula, twice that in products of two terms (a large float16 product reaches 1180). The matrix
 // cores are busy for a third of the time and the vector units for nearly half, and at two waves a
@@ -925,7 +925,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // One class of sequences, or (MIXED) two in one launch, of many rows (NC = 2) and then of few
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
 // (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
-// other 57 us, one of each 45; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
+// other 57 us, one of each 45, by now 41; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
 template <int D, int NC, int NW, bool MIXED>
 __global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,

@@ -9,6 +9,8 @@ Contents
   reference.py   numpy restatement of the reference's ground truth: nibble
                  unpacking, int4/MXFP4 dequantization, float64 GEMMs, exact
                  int64 W4A8 group accumulators, the per-token int8 quantizer.
+  kv_cache.py    the paged 8-bit key / value cache: E4M3 and E8M0 in closed form,
+                 append (float32 rotation, bit for bit) and attention in float64.
   csrc/          plain-C restatement of the same (the bit-exact quantizer, the
                  int64 group accumulators, float64 GEMMs), built into
                  oracle/_build/liblowbit_oracle.so; it checks the GPU at sizes
