@@ -492,8 +492,8 @@ int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const f
  * overlap q. Strides multiples of 4, q and out 16-byte aligned. work:
  * lbd_kv8_attention_work_bytes of the same arguments (0: they are refused), 16-byte aligned;
  * it needs no clearing, and calls that share it must be ordered (one stream, or graphs that
- * are not replayed at once). A code of NaN in a page written by other means counts as NaN
- * where it is seen. */
+ * are not replayed at once). Pages written by other means than lbd_kv8_append must hold no
+ * code of NaN (0x7f, 0xff) at a position that is attended to. */
 size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch,
                                     int H);
 int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q,

@@ -1561,9 +1561,10 @@ int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const f
       (bias && !aligned16(bias)))
     return fail(LB_ERR_ARG, "qkv, bias, the tables and q_out must be 16-byte aligned");
   if (q_out == qkv && q_stride != stride) return fail(LB_ERR_ARG, "q_out on qkv takes the same stride");
-  LB_LAUNCH(lbk::launch_kv8_append(a, pool->D, qkv, stride, bias, H, cos_table, sin_table, max_pos, q_out, q_stride,
-                                   static_cast<hipStream_t>(stream)),
-            "kv8 append launch");
+  const hipError_t e = lbk::launch_kv8_append(a, pool->D, qkv, stride, bias, H, cos_table, sin_table, max_pos, q_out,
+                                              q_stride, static_cast<hipStream_t>(stream));
+  if (e == hipErrorInvalidValue) return fail(LB_ERR_SHAPE, "too many rows of heads for a launch");
+  LB_LAUNCH(e, "kv8 append launch");
 }
 
 size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, int H) {

@@ -62,6 +62,14 @@ def test_attention_refuses(over, rc):
     assert attention(**over) == rc
 
 
+def test_too_many_rows_for_a_launch():
+    over = dict(B=1 << 24, T=1 << 24, H=16, KV=16)
+    assert attention(**over, q_stride=1024, out_stride=1024) == -1
+    pool, batch = structs(**over)
+    assert K.lib().lbd_kv8_attention_work_bytes(C.byref(pool), C.byref(batch), 16) == 0
+    assert append(**over, stride=3200, q_stride=1024) == -1
+
+
 def test_null_structures():
     pool, batch = structs()
     L = K.lib()
