@@ -499,7 +499,11 @@ struct Kv8Tile {
 // one stretch (3 %).
 template <int D, int NC, int NW>
 struct Kv8Lds {
-  float sh[NW][kv8_rows(NC)][D + 4];
+  union {
+    float sh[NC == 2 ? NW / 2 : NW][kv8_rows(NC)][D + 4];
+    uint4 q[NC == 2 ? D / 8 : 1][kWave];  // NC 2: the query rows' operands, [column block][product][term]
+  };
+  float cx[2][16];
   float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
 };
 
@@ -553,10 +557,13 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     t_ve = a.ve[block];
     t_ve = in ? t_ve : -1;
   };
-  v8h qh[NB][KS], ql[NB][SEP ? KS : 1];
-  float4 qf[NB][KS][2];
+  constexpr bool BIG = NC == 2;  // the query rows laid out by the waves together, in LDS
+  constexpr int QB = BIG ? 1 : NB;
+  v8h qh[QB][KS], ql[QB][SEP ? KS : 1];
+  float4 qf[QB][KS][2];
+  if constexpr (BIG) qr[0] = wave & 1 ? qr[1] : qr[0];
 #pragma unroll
-  for (int y = 0; y < NB; y++)
+  for (int y = 0; y < QB; y++)
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       const int d = D == 32 ? 8 * g : 64 * (s >> 1) + 16 * g + 8 * (s & 1);
@@ -635,7 +642,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const float minus1 = minus_one();
   float cx[NB];
 #pragma unroll
-  for (int y = 0; y < NB; y++) {
+  for (int y = 0; y < QB; y++) {
     float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
@@ -649,6 +656,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     cx[y] = down * (kKv8Log2e / sqrtf((float)D));
 #pragma unroll
     for (int s = 0; s < KS; s++) {
+      if (BIG && s * NW / 2 / KS != wave / 2) continue;  // another wave's
       const float4 a0 = qf[y][s][0], a1 = qf[y][s][1];
       const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
 #pragma unroll
@@ -664,7 +672,16 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           qh[y][s][e] = two.x, qh[y][s][e + 1] = two.y;
         }
       }
+      if constexpr (BIG) {
+        lds.q[((wave & 1) * KS + s) * 2][lane] = __builtin_bit_cast(uint4, qh[0][s]);
+        lds.q[((wave & 1) * KS + s) * 2 + 1][lane] = __builtin_bit_cast(uint4, ql[0][s]);
+      }
     }
+  }
+  if constexpr (BIG) {
+    if (g == 0 && wave < 2) lds.cx[wave][c] = cx[0];
+    __syncthreads();
+    cx[0] = lds.cx[0][c], cx[NB - 1] = lds.cx[1][c];
   }
 
   float m[NB], l[NB];
@@ -676,6 +693,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     for (int j = 0; j < VB; j++) acc[y][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
   bool huge = false;  // |m| with few bits left for fractions: x has to be rounded as it was for m
+  const auto q_at = [&](int y, int k, int term) {
+    if constexpr (BIG)
+      return __builtin_bit_cast(v8h, lds.q[(y * KS + k) * 2 + term][lane]);
+    else
+      return term ? ql[y][SEP ? k : 0] : qh[y][k];
+  };
   const auto chunk = [&](int i, auto more) {
     const int key0 = tile_key(2 * i);
     Kv8Tile now[2];
@@ -708,13 +731,13 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 #pragma unroll
       for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int y = 0; y < NB; y++) s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], qh[y][k], s[y][x], 0, 0, 0);
+        for (int y = 0; y < NB; y++) s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], q_at(y, k, 0), s[y][x], 0, 0, 0);
       if constexpr (SEP) {
 #pragma unroll
         for (int x = 0; x < 2; x++)
 #pragma unroll
           for (int y = 0; y < NB; y++)
-            s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], ql[y][k], s[y][x], 0, 0, 0);
+            s[y][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk[x], q_at(y, k, 1), s[y][x], 0, 0, 0);
       }
     }
     if constexpr (more) {
@@ -858,10 +881,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         for (int e = 0; e < 4; e++) acc[y][j][e] += dpp_f<0x128>(acc[y][j][e], 0.0f);
     }
     if (SEP || c < 8) {
+      if constexpr (!BIG) {
 #pragma unroll
       for (int e = 0; e < 4; e++)
 #pragma unroll
         for (int j = 0; j < VB; j++) lds.sh[wave][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
+      }
       if (g == 0) {
         lds.sm[wave][16 * y + c] = m[y];
         lds.sl[wave][16 * y + c] = l[y];
@@ -899,12 +924,48 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     lds.sl[0][rr] = (M - u.m) + u.mid;
   }
   __syncthreads();
+  if constexpr (BIG) {
+    float fy[NB];
+#pragma unroll
+    for (int y = 0; y < NB; y++) fy[y] = lds.sm[wave][16 * y + c];
+    const auto put = [&](int w0) {
+#pragma unroll
+      for (int y = 0; y < NB; y++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int j = 0; j < VB; j++) lds.sh[w0][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
+    };
+#pragma unroll
+    for (int y = 0; y < NB; y++)
+#pragma unroll
+      for (int j = 0; j < VB; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[y][j][e] *= fy[y];
+#pragma unroll
+    for (int half = NW / 2; half; half /= 2) {
+      if (wave >= half && wave < 2 * half) put(wave - half);
+      __syncthreads();
+      if (wave < half) {
+#pragma unroll
+        for (int y = 0; y < NB; y++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int j = 0; j < VB; j++) acc[y][j][e] += lds.sh[wave][16 * y + c][4 * VB * g + VB * e + j];
+      }
+      __syncthreads();
+    }
+    if (wave == 0) put(0);
+    __syncthreads();
+  }
   for (int i = threadIdx.x; i < R * D / 4; i += NW * kWave) {
     const int rr = i / (D / 4), d = 4 * (i % (D / 4)), ro = w.rb * R + rr;
     if (ro >= rows) break;
     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (BIG) num = *reinterpret_cast<const float4 *>(&lds.sh[0][rr][d]);
 #pragma unroll
-    for (int x = 0; x < NW; x++) {
+    for (int x = 0; x < (BIG ? 0 : NW); x++) {
       const float f = lds.sm[x][rr];
       const float4 v = *reinterpret_cast<const float4 *>(&lds.sh[x][rr][d]);
       num.x = __builtin_fmaf(v.x, f, num.x);
@@ -927,7 +988,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
 // other 57 us, one of each 45, by now 41; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
 template <int D, int NC, int NW, bool MIXED>
-__global__ __launch_bounds__(NW *kWave, NC == 2 ? 2 : D == 128 ? 3 : 4) void kv8_attend_kernel(
+__global__ __launch_bounds__(NW *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
     int out_stride, float *__restrict__ work) {
   union Lds {
@@ -1188,7 +1249,7 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
       p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f};
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
-      const int res = 256 * (D == 128 ? 2 : D == 64 ? 3 : 4);  // workgroups of four waves that the device holds
+      const int res = 256 * (D == 128 ? 3 : 4);  // workgroups of four waves that the device holds
       // two waves a workgroup where there are enough of them: a row's query is laid out by half as
       // many waves, and each sees more keys (2048 tokens of 32 heads on 8 98 -> 91 us)
       if (4 * blocks * a.KV >= 5 * res) plan.waves = 2;
