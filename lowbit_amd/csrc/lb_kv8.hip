@@ -286,6 +286,7 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 constexpr int kKv8GridY = 1 << 15;  // units of a call in the grid's second dimension
 constexpr float kKv8WUp = 14.0f;   // weights are scaled by 2^14
 constexpr float kKv8Head = 3.0f;  // a new reference lies this far above the largest x + ev: fewer follow
+constexpr int kKv8Waves = 4;       // of an attention workgroup
 constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
 // The reference before any key: finite, so that masked scores of -inf weigh exp2(-inf) = 0 under it.
 constexpr float kKv8None = -3.4028234663852886e38f;
@@ -497,8 +498,9 @@ struct Kv8Tile {
 // (0 to 6 %), the next chunk's scores beside this one's weights (0 to 40 %, it spills at D = 128),
 // matrix and vector instructions alternated by scheduling barriers, both column blocks' weights in
 // one stretch (3 %).
-template <int D, int NC, int NW>
+template <int D, int NC>
 struct Kv8Lds {
+  static constexpr int NW = kKv8Waves;
   union {
     float sh[NC == 2 ? NW / 2 : NW][kv8_rows(NC)][D + 4];
     uint4 q[NC == 2 ? D / 8 : 1][kWave];  // NC 2: the query rows' operands, [column block][product][term]
@@ -507,10 +509,11 @@ struct Kv8Lds {
   float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
 };
 
-template <int D, int NC, int NW>
+template <int D, int NC>
 __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, int kv, int unit,
                                            const float *__restrict__ q, int q_stride, float *__restrict__ out,
-                                           int out_stride, float *__restrict__ work, Kv8Lds<D, NC, NW> &lds) {
+                                           int out_stride, float *__restrict__ work, Kv8Lds<D, NC> &lds) {
+  constexpr int NW = kKv8Waves;
   constexpr bool SEP = NC > 0;
   constexpr int NB = SEP ? NC : 1, R = kv8_rows(NC), KS = D / 32, CK = 32;
   constexpr int KB = D >= 64 ? 16 : 8, KL = D / (4 * KB);  // bytes of a K load, loads per lane and tile
@@ -987,24 +990,24 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
 // (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
 // other 57 us, one of each 45, by now 41; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
-template <int D, int NC, int NW, bool MIXED>
-__global__ __launch_bounds__(NW *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
+template <int D, int NC, bool MIXED>
+__global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
     int out_stride, float *__restrict__ work) {
   union Lds {
-    Kv8Lds<D, NC, NW> one;
-    Kv8Lds<D, 1, NW> few;
+    Kv8Lds<D, NC> one;
+    Kv8Lds<D, 1> few;
   };
   __shared__ Lds lds;
   const int kv = blockIdx.x;
   const int unit = (int)(blockIdx.y + blockIdx.z * kKv8GridY);
   if constexpr (MIXED) {
     if (unit >= p0.units) {
-      kv8_attend<D, 1, NW>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
+      kv8_attend<D, 1>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
       return;
     }
   }
-  kv8_attend<D, NC, NW>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
+  kv8_attend<D, NC>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
 }
 
 // Partial sums of a row block's slices -> out, two ways: few rows of many slices, many rows of few.
@@ -1228,7 +1231,7 @@ constexpr int kKv8FewRows = 16;
 
 struct Kv8Plan {
   Kv8Part p[2];  // the call's classes: with both, many rows first
-  int parts, nc, waves;  // column blocks of the first one's kernel, waves of a workgroup
+  int parts, nc;  // nc: column blocks of the first one's kernel
   size_t floats;         // of the workspace
 };
 
@@ -1249,11 +1252,7 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
       p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f};
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
-      const int res = 256 * (D == 128 ? 3 : 4);  // workgroups of four waves that the device holds
-      // two waves a workgroup where there are enough of them: a row's query is laid out by half as
-      // many waves, and each sees more keys (2048 tokens of 32 heads on 8 98 -> 91 us)
-      if (4 * blocks * a.KV >= 5 * res) plan.waves = 2;
-      const int fits = plan.waves == 2 ? 2 * res : res;
+      const int fits = 256 * (D == 128 ? 3 : 4);  // workgroups that the device holds
       p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), (float)fits / (float)a.KV};
     }
     const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
@@ -1271,7 +1270,6 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     plan.parts++;
     return true;
   };
-  plan.waves = 4;
   plan.nc = many ? 2 : most > 8 ? 1 : 0;
   // a batch of one sequence is taken whole by the kernel that its largest size calls for
   if (!many) return add(plan.nc, 1, kKv8FewRows);
@@ -1292,14 +1290,11 @@ static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, 
   const int units = p0.units + p1.units;
   const dim3 grid(a.KV, std::min(units, kKv8GridY), (units + kKv8GridY - 1) / kKv8GridY);
   const auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(plan.waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
+    hipLaunchKernelGGL(kern, grid, dim3(kKv8Waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
   };
-  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, 4, false>);
-  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, 4, false>);
-  if (plan.nc == 2 && plan.waves == 4)
-    plan.parts == 1 ? go(kv8_attend_kernel<D, 2, 4, false>) : go(kv8_attend_kernel<D, 2, 4, true>);
-  if (plan.nc == 2 && plan.waves == 2)
-    plan.parts == 1 ? go(kv8_attend_kernel<D, 2, 2, false>) : go(kv8_attend_kernel<D, 2, 2, true>);
+  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, false>);
+  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, false>);
+  if (plan.nc == 2) plan.parts == 1 ? go(kv8_attend_kernel<D, 2, false>) : go(kv8_attend_kernel<D, 2, true>);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (a.max_pages << a.page_shift) <= p0.cut.min_keys) return e;
   const auto groups = [&](const Kv8Part &p) { return p.blocks * a.KV * (p.merge ? p.merge : p.cut.R); };
