@@ -299,7 +299,7 @@ struct Kv8Cut {
   int G, R, r_shift, rows_min, rows_max, min_keys;
   unsigned g_inv;  // ceil(2^32 / G)
   int few_blocks, slots_few, slots;  // slices a KV head: with at most few_blocks row blocks, and with more
-  float fits;                        // many rows: workgroups a KV head that the device holds at once, else 0
+  float units, fits;  // many rows: compute units a KV head, and workgroups that they hold; else 0
 };
 
 // One class of a call's sequences, by their rows, and where its slices' sums lie in the workspace:
@@ -329,21 +329,26 @@ __device__ __forceinline__ int kv8_keys(const Kv8Args &a, const Kv8Seq &s) {
 // Rows of a row block, by the column blocks of 16 a wave takes (0: 8 rows, both terms in one).
 __host__ __device__ constexpr int kv8_rows(int nc) { return nc ? 16 * nc : 8; }
 
-// How many keys a slice has, in steps of 256. `first`: sequences 0 .. 63 by lane.
+// How many keys a slice has, in steps of 128 (a chunk of each wave). `first`: sequences 0 .. 63 by lane.
 //
 // Few rows (the cache's bytes bound them): the batch's row blocks times keys over the slots, so
 // that however the lengths differ the slices are alike. Few row blocks (alike, mostly) get 512
 // slices in all, two a compute unit: 60000 keys of 8 KV heads 30 us, with 1024 34 (more sums to
 // merge); many get 2048: 61 sequences of 50 to 4096 keys 59.8 us, with 1024 62, with 512 64.
 //
-// Many rows (the matrix cores bound them): the mean row block's keys in ns slices, lane ns - 1
-// weighing the rounds that the device takes for them (the last one two thirds where it fills
-// half the device), each a slice's keys and the 512 that a workgroup's beginning and end cost,
-// and 256 for the merge. (200 tokens behind 8000, 25 row blocks of 8 KV heads on 512 workgroups:
-// five slices 76 us, three 100; 64 behind 8000, 8 row blocks: eight 31 us, sixteen 41; 1000
-// tokens, 219 of 2 KV heads: one 18 us, two 26.)
+// Many rows (the instructions bound them): the mean row block's keys in ns slices, lane ns - 1
+// weighing what they cost, in keys. For one sequence, whose slices are alike: a slice's keys and
+// 512 for a workgroup's beginning and end, times 0.72 k + 0.25 with k workgroups on the fullest
+// compute unit (measured 1, 1.5, 2.4), and the sums' way to the merge. (200 tokens behind 8000, 25
+// row blocks of 8 KV heads: five slices 72 us, four 82, three 74; 64 behind 8000, 8 row blocks:
+// four 31 us, six 36; 300 behind 2000 on 2 KV heads: three even slices 19.7 us, 1024 + 1024 + 252
+// keys 22.1; 1000 tokens, 219 row blocks of 2: one 16.5 us, two 21.8.) For several, whose slices
+// fill the units as they come: the rounds that the device takes, the last two thirds where it
+// fills half of it (3 of up to 100 tokens behind 6000, 32 heads on 8: 39 us, by the other 43.5; 16
+// of up to 40 behind 3000: 36 and 41.7).
 //
-// Slices are never more than slots and row blocks together: the sums in float, 1 % up.
+// Slices are never more than slots and row blocks together: the few's sum in float 1 % up, the
+// many's product 2 %.
 __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first) {
   const int lane = threadIdx.x & (kWave - 1);
   float blocks = (float)kv8_row_blocks(c, first), sum = blocks * (float)kv8_keys(a, first);
@@ -353,27 +358,35 @@ __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c,
     blocks += n;
     sum += n * (float)kv8_keys(a, s);
   }
-  blocks = fmaxf(wave_sum(blocks), 1.0f), sum = wave_sum(sum) * 1.01f;
-  float per;
-  if (c.fits > 0.0f) {
-    const float ns = (float)(lane + 1), mean = sum / blocks, each = mean / ns, full = blocks * ns / c.fits;
-    const float whole = floorf(full), rest = full - whole;
+  blocks = fmaxf(wave_sum(blocks), 1.0f), sum = wave_sum(sum);
+  if (c.units > 0.0f) {
+    const bool one = a.B == 1;
+    const float mean = (one ? 1.0f : 1.01f) * sum / blocks;
+    const auto keys_of = [&](float ns) {  // (for one, an exact multiple stays)
+      const float x = one ? 128.0f * ceilf(mean / ns * 0x1p-7f - 0x1p-11f) : 256.0f * ceilf(mean / ns * 0x1p-8f);
+      return fmaxf(x, (float)c.min_keys);
+    };
+    const float ns = (float)(lane + 1), load = blocks * ns / c.units, full = blocks * ns / c.fits;
+    const float k = load <= 4.0f ? ceilf(load) : load + 0.5f, whole = floorf(full), rest = full - whole;
     const float rounds = full < 3.0f ? whole + (rest == 0.0f ? 0.0f : rest <= 0.5f ? 0.67f : 1.0f) : full + 0.5f;
-    float cost = rounds * (each + 512.0f) + (lane ? 256.0f + 16.0f * ns : 0.0f);
-    if (lane && (each < (float)c.min_keys || blocks * ns > (float)c.slots)) cost = INFINITY;
+    float cost = one ? (0.72f * k + 0.25f) * (keys_of(ns) + 512.0f) : rounds * (mean / ns + 512.0f);
+    if (lane) cost += 256.0f + (one ? 180.0f * load : 16.0f * ns);
+    if (lane && (mean < ns * (float)c.min_keys || 1.02f * blocks * ns > (float)c.slots)) cost = INFINITY;
     const int best = __ffsll((unsigned long long)__ballot(cost == -wave_max(-cost)));
     // one: only sequences well longer than the mean are cut, the fewer the more row blocks there are
-    per = best > 1 ? mean / (float)best : blocks > 1.5f * c.fits ? 2.0f * mean : 1.25f * mean;
-  } else {
-    per = sum / (float)(blocks <= (float)c.few_blocks ? c.slots_few : c.slots);
+    // (and no more than there are slots for)
+    const float per = best > 1 ? keys_of((float)best)
+                               : fmaxf(keys_of(blocks > 1.5f * c.fits ? 0.5f : 0.8f), keys_of((float)c.slots / blocks));
+    return (int)fminf(per, (float)kKv8MaxPos);
   }
+  const float per = 1.01f * sum / (float)(blocks <= (float)c.few_blocks ? c.slots_few : c.slots);
   return max(c.min_keys, ((int)fminf(per, (float)kKv8MaxPos) | 255) + 1);
 }
 
-// ceil(keys / SL) for SL a multiple of 256 and keys <= 2^30, by way of float: both counts of
-// 256 keys are exact there, the quotient is at most one off.
+// ceil(keys / SL) for SL a multiple of 128 and keys <= 2^30, by way of float: both counts of
+// 128 keys are exact there, the quotient is at most one off.
 __device__ __forceinline__ int kv8_slices(int keys, int slice_keys) {
-  const int s = slice_keys >> 8, n = ((keys + 255) >> 8) + s - 1;
+  const int s = slice_keys >> 7, n = ((keys + 127) >> 7) + s - 1;
   int d = (int)((float)n * __builtin_amdgcn_rcpf((float)s));
   const int rest = n - d * s;
   d += rest < 0 ? -1 : rest >= s ? 1 : 0;
@@ -1249,11 +1262,12 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     long long blocks;
     if (nc < 2) {
       blocks = std::min(a.B, a.T);  // a row block each
-      p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f};
+      p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f, 0.0f};
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
       const int fits = 256 * (D == 128 ? 3 : 4);  // workgroups that the device holds
-      p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), (float)fits / (float)a.KV};
+      p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), 256.0f / (float)a.KV,
+               (float)fits / (float)a.KV};
     }
     const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
     if (blocks * a.KV >= 1 << 23) return false;  // threads of a launch are counted in 32 bits

@@ -356,6 +356,12 @@ def test_attention_slices(rng, D, KV, H, seqs):
     run_attention(rng, D, 32, KV, H, seqs)
 
 
+def test_attention_more_row_blocks_than_slots(rng):
+    """Many row blocks of short prompts, and a sequence longer than twice the mean whose own row blocks
+    outnumber the slices that a call may add."""
+    run_attention(rng, 32, 64, 32, 32, [(0, 320)] * 20 + [(0, 3200)], pad=0)
+
+
 def test_attention_prompts_and_steps(rng):
     run_attention(rng, 64, 32, 2, 8, [(700, 1), (0, 90), (1300, 1), (33, 2), (0, 1), (250, 40), (64, 0)])
 
