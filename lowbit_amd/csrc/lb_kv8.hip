@@ -485,7 +485,7 @@ struct Kv8Tile {
   float unit;    // 2^(mid - ev), what a weight counts in the denominator
 };
 
-// A row block's slice of keys. NW waves share it in chunks of 32 keys, two 16-key tiles, each
+// A row block's slice of keys. Four waves share it in chunks of 32 keys, two 16-key tiles, each
 // wave with its own running reference and sums, merged in LDS. Everything is transposed,
 // scores^T = K Q^T and out^T = V^T W^T, so a lane keeps one query row (lane % 16) of each column
 // block and what it gets from the first product (keys 4 (lane / 16) + r of either tile) is the
@@ -493,7 +493,10 @@ struct Kv8Tile {
 //   NC 0: 8 rows; columns 8 .. 15 hold the lo terms of the rows in 0 .. 7, one matrix instruction
 //     for both, and a row rotation by 8 adds them.
 //   NC 1: 16 rows, hi and lo one after the other.
-//   NC 2: 32 rows, two column blocks of 16, for which K and V are made float16 once.
+//   NC 2: 32 rows, two column blocks of 16, for which K and V are made float16 once. Their two
+//     terms are made once too, a part by each wave, and read from LDS in every chunk: the 64
+//     registers of a wave's own copy at D = 128 would leave room for two waves a SIMD, not three
+//     (24 sequences of prompts and steps, 14 heads on 2 of 64: 40.7 us, so 34.1).
 // K is read 16 bytes a lane (8 at D = 32), V D / 16 bytes a lane of eight keys: a lane's bytes
 // of two keys are interleaved by v_perm on their way to float16, which is all the transposing
 // that V needs, and its output elements come out contiguous. The next chunk's K is requested
@@ -503,14 +506,15 @@ struct Kv8Tile {
 // What bounds it. Few rows, the cache's bytes: 61 sequences of 50 to 4096 keys, 32 heads on 8 of
 // 128, 254 MB in 52 us and 5 for the merge, 4.3 to 4.5 TB/s; one of 60000 keys 25 us and 5. (Three waves a
 // SIMD at D = 128: with registers for four the loop spills, 72 us against 59.) Short ones, the
-// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.8 us.
-// Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 87 us, 397 TFLOP/s of the
+// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.6 us.
+// Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 86 us, 400 TFLOP/s of the
 // formula, twice that in products of two terms (a large float16 product reaches 1180). The matrix
-// cores are busy for a third of the time and the vector units for nearly half, and at two waves a
-// SIMD the two hardly overlap; loads cost 5 %. Tried and slower or alike: products of 32 x 32 x 16
-// (0 to 6 %), the next chunk's scores beside this one's weights (0 to 40 %, it spills at D = 128),
-// matrix and vector instructions alternated by scheduling barriers, both column blocks' weights in
-// one stretch (3 %).
+// cores are busy for a third of the time and the vector units for two thirds, 4 of 10 of whose
+// instructions belong to the waves' beginnings and ends; the two kinds hardly overlap, and loads
+// cost 5 %. Tried and slower or alike: products of 32 x 32 x 16 (0 to 6 %), the next chunk's scores
+// beside this one's weights (0 to 40 %, it spills), matrix and vector instructions alternated by
+// scheduling barriers, both column blocks' weights in one stretch (3 %), two waves a workgroup (1
+// to 15 %), the place of a workgroup found by one of its waves (1 %).
 template <int D, int NC>
 struct Kv8Lds {
   static constexpr int NW = kKv8Waves;
@@ -887,6 +891,14 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   if (chunks) chunk(chunks - 1, std::false_type());
 
   // ---- the waves' sums, merged; element 4 VB g + VB e + j of row c is acc[.][j][e]
+  const auto put = [&](int at) {
+#pragma unroll
+    for (int y = 0; y < NB; y++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int j = 0; j < VB; j++) lds.sh[at][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
+  };
 #pragma unroll
   for (int y = 0; y < NB; y++) {
     l[y] = quarters_sum(l[y]);
@@ -897,12 +909,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         for (int e = 0; e < 4; e++) acc[y][j][e] += dpp_f<0x128>(acc[y][j][e], 0.0f);
     }
     if (SEP || c < 8) {
-      if constexpr (!BIG) {
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int j = 0; j < VB; j++) lds.sh[wave][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
-      }
+      if constexpr (!BIG) put(wave);
       if (g == 0) {
         lds.sm[wave][16 * y + c] = m[y];
         lds.sl[wave][16 * y + c] = l[y];
@@ -928,8 +935,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       den = __builtin_fmaf(lds.sl[x][rr], __builtin_amdgcn_exp2f((lds.sm[x][rr] - u.m) - (lds.smid[x] - u.mid)), den);
     }
     if (w.slices > 1) {
-      reinterpret_cast<float4 *>(part + pt.sums)[pu * R + rr] =
-          make_float4(M, u.m, u.mid, den);
+      reinterpret_cast<float4 *>(part + pt.sums)[pu * R + rr] = make_float4(M, u.m, u.mid, den);
     } else {
       const float inv = den == 0.0f ? 0.0f : 1.0f / den;
 #pragma unroll
@@ -944,20 +950,13 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     float fy[NB];
 #pragma unroll
     for (int y = 0; y < NB; y++) fy[y] = lds.sm[wave][16 * y + c];
-    const auto put = [&](int w0) {
-#pragma unroll
-      for (int y = 0; y < NB; y++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-          for (int j = 0; j < VB; j++) lds.sh[w0][16 * y + c][4 * VB * g + VB * e + j] = acc[y][j][e];
-    };
 #pragma unroll
     for (int y = 0; y < NB; y++)
 #pragma unroll
       for (int j = 0; j < VB; j++)
 #pragma unroll
         for (int e = 0; e < 4; e++) acc[y][j][e] *= fy[y];
+    // half of the waves to the other half, twice (half the LDS of all at once, which three workgroups share)
 #pragma unroll
     for (int half = NW / 2; half; half /= 2) {
       if (wave >= half && wave < 2 * half) put(wave - half);
@@ -1002,7 +1001,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // One class of sequences, or (MIXED) two in one launch, of many rows (NC = 2) and then of few
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
 // (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
-// other 57 us, one of each 45, by now 41; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
+// other 57 us, one of each 45, by now 34; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
 template <int D, int NC, bool MIXED>
 __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
