@@ -272,20 +272,23 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 // one workgroup's. Slices that share a row block leave partial sums that a second launch adds.
 //
 // Scores are kept in base 2: x = q k log2(e) / sqrt(D). A block's V exponent ev joins the
-// exponential: a row's reference m is the largest x + ev so far, rounded up to a whole number
-// (so rescaling by 2^(m - m') is exact), and its weights w = 2^(x + ev - m) <= 1 multiply V's
-// codes as they are, so that what a row sees of V decides its precision, however far apart the
-// blocks' exponents are. The denominator is sum w 2^(mid - ev), in the unit 2^(m - mid), with
+// exponential: a row's reference m is a whole number (so rescaling by 2^(m - m') is exact) at most
+// kKv8Head below the largest x + ev so far, and its weights w = 2^(x + ev - m) multiply V's codes
+// as they are, so that what a row sees of V decides its precision, however far apart the blocks'
+// exponents are. The denominator is sum w 2^(mid - ev), in the unit 2^(m - mid), with
 // mid 50 below the slice's largest ev: every factor stays within 2^+-50. Blocks of V more than
 // 2^100 below the largest (blocks of zeros among them) count as zeros.
 //
-// The matrix products run on float16: an E4M3 code is exact there, q and w are taken as two
-// terms each (hi + lo: 22 bits; q relative to its row's largest element, w times 2^14, so that
-// the subnormals that the matrix cores flush lie 2^-28 below).
+// An E4M3 code is exact in float16 and in bf16, so the matrix products take codes as they are and
+// q and w in terms whose sum they are. q, two float16 terms: 22 bits of an element, and 2^-38 of its
+// row's largest where that is more (the matrix cores take float16's subnormals as they are). w, three
+// bf16 terms: all 24 bits however far it lies below the largest, as the keys that it outweighs may
+// hold the larger values (two float16 terms lost weights e^-17 below the row's largest, and those
+// e^-30 below it altogether; 2048 tokens of 32 heads took 86.3 us so, 93.8 now. Two bf16 terms,
+// rounded: 85.0, but errors of 2e-6 to 7e-6 in place of 4e-7 to 1.2e-6).
 
 constexpr int kKv8GridY = 1 << 15;  // units of a call in the grid's second dimension
-constexpr float kKv8WUp = 14.0f;   // weights are scaled by 2^14
-constexpr float kKv8Head = 3.0f;  // a new reference lies this far above the largest x + ev: fewer follow
+constexpr float kKv8Head = 8.0f;  // x + ev may lie this far above the reference: few new ones are needed
 constexpr int kKv8Waves = 4;       // of an attention workgroup
 constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
 // The reference before any key: finite, so that masked scores of -inf weigh exp2(-inf) = 0 under it.
@@ -453,6 +456,18 @@ __device__ __forceinline__ void kv8_q_scale(int big, float &up, float &down) {
   down = __int_as_float((254 - e) << 23);
 }
 
+// Two weights in three bf16 terms each, 8 significant bits a term and all 24 together (the first of
+// a pair in the low half).
+struct Kv8Terms {
+  uint32_t hi, mid, lo;
+};
+__device__ __forceinline__ Kv8Terms kv8_terms(float a, float b) {
+  const auto top = [](float x) { return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u); };
+  const auto pack = [](float x, float y) { return pack_bf16(__float_as_uint(x), __float_as_uint(y)); };
+  const float ra = a - top(a), rb = b - top(b);
+  return {pack(a, b), pack(ra, rb), pack(ra - top(ra), rb - top(rb))};
+}
+
 // Sum (or larger) of a value over the four lanes c, c + 16, c + 32, c + 48.
 __device__ __forceinline__ float quarters_sum(float v) {
   v += __shfl_xor(v, 16);
@@ -481,7 +496,6 @@ struct Kv8Tile {
   bool nan;      // K's or V's block is NaN
   float kscale;  // 2^ke of K
   float ev;      // V's exponent
-  float ev_up;   // and that of the weights' scale
   float unit;    // 2^(mid - ev), what a weight counts in the denominator
 };
 
@@ -490,9 +504,9 @@ struct Kv8Tile {
 // scores^T = K Q^T and out^T = V^T W^T, so a lane keeps one query row (lane % 16) of each column
 // block and what it gets from the first product (keys 4 (lane / 16) + r of either tile) is the
 // operand of the second as it is.
-//   NC 0: 8 rows; columns 8 .. 15 hold the lo terms of the rows in 0 .. 7, one matrix instruction
-//     for both, and a row rotation by 8 adds them.
-//   NC 1: 16 rows, hi and lo one after the other.
+//   NC 0: 8 rows; columns 8 .. 15 hold the second terms of the rows in 0 .. 7, one matrix
+//     instruction for both, and a row rotation by 8 adds them.
+//   NC 1: 16 rows, a matrix instruction a term.
 //   NC 2: 32 rows, two column blocks of 16, for which K and V are made float16 once. Their two
 //     terms are made once too, a part by each wave, and read from LDS in every chunk: the 64
 //     registers of a wave's own copy at D = 128 would leave room for two waves a SIMD, not three
@@ -731,7 +745,6 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       now[x].nan = t_nan >> o & 1;
       now[x].kscale = of(t_kscale);
       now[x].ev = of(t_ev);
-      now[x].ev_up = now[x].ev + kKv8WUp;
       now[x].unit = of(t_unit);
     }
     // ---- scores of 32 keys
@@ -793,7 +806,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           if (key >= k_end || now[x].unused) vf[x][e] = make_uint2(0, 0);
         }
     }
-    v8h ph[NB], pl[NB];
+    constexpr int NT = SEP ? 3 : 2;  // matrix instructions for a weight's terms
+    v4u pw[NT][NB];
 #pragma unroll
     for (int y = 0; y < NB; y++) {
       // ---- the running reference
@@ -802,8 +816,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
       const float t0 = fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3]));
       const float t1 = fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3]));
       const float top = fmaxf(__builtin_fmaf(t0, c0, now[0].ev), __builtin_fmaf(t1, c1, now[1].ev));
-      if (__any(top > m[y])) {
-        const float mnew = fmaxf(m[y], ceilf(quarters_max(top)) + kKv8Head);
+      if (__any(top > m[y] + kKv8Head)) {
+        const float mnew = fmaxf(m[y], ceilf(quarters_max(top)));
         const float alpha = __builtin_amdgcn_exp2f(m[y] - mnew);
         m[y] = mnew;
         huge = huge || __any(fabsf(mnew) > 0x1p22f && mnew != kKv8None);
@@ -813,17 +827,17 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 #pragma unroll
           for (int e = 0; e < 4; e++) acc[y][j][e] *= alpha;
       }
-      // ---- weights, their sum, and their two terms
+      // ---- weights, their sum, and their terms
       const auto weights = [&](auto slow) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-          const float cc = x ? c1 : c0, off = now[x].ev_up - m[y];
+          const float cc = x ? c1 : c0, off = now[x].ev - m[y];
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             p[e] = __builtin_fmaf(s[y][x][e], cc, off);
             if constexpr (slow) {
-              if (huge) p[e] = (__builtin_fmaf(s[y][x][e], cc, now[x].ev) - m[y]) + kKv8WUp;
+              if (huge) p[e] = __builtin_fmaf(s[y][x][e], cc, now[x].ev) - m[y];
               p[e] = __builtin_amdgcn_exp2f(p[e]);
               // a block whose exponent is NaN counts where it is seen
               const bool seen = s[y][x][e] != -INFINITY;
@@ -836,15 +850,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           }
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
-            const h2v hi = pk_half(p[e], p[e + 1]);
-            const h2v lo = {half_rest(p[e], hi.x, minus1), half_rest(p[e + 1], hi.y, minus1)};
+            const Kv8Terms t = kv8_terms(p[e], p[e + 1]);
             if constexpr (SEP) {
-              ph[y][4 * x + e] = hi.x, ph[y][4 * x + e + 1] = hi.y;
-              pl[y][4 * x + e] = lo.x, pl[y][4 * x + e + 1] = lo.y;
+              pw[0][y][2 * x + e / 2] = t.hi, pw[1][y][2 * x + e / 2] = t.mid, pw[NT - 1][y][2 * x + e / 2] = t.lo;
             } else {
-              const h2v two = __builtin_bit_cast(
-                  h2v, c < 8 ? __builtin_bit_cast(uint32_t, hi) : __builtin_bit_cast(uint32_t, lo));
-              ph[y][4 * x + e] = two.x, ph[y][4 * x + e + 1] = two.y;
+              pw[0][y][2 * x + e / 2] = c < 8 ? t.hi : t.mid;
+              pw[1][y][2 * x + e / 2] = c < 8 ? t.lo : 0u;
             }
           }
         }
@@ -869,19 +880,17 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 #pragma unroll
       for (int y = 0; y < 2; y++) {
         const auto two = [&](uint32_t v) {
-          return y ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, true)
-                   : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v, 1.0f, false);
+          return y ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, true)
+                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, 1.0f, false);
         };
-        const h2v e0 = two(z[0][0]), e1 = two(z[0][1]), e2 = two(z[1][0]), e3 = two(z[1][1]);
-        const v8h vv = {e0.x, e0.y, e1.x, e1.y, e2.x, e2.y, e3.x, e3.y};
+        const v2bf e0 = two(z[0][0]), e1 = two(z[0][1]), e2 = two(z[1][0]), e3 = two(z[1][1]);
+        const v8bf vv = {e0.x, e0.y, e1.x, e1.y, e2.x, e2.y, e3.x, e3.y};
         const int o = 2 * b + y;
 #pragma unroll
-        for (int n = 0; n < NB; n++) acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph[n], acc[n][o], 0, 0, 0);
-        if constexpr (SEP) {
+        for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int n = 0; n < NB; n++)
-            acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl[n], acc[n][o], 0, 0, 0);
-        }
+            acc[n][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, __builtin_bit_cast(v8bf, pw[t][n]), acc[n][o], 0, 0, 0);
       }
     }
     if constexpr (more) load_v();
