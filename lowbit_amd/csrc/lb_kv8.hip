@@ -306,13 +306,23 @@ struct Kv8Cut {
 };
 
 // One class of a call's sequences, by their rows, and where its slices' sums lie in the workspace:
-// `sums` floats of them from `at` on, their scalars behind. Of a KV head at most `blocks` row
-// blocks and `units` slices. merge: workgroups a row block of the second launch, 0: one a row.
+// `sums` floats of them from `at` on, their scalars behind, and before them (4 bytes of 16) the
+// keys of a slice, which the first launch decides and the merge reads: the merge finds the sums
+// where they were written, whatever the compiler makes of the decision's float arithmetic.
+// Of a KV head at most `blocks` row blocks and `units` slices. merge: workgroups a row block of the
+// second launch, 0: one a row.
 struct Kv8Part {
   Kv8Cut cut;
   int blocks, units, merge;
   size_t at, sums;
 };
+
+__device__ __forceinline__ void kv8_put_cut(float *work, const Kv8Part &pt, int slice_keys) {
+  *reinterpret_cast<int *>(work + pt.at - 4) = slice_keys;
+}
+__device__ __forceinline__ int kv8_cut_of(const float *work, const Kv8Part &pt) {
+  return max(*reinterpret_cast<const int *>(work + pt.at - 4) & ~127, 128);  // (what kv8_slices takes, whatever it holds)
+}
 
 // r / G for 0 <= r < 2^32 / 2: the product is at most one too large.
 __device__ __forceinline__ int kv8_token(const Kv8Cut &c, int r) {
@@ -397,15 +407,13 @@ __device__ __forceinline__ int kv8_slices(int keys, int slice_keys) {
 }
 
 // Row block and slice of unit u; or, u a row block, that row block and the units before its
-// sequence's.
+// sequence's. By slices of w.slice_keys keys.
 struct Kv8Unit {
   Kv8Seq s;
   int rb, slice, slices, slice_keys, before, at;
 };
 template <bool BLOCK>
-__device__ __forceinline__ bool kv8_unit(const Kv8Args &a, const Kv8Cut &c, int u, Kv8Unit &w) {
-  const Kv8Seq first = kv8_seq(a, threadIdx.x & (kWave - 1));
-  w.slice_keys = kv8_slice_keys(a, c, first);
+__device__ __forceinline__ bool kv8_unit(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first, int u, Kv8Unit &w) {
   const auto blocks = [&](const Kv8Seq &s) { return kv8_row_blocks(c, s); };
   const auto slices = [&](const Kv8Seq &s) { return kv8_slices(kv8_keys(a, s), w.slice_keys); };
   const auto units = [&](const Kv8Seq &s) { return blocks(s) * slices(s); };
@@ -553,8 +561,11 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   float *part = work + pt.at;
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;
+  const Kv8Seq first = kv8_seq(a, lane);
   Kv8Unit w;
-  if (!kv8_unit<false>(a, cut, unit, w)) return;
+  w.slice_keys = kv8_slice_keys(a, cut, first);
+  if (unit == 0 && kv == 0 && threadIdx.x == 0) kv8_put_cut(work, pt, w.slice_keys);
+  if (!kv8_unit<false>(a, cut, first, unit, w)) return;
   const int place = unit - w.at + w.rb * w.slices + w.slice;  // in the workspace
   if (place >= pt.units) return;  // (rows of several sequences at once, which is not allowed)
   const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
@@ -1047,7 +1058,8 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   const int wr = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int rr = block % cut.R, idx = block / cut.R, kv = idx % a.KV;
   Kv8Unit w;
-  if (!kv8_unit<true>(a, cut, idx / a.KV, w)) return;
+  w.slice_keys = kv8_cut_of(work, pt);
+  if (!kv8_unit<true>(a, cut, kv8_seq(a, lane), idx / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
   if (ns < 2 || ro >= w.s.n * cut.G || w.before + (w.rb + 1) * ns > pt.units) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
@@ -1190,7 +1202,8 @@ __device__ __forceinline__ void kv8_merge(const Kv8Args &a, const Kv8Part &pt, i
   }
   const int idx = block / pt.merge, kv = idx % a.KV;
   Kv8Unit w;
-  if (!kv8_unit<true>(a, pt.cut, idx / a.KV, w) || w.slices < 2) return;
+  w.slice_keys = kv8_cut_of(work, pt);
+  if (!kv8_unit<true>(a, pt.cut, kv8_seq(a, threadIdx.x & (kWave - 1)), idx / a.KV, w) || w.slices < 2) return;
   if (w.before + (w.rb + 1) * w.slices > pt.units) return;
   const int rows = min(pt.cut.R, w.s.n * pt.cut.G - w.rb * pt.cut.R);
   for (int rr = block % pt.merge * ROWS + threadIdx.x / (D / 4); rr < rows; rr += pt.merge * ROWS)
@@ -1286,9 +1299,9 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     // a time, and where there are workgroups enough a whole row block one after the other, as each
     // finds its place anew (1000 tokens, 32 heads on 8: 39.6 us, with four a row block 44.3).
     p.merge = rows <= 512 ? 0 : blocks * a.KV >= 256 ? 1 : std::max(1, R * D / 1024);
-    p.at = plan.floats;
+    p.at = plan.floats + 4;
     p.sums = (size_t)units * a.KV * R * D;
-    plan.floats += p.sums + (size_t)units * a.KV * R * 4;
+    plan.floats = p.at + p.sums + (size_t)units * a.KV * R * 4;
     plan.parts++;
     return true;
   };
