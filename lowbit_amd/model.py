@@ -208,10 +208,20 @@ class KV8Cache:
         self.truncate(0, n)
 
     def truncate(self, seq: int, n: int = 0):
-        """Sequence `seq` keeps its first n tokens (pages past them return to the pool)."""
+        """Sequence `seq` keeps its first n tokens (pages past them return to the pool). The page that
+        the last of them lies in keeps its blocks' exponents: tokens that are appended to it later
+        are rounded in the unit that the dropped ones called for, and a block that a dropped token
+        made NaN stays NaN until the page is begun again (n a multiple of the page: at once)."""
+        if not 0 <= n <= self.lengths[seq]:
+            raise ValueError(f"sequence {seq} does not hold {n} tokens")
+        self.commit(seq, n)
+
+    def commit(self, seq: int, n: int):
+        """The first n positions of sequence `seq` hold its tokens, as a pass over positions that reserve
+        gave it has written them (pages past them return to the pool)."""
         keep = -(-int(n) // self.page)
         if n < 0 or keep > self._held[seq]:
-            raise ValueError(f"sequence {seq} does not hold {n} tokens")
+            raise ValueError(f"sequence {seq} has no pages for {n} tokens")
         gone = self._table[seq, keep:self._held[seq]]
         self._free.extend(int(p) for p in gone[::-1])
         if len(gone):
@@ -238,7 +248,7 @@ class KV8Cache:
             self._dirty = False
 
     def batch(self, q_start: int, past: int, seqs: int, max_new: int, rows: int) -> K.LbdKv8Batch:
-        """The lbd_kv8_batch of the first `seqs` sequences, with room for its attention in `work`."""
+        """The lbd_kv8_batch of the first `seqs` sequences (room: the workspace that its attention takes)."""
         return K.LbdKv8Batch(q_start, past, self.table.ptr, seqs, self.max_pages, max_new, rows)
 
     def room(self, b: K.LbdKv8Batch, heads: int):
@@ -544,6 +554,14 @@ class Model:
         a = np.array([p], np.int32)
         _check(self.L.lb_memcpy_h2d(self.pos.ptr, a.ctypes.data, 4), "pos upload")
 
+    @staticmethod
+    def _set_length(cache, n: int):
+        """A one-sequence cache after a pass that has written its first n tokens."""
+        if isinstance(cache, KV8Cache):
+            cache.commit(0, n)
+        else:
+            cache.length = n
+
     def _sync(self):
         _check(self.L.lb_stream_synchronize(self.stream), "synchronize")
 
@@ -576,7 +594,7 @@ class Model:
         self._step(T, cache, logits, argmax_hist=False)
         self._sync()
         if not own:
-            cache.length = pos + T
+            self._set_length(cache, pos + T)
         if logits == "last":
             return self.logits.to_array((cfg.vocab_size,), np.float32)
         if logits == "all":
@@ -637,7 +655,7 @@ class Model:
                 self._step(1, cache, "last", argmax_hist=True)
             self._sync()
         t2 = time.perf_counter()
-        cache.length = start + T + steps
+        self._set_length(cache, start + T + steps)
         out = self.hist.to_array((cache.capacity + 1,), np.int32)[start + T:start + T + n_new]
         if timings is not None:
             timings["prefill_s"] = t1 - t0
@@ -665,7 +683,7 @@ class Model:
                 cache.reserve(i, int(cache.lengths[i] + news[i]))
         except ValueError:
             for i in range(S):  # what the others had taken goes back
-                cache.truncate(i, int(cache.lengths[i]))
+                cache.commit(i, int(cache.lengths[i]))
             raise
         self._sync()
         if max(T, S) > self.tmax:
