@@ -253,7 +253,7 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
     }
   }
   // codes y 2^(127 - e), exact but for the rounding to E4M3; zeros in a NaN block
-  const float inv = __int_as_float((254 - min(e, 253)) << 23);
+  const float inv = __int_as_float(e < 254 ? (254 - e) << 23 : 0x00400000);  // 2^-127 is a subnormal
 #pragma unroll
   for (int i = 0; i < IT; i++) {
     const int it = tid + NT * i, tok = it / PER, el = 4 * (it % PER);

@@ -1,10 +1,10 @@
 """The paged 8-bit cache on the GPU where its numbers lie far apart: weights far below a row's
-largest, query elements far below a row's largest."""
+largest, query elements far below a row's largest, blocks of great exponents."""
 import numpy as np
 import pytest
 
 from oracle import kv_cache as O
-from test_gpu_kv8 import FILL, Device, batch_of
+from test_gpu_kv8 import FILL, Device, batch_of, same_pool
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,25 @@ def test_query_elements_far_below_the_largest(rng, call, bits):
     tol = (2 * (((D + 16) * 2.0 ** -24 + 2.0 ** -20) * a + floor) + 2.0 ** -19 + (keys / 32 + 64) * 2.0 ** -24) * v
     err = np.abs(got - ref)
     assert (err <= tol).all(), (np.nanmax(err / np.maximum(v, 1e-300)), np.nanmax(tol / np.maximum(v, 1e-300)))
+
+
+@pytest.mark.parametrize("old", [100, 200, 247, 253, 254])
+@pytest.mark.parametrize("D,n", [(64, 1), (128, 3)])
+def test_append_to_blocks_of_great_exponents(rng, D, n, old):
+    """Pages written by other means may hold any exponent: a later token's codes are in its unit."""
+    page, KV, H = 16, 2, 2
+    pages, q_start, past, table, T = batch_of(rng, page, [(5, n)])
+    pool = O.Pool(rng, pages, page, KV, D)
+    pool.k[:], pool.v[:] = O.e4m3_round(rng.uniform(-400, 400, (2,) + pool.k.shape))
+    pool.ke[:], pool.ve[:] = old, old
+    # values up to the unit times 256, or 2^126
+    qkv = (rng.uniform(-1, 1, (T, (H + 2 * KV) * D)) * 2.0 ** min(old - 119, 126)).astype(np.float32)
+    cos, sin = np.ones((40, D // 2), np.float32), np.zeros((40, D // 2), np.float32)
+    q = np.full((T, H * D), FILL)
+    dev, want = Device(pool, q_start, past, table, n, T), pool.copy()
+    got = dev.append(qkv, None, H, cos, sin, q)
+    want.append(q_start, past, table, n, qkv, None, H, cos, sin, q)
+    assert np.array_equal(got, q)
+    held = dev.held()
+    assert (held.ve[table[0, 0]] == old).all()
+    same_pool(held, want)
