@@ -486,10 +486,12 @@ int lbd_kv8_append(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const f
                    const float *sin_table, int max_pos, float *q_out, int q_stride,
                    void *stream);
 /* out rows = softmax(q k^T / sqrt(D)) v of the new tokens' query heads (rotated rows q,
- * H heads of D, row stride q_stride; float32 throughout) over their sequence's positions 0
- * .. their own, which the cache must hold: lbd_kv8_append first. A row whose positions are
- * on no page at all gets zeros. Rows of no sequence are left as they are. out must not
- * overlap q. Strides multiples of 4, q and out 16-byte aligned. work:
+ * H heads of D, row stride q_stride; float32 throughout, an element of q to 2^-38 of its
+ * head's largest) over their sequence's positions 0 .. their own, which the cache must hold:
+ * lbd_kv8_append first. A row whose positions are on no page at all gets zeros. Beside a
+ * block of V, those whose exponents are more than 100 below its may count as blocks of
+ * zeros, to rows of the call that do not see it as well. Rows of no sequence are left as
+ * they are. out must not overlap q. Strides multiples of 4, q and out 16-byte aligned. work:
  * lbd_kv8_attention_work_bytes of the same arguments (0: they are refused), 16-byte aligned;
  * it needs no clearing, and calls that share it must be ordered (one stream, or graphs that
  * are not replayed at once). Pages written by other means than lbd_kv8_append must hold no

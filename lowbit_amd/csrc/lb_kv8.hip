@@ -277,7 +277,7 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 // as they are, so that what a row sees of V decides its precision, however far apart the blocks'
 // exponents are. The denominator is sum w 2^(mid - ev), in the unit 2^(m - mid), with
 // mid 50 below the slice's largest ev: every factor stays within 2^+-50. Blocks of V more than
-// 2^100 below the largest (blocks of zeros among them) count as zeros.
+// 2^100 below the largest count as zeros.
 //
 // An E4M3 code is exact in float16 and in bf16, so the matrix products take codes as they are and
 // q and w in terms whose sum they are. q, two float16 terms: 22 bits of an element, and 2^-38 of its
@@ -676,7 +676,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     const int ve = max(t_ve, least);
     t_held = __ballot(t_ve >= 0);
     t_nan = __ballot(t_ke == 255 || t_ve == 255);
-    t_unused = __ballot(t_ve < max(least, 1));
+    t_unused = __ballot(t_ve < least);
     t_kscale = e8m0_to_f32((uint32_t)t_ke);
     t_ev = t_ve == 255 ? __builtin_nanf("") : (float)(ve - 127);
     t_unit = t_ve == 255 ? __builtin_nanf("") : __int_as_float((127 + imid - ve) << 23);

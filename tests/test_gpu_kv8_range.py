@@ -1,5 +1,5 @@
 """The paged 8-bit cache on the GPU where its numbers lie far apart: weights far below a row's
-largest, query elements far below a row's largest, blocks of great exponents."""
+largest, query elements far below a row's largest, blocks of the least and the greatest exponents."""
 import numpy as np
 import pytest
 
@@ -104,3 +104,27 @@ def test_append_to_blocks_of_great_exponents(rng, D, n, old):
     held = dev.held()
     assert (held.ve[table[0, 0]] == old).all()
     same_pool(held, want)
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("low,high", [(0, 0), (0, 60), (1, 90), (154, 254)])
+def test_value_blocks_of_extreme_exponents(rng, call, low, high):
+    """V's exponents from the least, 2^-127, to the greatest: blocks within 2^100 of the sequence's
+    largest count in full, alone and beside each other. Keys are zeros: each counts alike. Outputs below 2^-126 are
+    float32 subnormals, off by 2^-149."""
+    D, KV, H, seqs = CALLS[call]
+    pages, q_start, past, table, T = batch_of(rng, 32, seqs, 2, 1)
+    pool = O.Pool(rng, pages, 32, KV, D)
+    pool.k[:], pool.ke[:] = 0, 120
+    pool.v[:] = O.e4m3_round(np.clip(rng.standard_normal(pool.v.shape) * 130, -448, 448) / (64 if high == 254 else 1))
+    pool.ve[:] = low
+    for b in range(len(seqs)):  # every third block of a sequence
+        pool.ve[table[b, 2::3]] = high
+    q = rng.standard_normal((T, H * D)).astype(np.float32)
+    most = max(n for _, n in seqs)
+    got = Device(pool, q_start, past, table, most, T).attention(q, H, H * D)
+    ref = np.full(got.shape, FILL, np.float64)
+    _, v, keys = np.moveaxis(np.repeat(pool.attention(q_start, past, table, most, q, H, ref), D, 1), 2, 0)
+    tol = (2.0 ** -19 + (keys / 32 + 64) * 2.0 ** -24) * v + 2.0 ** -149
+    err = np.abs(got - ref)
+    assert (err <= tol).all(), (np.nanmax(err / np.maximum(v, 1e-300)), np.nanmax(tol / np.maximum(v, 1e-300)))
