@@ -290,6 +290,8 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 constexpr int kKv8GridY = 1 << 15;  // units of a call in the grid's second dimension
 constexpr float kKv8Head = 8.0f;  // x + ev may lie this far above the reference: few new ones are needed
 constexpr int kKv8Waves = 4;       // of an attention workgroup
+// Floats before a class's sums: 256 bytes, as sums 16 bytes off the cache lines cost 61 steps 0.8 of 59 us.
+constexpr int kKv8CutHead = 64;
 constexpr int kKv8Spread = 100;    // exponents of V below the largest that still count
 // The reference before any key: finite, so that masked scores of -inf weigh exp2(-inf) = 0 under it.
 constexpr float kKv8None = -3.4028234663852886e38f;
@@ -306,7 +308,7 @@ struct Kv8Cut {
 };
 
 // One class of a call's sequences, by their rows, and where its slices' sums lie in the workspace:
-// `sums` floats of them from `at` on, their scalars behind, and before them (4 bytes of 16) the
+// `sums` floats of them from `at` on, their scalars behind, and kKv8CutHead floats before them the
 // keys of a slice, which the first launch decides and the merge reads: the merge finds the sums
 // where they were written, whatever the compiler makes of the decision's float arithmetic.
 // Of a KV head at most `blocks` row blocks and `units` slices. merge: workgroups a row block of the
@@ -318,10 +320,11 @@ struct Kv8Part {
 };
 
 __device__ __forceinline__ void kv8_put_cut(float *work, const Kv8Part &pt, int slice_keys) {
-  *reinterpret_cast<int *>(work + pt.at - 4) = slice_keys;
+  *reinterpret_cast<int *>(work + pt.at - kKv8CutHead) = slice_keys;
 }
 __device__ __forceinline__ int kv8_cut_of(const float *work, const Kv8Part &pt) {
-  return max(*reinterpret_cast<const int *>(work + pt.at - 4) & ~127, 128);  // (what kv8_slices takes, whatever it holds)
+  // (whatever it holds, a number that kv8_slices takes)
+  return max(*reinterpret_cast<const int *>(work + pt.at - kKv8CutHead) & ~127, 128);
 }
 
 // r / G for 0 <= r < 2^32 / 2: the product is at most one too large.
@@ -564,7 +567,6 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const Kv8Seq first = kv8_seq(a, lane);
   Kv8Unit w;
   w.slice_keys = kv8_slice_keys(a, cut, first);
-  if (unit == 0 && kv == 0 && threadIdx.x == 0) kv8_put_cut(work, pt, w.slice_keys);
   if (!kv8_unit<false>(a, cut, first, unit, w)) return;
   const int place = unit - w.at + w.rb * w.slices + w.slice;  // in the workspace
   if (place >= pt.units) return;  // (rows of several sequences at once, which is not allowed)
@@ -937,6 +939,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     }
   }
   if (lane == 0) lds.smid[wave] = mid;
+  if (unit == 0 && kv == 0 && threadIdx.x == 0) kv8_put_cut(work, pt, w.slice_keys);
   __syncthreads();
   const size_t pu = (size_t)place * a.KV + kv;
   float *po = part + pu * R * D;
@@ -1061,7 +1064,7 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   w.slice_keys = kv8_cut_of(work, pt);
   if (!kv8_unit<true>(a, cut, kv8_seq(a, lane), idx / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
-  if (ns < 2 || ro >= w.s.n * cut.G || w.before + (w.rb + 1) * ns > pt.units) return;
+  if (ns < 2 || ro >= w.s.n * cut.G || w.before + (w.rb + 1ll) * ns > pt.units) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
   const float4 *sc = reinterpret_cast<const float4 *>(work + pt.at + pt.sums) + pu * cut.R + rr;
   const float4 *v = reinterpret_cast<const float4 *>(work + pt.at) + (pu * cut.R + rr) * LPR + e4;
@@ -1204,7 +1207,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8Args &a, const Kv8Part &pt, i
   Kv8Unit w;
   w.slice_keys = kv8_cut_of(work, pt);
   if (!kv8_unit<true>(a, pt.cut, kv8_seq(a, threadIdx.x & (kWave - 1)), idx / a.KV, w) || w.slices < 2) return;
-  if (w.before + (w.rb + 1) * w.slices > pt.units) return;
+  if (w.before + (w.rb + 1ll) * w.slices > pt.units) return;
   const int rows = min(pt.cut.R, w.s.n * pt.cut.G - w.rb * pt.cut.R);
   for (int rr = block % pt.merge * ROWS + threadIdx.x / (D / 4); rr < rows; rr += pt.merge * ROWS)
     kv8_merge_row<D>(a, pt, w, kv, rr, work, out, out_stride);
@@ -1299,7 +1302,7 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     // a time, and where there are workgroups enough a whole row block one after the other, as each
     // finds its place anew (1000 tokens, 32 heads on 8: 39.6 us, with four a row block 44.3).
     p.merge = rows <= 512 ? 0 : blocks * a.KV >= 256 ? 1 : std::max(1, R * D / 1024);
-    p.at = plan.floats + 4;
+    p.at = plan.floats + kKv8CutHead;
     p.sums = (size_t)units * a.KV * R * D;
     plan.floats = p.at + p.sums + (size_t)units * a.KV * R * 4;
     plan.parts++;

@@ -9,13 +9,14 @@ from lowbit_amd import kernels as K
 from test_gpu_kv8 import FILL, Device, batch_of, cached, ok
 
 pytestmark = pytest.mark.gpu
+HEAD = 64  # words before the sums
 
 
 @pytest.mark.parametrize("D,KV,H,seqs,R", [
     (64, 1, 4, [(3000, 1)], 8), (128, 2, 8, [(5000, 1)], 8), (32, 1, 16, [(9000, 1)], 16), (64, 2, 4, [(2500, 70)], 32),
     (128, 1, 2, [(6000, 16)], 32)], ids=str)
 def test_the_cut_stands_in_the_workspace(rng, D, KV, H, seqs, R):
-    """One sequence's workspace: 16 bytes that begin with a slice's keys, then for every slice of every row
+    """One sequence's workspace: 256 bytes that begin with a slice's keys, then for every slice of every row
     block and KV head the rows' sums, then their scalars (reference, unit, its mid, denominator). The
     slices that the first word tells, added in 64 bits, are the output."""
     (past, n), G = seqs[0], H // KV
@@ -28,13 +29,13 @@ def test_the_cut_stands_in_the_workspace(rng, D, KV, H, seqs, R):
     ok(L.lbd_kv8_attention(C.byref(dev.pool), C.byref(dev.batch), dq.ptr, H * D, H, do.ptr, H * D, ws.ptr, need, None))
     ok(L.lb_dev_synchronize())
     words = ws.to_array((need // 4,), np.float32)
-    units = (need // 4 - 4) // (KV * R * (D + 4))
-    assert 4 + units * KV * R * (D + 4) == need // 4
+    units = (need // 4 - HEAD) // (KV * R * (D + 4))
+    assert HEAD + units * KV * R * (D + 4) == need // 4
     keys, cut = past + n, int(words[:1].view(np.int32)[0])
     blocks, slices = -(-n * G // R), -(-keys // cut)
     assert cut % 128 == 0 and 1 < slices and blocks * slices <= units
-    sums = words[4:4 + units * KV * R * D].reshape(units, KV, R, D).astype(np.float64)
-    m, um, mid, den = np.moveaxis(words[4 + units * KV * R * D:].reshape(units, KV, R, 4).astype(np.float64), 3, 0)
+    sums = words[HEAD:HEAD + units * KV * R * D].reshape(units, KV, R, D).astype(np.float64)
+    m, um, mid, den = np.moveaxis(words[HEAD + units * KV * R * D:].reshape(units, KV, R, 4).astype(np.float64), 3, 0)
     got = do.to_array(q.shape, np.float32).reshape(n, KV, G, D)
     for r in range(n * G):
         at = slice(r // R * slices, r // R * slices + slices)
