@@ -953,10 +953,10 @@ hipError_t launch_split3(int fmt, const float *x, int M, int Kp, uint4 *x3, hipS
 // row). The row is scaled by 2^E, E chosen so that its largest magnitude lands in
 // [2^14, 2^15) (E = 0 for a zero or non-finite row); then xs = x 2^E = hi + lo 2^-11
 // with hi = fp16(xs) and lo = fp16((xs - hi) 2^11) (the remainder is exact in fp32;
-// the 2^11 keeps lo clear of float16's subnormals, which the matrix cores flush, for
+// the 2^11 keeps lo clear of float16's subnormals, counted as zeros here, for
 // |xs| >= 2^-3). So an element keeps 22 significant bits within 2^17 of the row's
 // largest, has an absolute error of at most 2^-39 of the largest down to 2^28 below
-// it, and is dropped below that. Slots as in split3_kernel's W4A16 tiles, two terms
+// it, and may count for nothing below that. Slots as in split3_kernel's W4A16 tiles, two terms
 // per slot.
 // Workgroups (m, p) of a row each take the row's maximum over all of it (from the
 // caches after the first) and split part p of its slots.

@@ -152,8 +152,8 @@ __device__ __forceinline__ void rope4_pair(float4 &a, float4 &b, float4 c, float
 //   the others: 8 NT elements of a row's query heads, rotated into q_out.
 //
 // What bounds it: a step, the launch and three loads one after the other (the batch, the page, the
-// block's exponent): one token of 14 heads on 2 2.6 us, 64 sequences of 32 heads on 8 3.4 us.
-// Prompts, the bytes: 4 sequences of up to 1000 tokens, 32 heads on 8, 45.8 MB in 10.7 us = 4.3
+// block's exponent): one token of 14 heads on 2 2.6 us, 64 sequences of 32 heads on 8 3.2 us.
+// Prompts, the bytes: 4 sequences of up to 1000 tokens, 32 heads on 8, 45.8 MB in 10.6 us = 4.3
 // TB/s (a large copy reaches 5.2). A block is one workgroup's so that its largest element costs no
 // second pass over the rows and no atomic, and codes leave as whole words.
 //
@@ -284,8 +284,8 @@ __global__ __launch_bounds__(NT) void kv8_append_kernel(Kv8Args a, const float *
 // row's largest where that is more (the matrix cores take float16's subnormals as they are). w, three
 // bf16 terms: all 24 bits however far it lies below the largest, as the keys that it outweighs may
 // hold the larger values (two float16 terms lost weights e^-17 below the row's largest, and those
-// e^-30 below it altogether; 2048 tokens of 32 heads took 86.3 us so, 93.8 now. Two bf16 terms,
-// rounded: 85.0, but errors of 2e-6 to 7e-6 in place of 4e-7 to 1.2e-6).
+// e^-30 below it altogether; three bf16 terms made 2048 tokens of 32 heads 9 % slower. Two of them,
+// rounded: 1 % faster, but errors of 2e-6 to 7e-6 in place of 4e-7 to 1.2e-6).
 
 constexpr int kKv8GridY = 1 << 15;  // units of a call in the grid's second dimension
 constexpr float kKv8Head = 8.0f;  // x + ev may lie this far above the reference: few new ones are needed
@@ -349,19 +349,19 @@ __host__ __device__ constexpr int kv8_rows(int nc) { return nc ? 16 * nc : 8; }
 //
 // Few rows (the cache's bytes bound them): the batch's row blocks times keys over the slots, so
 // that however the lengths differ the slices are alike. Few row blocks (alike, mostly) get 512
-// slices in all, two a compute unit: 60000 keys of 8 KV heads 30 us, with 1024 34 (more sums to
-// merge); many get 2048: 61 sequences of 50 to 4096 keys 59.8 us, with 1024 62, with 512 64.
+// slices in all, two a compute unit: 60000 keys of 8 KV heads 28.6 us, with 1024 32.5 (more sums to
+// merge); many get 2048: 61 sequences of 50 to 4096 keys 59.0 us, with 1024 60.1, with 512 61.9.
 //
 // Many rows (the instructions bound them): the mean row block's keys in ns slices, lane ns - 1
 // weighing what they cost, in keys. For one sequence, whose slices are alike: a slice's keys and
 // 512 for a workgroup's beginning and end, times 0.72 k + 0.25 with k workgroups on the fullest
 // compute unit (measured 1, 1.5, 2.4), and the sums' way to the merge. (200 tokens behind 8000, 25
-// row blocks of 8 KV heads: five slices 72 us, four 82, three 74; 64 behind 8000, 8 row blocks:
-// four 31 us, six 36; 300 behind 2000 on 2 KV heads: three even slices 19.7 us, 1024 + 1024 + 252
-// keys 22.1; 1000 tokens, 219 row blocks of 2: one 16.5 us, two 21.8.) For several, whose slices
-// fill the units as they come: the rounds that the device takes, the last two thirds where it
-// fills half of it (3 of up to 100 tokens behind 6000, 32 heads on 8: 39 us, by the other 43.5; 16
-// of up to 40 behind 3000: 36 and 41.7).
+// row blocks of 8 KV heads: five slices 74.9 us, four 87.4, three 82.1; 64 behind 8000, 8 row
+// blocks: four 33.0 us, six 36.6, three 39.1; 300 behind 2000 on 2 KV heads: three even slices 20.5
+// us, 1024 + 1024 + 252 keys 25.0; 1000 tokens, 219 row blocks of 2: one 17.1 us, two 22.3.) For
+// several, whose slices fill the units as they come: the rounds that the device takes, the last two
+// thirds where it fills half of it (3 of up to 100 tokens behind 6000, 32 heads on 8: 41.6 us, by
+// the other rule 45.2; 16 of up to 40 behind 3000: 38.6 and 44.3).
 //
 // Slices are never more than slots and row blocks together: the few's sum in float 1 % up, the
 // many's product 2 %.
@@ -521,7 +521,7 @@ struct Kv8Tile {
 //   NC 2: 32 rows, two column blocks of 16, for which K and V are made float16 once. Their two
 //     terms are made once too, a part by each wave, and read from LDS in every chunk: the 64
 //     registers of a wave's own copy at D = 128 would leave room for two waves a SIMD, not three
-//     (24 sequences of prompts and steps, 14 heads on 2 of 64: 40.7 us, so 34.1).
+//     (24 sequences of prompts and steps, 14 heads on 2 of 64, took 19 % longer with them).
 // K is read 16 bytes a lane (8 at D = 32), V D / 16 bytes a lane of eight keys: a lane's bytes
 // of two keys are interleaved by v_perm on their way to float16, which is all the transposing
 // that V needs, and its output elements come out contiguous. The next chunk's K is requested
@@ -529,14 +529,14 @@ struct Kv8Tile {
 // LDS lies between them and the matrix cores.
 //
 // What bounds it. Few rows, the cache's bytes: 61 sequences of 50 to 4096 keys, 32 heads on 8 of
-// 128, 254 MB in 52 us and 5 for the merge, 4.3 to 4.5 TB/s; one of 60000 keys 25 us and 5. (Three waves a
-// SIMD at D = 128: with registers for four the loop spills, 72 us against 59.) Short ones, the
-// launch and four loads one after the other (batch, page, exponents beside codes): 700 keys 7.6 us.
-// Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 86 us, 400 TFLOP/s of the
-// formula, twice that in products of two terms (a large float16 product reaches 1180). The matrix
-// cores are busy for a third of the time and the vector units for two thirds, 4 of 10 of whose
-// instructions belong to the waves' beginnings and ends; the two kinds hardly overlap, and loads
-// cost 5 %. Tried and slower or alike: products of 32 x 32 x 16 (0 to 6 %), the next chunk's scores
+// 128, 254 MB in 54 us and 5 for the merge, 4.7 TB/s; one of 60000 keys 25 us and 5. (Three waves a
+// SIMD at D = 128: with registers for four the loop spills, 22 % slower.) Short ones, the launch and
+// four loads one after the other (batch, page, exponents beside codes): 700 keys 7.8 us.
+// Many rows, the instructions: 2048 tokens of 32 heads on 8 of 128 91 us, 376 TFLOP/s of the
+// formula, 2.5 times that in products of terms (a large float16 product reaches 1180). The matrix
+// cores are busy for 38 % of the time; a wave issues 2300 vector instructions, 370 of them matrix
+// ones, more than a third of the others in its beginning and end; the two kinds hardly overlap.
+// Tried and slower or alike: products of 32 x 32 x 16 (0 to 6 %), the next chunk's scores
 // beside this one's weights (0 to 40 %, it spills), matrix and vector instructions alternated by
 // scheduling barriers, both column blocks' weights in one stretch (3 %), two waves a workgroup (1
 // to 15 %), the place of a workgroup found by one of its waves (1 %).
@@ -1023,8 +1023,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 
 // One class of sequences, or (MIXED) two in one launch, of many rows (NC = 2) and then of few
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
-// (24 sequences of prompts and steps, 14 heads on 2: two launches and two merges one after the
-// other 57 us, one of each 45, by now 34; 8 of up to 1100, 32 heads on 8: 35 and 28, few rows first 36).
+// (24 sequences of prompts and steps, 14 heads on 2: 36.6 us; two launches and two merges one after
+// the other took 27 % longer, 8 of up to 1100, 32 heads on 8, 25 %, and few rows first 29 %).
 template <int D, int NC, bool MIXED>
 __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
@@ -1049,8 +1049,8 @@ __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend
 //
 // Few rows: a workgroup a row. Lane s of every wave holds slice s's scalars (m, the denominator's
 // unit and it), and the D-element sums, 256 / D slices to a wave load, go round the four waves,
-// eight loads requested before the scalars are waited for (118 slices of 32 rows: a wave a row
-// took 22.8 us, this 6.4).
+// eight loads requested before the scalars are waited for (64 slices of 8 KV heads' rows: 4.7 us; a
+// wave a row took 3.5 times as long).
 template <int D>
 __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &pt, int block,
                                                const float *__restrict__ work, float4 (*sh)[D / 4],
@@ -1142,7 +1142,8 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
 
 // Many rows: D / 4 lanes a row, 1024 / D rows a workgroup at a time, `groups` workgroups a row
 // block. Eight slices at a time, all of their loads in flight together and nothing exchanged
-// between lanes (200 rows of 8200 keys in five slices, 32 heads: 13.9 us a wave a row, 6.3 so).
+// between lanes (200 rows of 8200 keys in five slices, 32 heads: 7.4 us; a wave a row took twice as
+// long).
 template <int D>
 __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &pt, const Kv8Unit &w, int kv, int rr,
                                               const float *__restrict__ work, float *__restrict__ out,
@@ -1298,9 +1299,9 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     p.blocks = (int)blocks;
     p.units = (int)units;
     // Few rows (of many slices): a workgroup a row (but 16 sequences of up to 2000
-    // keys and 4 tokens, 32 heads on 8, 2048 rows: 16.2 us, a workgroup a row 21.1). Many: 1024 / D rows at
+    // keys and 4 tokens, 32 heads on 8, 2048 rows: 16.0 us, a workgroup a row 20.6). Many: 1024 / D rows at
     // a time, and where there are workgroups enough a whole row block one after the other, as each
-    // finds its place anew (1000 tokens, 32 heads on 8: 39.6 us, with four a row block 44.3).
+    // finds its place anew (1000 tokens, 32 heads on 8: 37.6 us, with four a row block 40.2).
     p.merge = rows <= 512 ? 0 : blocks * a.KV >= 256 ? 1 : std::max(1, R * D / 1024);
     p.at = plan.floats + kKv8CutHead;
     p.sums = (size_t)units * a.KV * R * D;
