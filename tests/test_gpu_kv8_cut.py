@@ -48,3 +48,42 @@ def test_the_cut_stands_in_the_workspace(rng, D, KV, H, seqs, R):
             # float32: a factor, a division, and one addition a slice of sums that may be larger than theirs
             size = (np.abs(sums[at, h, r % R]) * np.exp2(M - top)[:, None]).sum(0) * np.abs(want / num)
             assert (np.abs(have - want) <= (slices + 16) * 2.0 ** -24 * size).all()
+
+
+def test_graphs_that_share_a_workspace(rng):
+    """Three recorded calls that are cut differently, replayed in turn on one stream with one workspace (on the
+    16 bytes that it has to be aligned to), eager calls on another between them."""
+    D, page, KV, H = 64, 32, 2, 8
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    s = C.c_void_p()
+    ok(L.lb_stream_create(C.byref(s)))
+    runs = []
+    for seqs in ([(3000, 1), (5, 1)], [(700, 90), (0, 40), (2000, 1)], [(9000, 20)]):
+        pages, q_start, past, table, T = batch_of(rng, page, seqs)
+        pool = cached(rng, pages, page, KV, D, table, seqs)
+        q = rng.standard_normal((T, H * D)).astype(np.float32)
+        dev = Device(pool, q_start, past, table, max(n for _, n in seqs), T)
+        runs.append((dev, q, up(q), up(np.full(q.shape, FILL)), dev.attention(q, H, H * D)))
+    need = max(L.lbd_kv8_attention_work_bytes(C.byref(d.pool), C.byref(d.batch), H) for d, *_ in runs)
+    ws, graphs = K.DeviceBuffer(need + 16), []
+    for dev, q, dq, do, _ in runs:
+        ex = C.c_void_p()
+        ok(L.lb_stream_begin_capture(s.value))
+        ok(L.lbd_kv8_attention(C.byref(dev.pool), C.byref(dev.batch), dq.ptr, H * D, H, do.ptr, H * D, ws.ptr + 16,
+                               need, s.value))
+        ok(L.lb_stream_end_capture(s.value, C.byref(ex)))
+        graphs.append(ex)
+    fill = np.full(max(q.size for _, q, *_ in runs), FILL)
+    for turn in range(4):
+        for _, q, _, do, _ in runs:
+            ok(L.lb_memcpy_h2d(do.ptr, fill.ctypes.data, q.nbytes))
+        for i in (0, 1, 2, 1, 0, 2):
+            ok(L.lb_graph_launch(graphs[i].value, s.value))
+        for dev, q, _, _, want in runs:
+            assert np.array_equal(dev.attention(q, H, H * D), want)
+        ok(L.lb_stream_synchronize(s.value))
+        for _, q, _, do, want in runs:
+            assert np.array_equal(do.to_array(q.shape, np.float32), want)
+    for ex in graphs:
+        ok(L.lb_graph_destroy(ex.value))
+    ok(L.lb_stream_destroy(s.value))

@@ -128,3 +128,28 @@ def test_value_blocks_of_extreme_exponents(rng, call, low, high):
     tol = (2.0 ** -19 + (keys / 32 + 64) * 2.0 ** -24) * v + 2.0 ** -149
     err = np.abs(got - ref)
     assert (err <= tol).all(), (np.nanmax(err / np.maximum(v, 1e-300)), np.nanmax(tol / np.maximum(v, 1e-300)))
+
+
+@pytest.mark.parametrize("nats", [0, 12, 30, 55, 75])
+@pytest.mark.parametrize("call", CALLS)
+def test_pages_of_zero_values_that_take_the_weight(rng, call, nats):
+    """As append leaves a page whose values are zeros: exponent 0, 120 below the others'. Every fourth page is
+    one, its keys `nats` above the rest.
+
+    Tolerance as in test_keys_far_below_the_largest."""
+    D, KV, H, seqs = CALLS[call]
+    pool, q_start, past, table, T = sinks(rng, D, KV, seqs, (), 0)
+    for b in range(len(seqs)):
+        pg = table[b, 0::4]
+        pool.k[pg[pg >= 0], :, :, 0] = 0x7E
+        pool.v[pg[pg >= 0]], pool.ve[pg[pg >= 0]] = 0, 0
+    q = np.zeros((T, H * D), np.float32)
+    q[:, 0::D] = nats * np.sqrt(D) / (448 * 2.0 ** (119 - 127))
+    q[:, 1::D] = rng.uniform(-1, 1, (T, H)) * np.sqrt(D)
+    most = max(n for _, n in seqs)
+    got = Device(pool, q_start, past, table, most, T).attention(q, H, H * D)
+    ref = np.full(got.shape, FILL, np.float64)
+    a, v, keys = np.moveaxis(np.repeat(pool.attention(q_start, past, table, most, q, H, ref), D, 1), 2, 0)
+    tol = (18 * 2.0 ** -24 * a + 2.0 ** -19 + (keys / 32 + 64) * 2.0 ** -24) * v
+    err = np.abs(got - ref)
+    assert (err <= tol).all(), (np.nanmax(err / np.maximum(v, 1e-300)), np.nanmax(tol / np.maximum(v, 1e-300)))
