@@ -502,6 +502,80 @@ int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, cons
                       int q_stride, int H, float *out, int out_stride, void *work,
                       size_t work_bytes, void *stream);
 
+/* lbd_kv8_attention of a window: a row at position p sees the positions x <= p of its
+ * sequence with p - x < window or x < sinks (window >= 1, sinks >= 0: the window and a few
+ * first tokens that stay visible). Only pages that hold such a position are read, so that the
+ * table's entries for the others may be -1 (pages given back to the pool). Everything else as
+ * lbd_kv8_attention; work: lbd_kv8_attention_window_work_bytes of the same arguments. */
+size_t lbd_kv8_attention_window_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch,
+                                           int H, int window, int sinks);
+int lbd_kv8_attention_window(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q,
+                             int q_stride, int H, int window, int sinks, float *out, int out_stride,
+                             void *work, size_t work_bytes, void *stream);
+/* Page dst[i] of each of the n_pools pools (a decoder's layers: the same pages, page, KV and D
+ * in all) becomes a copy of page src[i], codes and exponents, i < n. src and dst [n] in device
+ * memory, so that a recorded graph replays with other pages; a pair with an entry outside
+ * [0, pages) is skipped. No page may be dst twice, nor dst of one pair and src of another (in
+ * such a pair what the page holds is not defined); src may repeat. `pools` is host memory, read
+ * before the call returns. n == 0 does nothing. */
+int lbd_kv8_copy_pages(const lbd_kv8_pool *pools, int n_pools, const int32_t *src,
+                       const int32_t *dst, int n, void *stream);
+
+/* ---- beam search on the device (no lowbit.h counterpart: the reference decodes greedily,
+ *      src/lowbit/model.py:437-458). Place i = b W + w of the B W places is beam w of prompt b. ---- */
+typedef struct {
+  const float *score;  /* [B W] the beam's sum of log-probabilities; -inf or NaN: no beam here */
+  const int32_t *done; /* [B W] not 0: the beam has ended; NULL: none has */
+  float *new_score;    /* [B W], may be score */
+  int32_t *new_done;   /* [B W], may be done */
+  int32_t *tok;        /* [B W] the token that the place's new beam ends in */
+  int32_t *parent;     /* [B W] the place of the beam that it continues, -1: no beam here */
+  int32_t *hist_tok;   /* [hist_len][B W] tok and parent of each step, with step; all three NULL: */
+  int32_t *hist_parent; /* not recorded */
+  int32_t *step;       /* [B] steps so far: step s < hist_len is recorded in row s, then s + 1 */
+  int hist_len;
+  int B, W; /* prompts, and beams of each: 1 <= W <= LBD_MAX_BEAMS, B W <= 2^20 */
+  int V;    /* vocabulary, at most 2^24 */
+  int eos;  /* a beam that takes this token has ended; -1: none does */
+} lbd_beams;
+#define LBD_MAX_BEAMS 32
+/* One step of beam search: logits [B W, V] (row stride ld floats) of the places' beams. A beam
+ * of sum s and logits x offers, for every token v, the sum s + x[v] - log(sum exp x); one that
+ * has ended offers itself, with its sum. The W largest of a prompt's offers, in descending order,
+ * are its new beams. Equal sums: the lower place first, within a beam the larger logit, then the
+ * lower token. Sums are compared in float64 and rounded to float32 once; sum exp x is added in
+ * float32. An offer of -inf (a masked token) is none; a beam whose logits hold a NaN or +inf, or
+ * are all -inf, offers nothing; rows of ended beams and of no beam are not read. Where fewer than
+ * W are offered the last places get parent -1, sum -inf. tok of an ended beam and of no beam is
+ * eos (0 without one), a token that may be embedded like any other. work:
+ * lbd_beam_select_work_bytes of the same arguments (0: they are refused), 16-byte aligned; it
+ * needs no clearing, and calls that share it must be ordered. */
+size_t lbd_beam_select_work_bytes(const lbd_beams *beams);
+int lbd_beam_select(const float *logits, int ld, const lbd_beams *beams, void *work,
+                    size_t work_bytes, void *stream);
+/* The beams' sequences in a paged cache follow their parents. All arrays in device memory. */
+typedef struct {
+  const int32_t *parent; /* [B W] as lbd_beam_select's: a place of the same prompt, else no sequence */
+  const int32_t *done;   /* [B W] not 0: the new beam has ended and holds no sequence; NULL: none */
+  const int32_t *past;   /* [B W] tokens that each sequence held before the last pass; < 0: none */
+  const int32_t *table;  /* [B W][max_pages] the sequences' pages */
+  const int32_t *own;    /* [B W][max_pages] the pages that a place may begin (see below), else -1 */
+  int32_t *new_past;     /* [B W] past of the parent + add; -1 without a sequence */
+  int32_t *new_table;    /* [B W][max_pages], not overlapping table */
+  int B, W, max_pages;   /* 1 <= W <= LBD_MAX_BEAMS, B W <= 2^20 */
+  int add;               /* tokens that the last pass appended to each sequence, >= 0 */
+} lbd_kv8_order;
+/* new_table and new_past of every place, and in each of the n_pools pools the copies that they
+ * call for. A sequence shares its parent's full pages. The page that is being written (past + add
+ * not a multiple of the page) stays with the first place that continues the parent; for each
+ * other one its tokens are copied, slots behind them left as they are, into a page that no
+ * first place keeps: of own[i][that index], i the prompt's places in order, the next one. Pages
+ * behind it are own's of the place itself. Places without a sequence get entries of -1. So with
+ * own's pages all different, and a prompt's first page in writing among them, every sequence
+ * writes to pages of its own, however parents change. pools as for lbd_kv8_copy_pages. */
+int lbd_kv8_reorder(const lbd_kv8_pool *pools, int n_pools, const lbd_kv8_order *order,
+                    void *stream);
+
 /* ---- device plumbing for the ctypes layer and benchmarks ---- */
 int lb_dev_malloc(void **ptr, size_t bytes);
 int lb_dev_free(void *ptr);

@@ -1542,6 +1542,64 @@ int kv8_pointers(const lbk::Kv8Args &a) {
   return 0;
 }
 
+// Attention over the pool by arguments that kv8_args has taken.
+int kv8_attend(const lbk::Kv8Args &a, int D, const float *q, int q_stride, int H, float *out, int out_stride,
+               void *work, size_t work_bytes, void *stream) {
+  if (q_stride % 4 || out_stride % 4 || q_stride < (long long)H * D || out_stride < (long long)H * D)
+    return fail(LB_ERR_SHAPE, "bad shape: strides are multiples of 4 floats that hold a row");
+  if (!q || !out) return fail(LB_ERR_ARG, "null pointer");
+  const int rc = kv8_pointers(a);
+  if (rc < 0) return rc;
+  if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ARG, "q and out must be 16-byte aligned");
+  const size_t need = lbk::kv8_attention_work_bytes(a, D, H);
+  if (!need) return fail(LB_ERR_SHAPE, "too many rows of heads for a launch");
+  if (!work || work_bytes < need) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
+  if (!aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
+  LB_LAUNCH(lbk::launch_kv8_attention(a, D, q, q_stride, H, out, out_stride, work, static_cast<hipStream_t>(stream)),
+            "kv8 attention launch");
+}
+
+int kv8_window(lbk::Kv8Args &a, int window, int sinks) {
+  if (window <= 0 || sinks < 0) return fail(LB_ERR_SHAPE, "bad shape: window of at least 1, sinks of at least 0");
+  a.window = window;  // (positions may lie past the table, so it may count for more than the table holds)
+  a.sinks = std::min(sinks, a.max_pages << a.page_shift);
+  return 0;
+}
+
+// The pools of a decoder's layers, from `first` on as many as a launch takes.
+int kv8_layers(const lbd_kv8_pool *pools, int n, int first, lbk::Kv8Layers &l) {
+  if (!pools) return fail(LB_ERR_ARG, "null pointer");
+  if (n <= 0) return fail(LB_ERR_SHAPE, "bad shape");
+  const lbd_kv8_pool &p = pools[0];
+  int shift = 4, d_shift = 5;
+  while (shift < 7 && (1 << shift) != p.page) shift++;
+  while (d_shift < 7 && (1 << d_shift) != p.D) d_shift++;
+  if ((1 << shift) != p.page || (1 << d_shift) != p.D || p.pages <= 0 || p.KV <= 0 || p.KV > 65535)
+    return fail(LB_ERR_SHAPE, "bad shape: pages of 16, 32, 64 or 128 tokens, heads of 32, 64 or 128");
+  l.n = std::min(n - first, lbk::kKv8Layers);
+  l.pages = p.pages, l.page_shift = shift, l.KV = p.KV, l.d_shift = d_shift;
+  for (int i = first; i < (first ? first + l.n : n); i++) {  // the first call looks at all of them
+    const lbd_kv8_pool &q = pools[i];
+    if (q.pages != p.pages || q.page != p.page || q.KV != p.KV || q.D != p.D)
+      return fail(LB_ERR_SHAPE, "the layers' pools must have the same pages, page, KV and D");
+    if (!q.k || !q.v || !q.ke || !q.ve) return fail(LB_ERR_ARG, "null pointer");
+    if (!aligned16(q.k) || !aligned16(q.v)) return fail(LB_ERR_ARG, "the pool's codes must be 16-byte aligned");
+    if (i < first + l.n) l.of[i - first] = {q.k, q.v, q.ke, q.ve};
+  }
+  return 0;
+}
+
+int beam_args(const lbd_beams *b, lbk::BeamArgs &a) {
+  if (!b) return fail(LB_ERR_ARG, "null pointer");
+  if (b->B <= 0 || b->W <= 0 || b->W > lbk::kMaxBeams || (long long)b->B * b->W > lbk::kMaxPlaces || b->V <= 0 ||
+      b->V > 1 << 24)
+    return fail(LB_ERR_SHAPE, "bad shape: 1..32 beams, at most 2^20 places and 2^24 tokens");
+  if (b->eos < -1 || b->eos >= b->V) return fail(LB_ERR_ARG, "eos is a token or -1");
+  a = {nullptr, 0, b->score, b->done, b->new_score, b->new_done, b->tok, b->parent, b->hist_tok, b->hist_parent,
+       b->step, b->hist_len, b->B, b->W, b->V, b->eos};
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1575,20 +1633,87 @@ size_t lbd_kv8_attention_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batc
 int lbd_kv8_attention(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q, int q_stride, int H,
                       float *out, int out_stride, void *work, size_t work_bytes, void *stream) {
   lbk::Kv8Args a;
+  const int rc = kv8_args(pool, batch, H, a);
+  return rc < 0 ? rc : kv8_attend(a, pool->D, q, q_stride, H, out, out_stride, work, work_bytes, stream);
+}
+
+size_t lbd_kv8_attention_window_work_bytes(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, int H, int window,
+                                           int sinks) {
+  lbk::Kv8Args a;
+  if (kv8_args(pool, batch, H, a) < 0 || kv8_window(a, window, sinks) < 0) return 0;
+  return lbk::kv8_attention_work_bytes(a, pool->D, H);
+}
+
+int lbd_kv8_attention_window(const lbd_kv8_pool *pool, const lbd_kv8_batch *batch, const float *q, int q_stride, int H,
+                             int window, int sinks, float *out, int out_stride, void *work, size_t work_bytes,
+                             void *stream) {
+  lbk::Kv8Args a;
   int rc = kv8_args(pool, batch, H, a);
+  if (rc < 0 || (rc = kv8_window(a, window, sinks)) < 0) return rc;
+  return kv8_attend(a, pool->D, q, q_stride, H, out, out_stride, work, work_bytes, stream);
+}
+
+int lbd_kv8_copy_pages(const lbd_kv8_pool *pools, int n_pools, const int32_t *src, const int32_t *dst, int n,
+                       void *stream) {
+  lbk::Kv8Layers l;
+  int rc = kv8_layers(pools, n_pools, 0, l);
   if (rc < 0) return rc;
-  if (q_stride % 4 || out_stride % 4 || q_stride < (long long)H * pool->D || out_stride < (long long)H * pool->D)
-    return fail(LB_ERR_SHAPE, "bad shape: strides are multiples of 4 floats that hold a row");
-  if (!q || !out) return fail(LB_ERR_ARG, "null pointer");
-  if ((rc = kv8_pointers(a)) < 0) return rc;
-  if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ARG, "q and out must be 16-byte aligned");
-  const size_t need = lbk::kv8_attention_work_bytes(a, pool->D, H);
-  if (!need) return fail(LB_ERR_SHAPE, "too many rows of heads for a launch");
-  if (!work || work_bytes < need) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
+  if (n < 0 || n > 1 << 24) return fail(LB_ERR_SHAPE, "bad shape: at most 2^24 pages");
+  if (n && (!src || !dst)) return fail(LB_ERR_ARG, "null pointer");
+  for (int first = 0; n && first < n_pools; first += l.n) {
+    if (first && (rc = kv8_layers(pools, n_pools, first, l)) < 0) return rc;
+    const hipError_t e = lbk::launch_kv8_copy_pages(l, src, dst, n, static_cast<hipStream_t>(stream));
+    if (e == hipErrorInvalidValue) return fail(LB_ERR_SHAPE, "too many pages for a launch");
+    if (e != hipSuccess) return fail_hip(e, "kv8 page copy launch");
+  }
+  return ok(0);
+}
+
+size_t lbd_beam_select_work_bytes(const lbd_beams *beams) {
+  lbk::BeamArgs a;
+  return beam_args(beams, a) < 0 ? 0 : lbk::beam_select_work_bytes(a.B, a.W, a.V);
+}
+
+int lbd_beam_select(const float *logits, int ld, const lbd_beams *beams, void *work, size_t work_bytes, void *stream) {
+  lbk::BeamArgs a;
+  const int rc = beam_args(beams, a);
+  if (rc < 0) return rc;
+  if (ld < a.V) return fail(LB_ERR_SHAPE, "bad shape: rows of ld >= V floats");
+  if (!logits || !a.score || !a.new_score || !a.new_done || !a.tok || !a.parent)
+    return fail(LB_ERR_ARG, "null pointer");
+  const bool hist = a.hist_tok || a.hist_parent || a.step;
+  if (hist && (!a.hist_tok || !a.hist_parent || !a.step || a.hist_len <= 0))
+    return fail(LB_ERR_ARG, "hist_tok, hist_parent, step and hist_len come together");
+  if (!work || work_bytes < lbk::beam_select_work_bytes(a.B, a.W, a.V))
+    return fail(LB_ERR_ARG, "work smaller than lbd_beam_select_work_bytes");
   if (!aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
-  LB_LAUNCH(lbk::launch_kv8_attention(a, pool->D, q, q_stride, H, out, out_stride, work,
-                                      static_cast<hipStream_t>(stream)),
-            "kv8 attention launch");
+  a.logits = logits;
+  a.ld = ld;
+  LB_LAUNCH(lbk::launch_beam_select(a, work, static_cast<hipStream_t>(stream)), "beam selection launch");
+}
+
+int lbd_kv8_reorder(const lbd_kv8_pool *pools, int n_pools, const lbd_kv8_order *o, void *stream) {
+  lbk::Kv8Layers l;
+  int rc = kv8_layers(pools, n_pools, 0, l);
+  if (rc < 0) return rc;
+  if (!o) return fail(LB_ERR_ARG, "null pointer");
+  if (o->B <= 0 || o->W <= 0 || o->W > lbk::kMaxBeams || (long long)o->B * o->W > lbk::kMaxPlaces ||
+      o->max_pages <= 0 || ((long long)o->max_pages << l.page_shift) > lbk::kKv8MaxPos || o->add < 0 ||
+      o->add > lbk::kKv8MaxPos)
+    return fail(LB_ERR_SHAPE, "bad shape: 1..32 beams, at most 2^20 places and 2^30 positions");
+  if (!o->parent || !o->past || !o->table || !o->own || !o->new_past || !o->new_table)
+    return fail(LB_ERR_ARG, "null pointer");
+  if (o->new_table == o->table || o->new_past == o->past)
+    return fail(LB_ERR_ARG, "new_table and new_past must not be table and past");
+  const lbk::Kv8Order a = {o->parent, o->done, o->past, o->table, o->own, o->new_past, o->new_table, o->B, o->W,
+                           o->max_pages, o->add};
+  for (int first = 0; first < n_pools; first += l.n) {
+    if (first && (rc = kv8_layers(pools, n_pools, first, l)) < 0) return rc;
+    const hipError_t e = lbk::launch_kv8_reorder(l, a, first == 0, static_cast<hipStream_t>(stream));
+    if (e == hipErrorInvalidValue) return fail(LB_ERR_SHAPE, "too many places for a launch");
+    if (e != hipSuccess) return fail_hip(e, "kv8 reorder launch");
+  }
+  return ok(0);
 }
 
 }  // extern "C"

@@ -269,6 +269,7 @@ struct Kv8Args {
   int pages, page_shift, KV;  // page = 1 << page_shift tokens
   const int32_t *q_start, *past, *table;
   int B, max_pages, max_new, T;
+  int window = 0, sinks = 0;  // of a windowed attention; sinks at most max_pages page
 };
 hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stride, const float *bias, int H,
                              const float *cosT, const float *sinT, int max_pos, float *q_out, int q_stride,
@@ -276,5 +277,39 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
 size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H);
 hipError_t launch_kv8_attention(const Kv8Args &a, int D, const float *q, int q_stride, int H, float *out,
                                 int out_stride, void *work, hipStream_t s);
+
+// Pages of the layers' pools (lb_kv8_pages.hip), kKv8Layers a launch.
+constexpr int kKv8Layers = 64;
+struct Kv8Codes {
+  uint8_t *k, *v, *ke, *ve;
+};
+struct Kv8Layers {
+  Kv8Codes of[kKv8Layers];
+  int n;                       // layers in this launch
+  int pages, page_shift, KV, d_shift;  // page = 1 << page_shift tokens, heads of 1 << d_shift
+};
+constexpr int kMaxBeams = 32;
+constexpr int kMaxPlaces = 1 << 20;
+struct Kv8Order {
+  const int32_t *parent, *done, *past, *table, *own;
+  int32_t *new_past, *new_table;
+  int B, W, max_pages, add;
+};
+hipError_t launch_kv8_copy_pages(const Kv8Layers &l, const int32_t *src, const int32_t *dst, int n, hipStream_t s);
+// write: this launch writes new_past and new_table too
+hipError_t launch_kv8_reorder(const Kv8Layers &l, const Kv8Order &o, bool write, hipStream_t s);
+
+// Beam search's selection (lb_beam.hip): lbd_beams as the kernels take it.
+struct BeamArgs {
+  const float *logits;
+  size_t ld;
+  const float *score;
+  const int32_t *done;
+  float *new_score;
+  int32_t *new_done, *tok, *parent, *hist_tok, *hist_parent, *step;
+  int hist_len, B, W, V, eos;
+};
+size_t beam_select_work_bytes(int B, int W, int V);
+hipError_t launch_beam_select(const BeamArgs &a, void *work, hipStream_t s);
 
 }  // namespace lbk

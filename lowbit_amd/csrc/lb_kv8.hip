@@ -305,6 +305,7 @@ struct Kv8Cut {
   unsigned g_inv;  // ceil(2^32 / G)
   int few_blocks, slots_few, slots;  // slices a KV head: with at most few_blocks row blocks, and with more
   float units, fits;  // many rows: compute units a KV head, and workgroups that they hold; else 0
+  int span;           // keys that a row block reads at most
 };
 
 // One class of a call's sequences, by their rows, and where its slices' sums lie in the workspace:
@@ -338,8 +339,11 @@ __device__ __forceinline__ int kv8_row_blocks(const Kv8Cut &c, const Kv8Seq &s) 
   const int rows = s.n * c.G;  // T H <= 2^30
   return rows >= c.rows_min && rows <= c.rows_max ? (rows + (1 << c.r_shift) - 1) >> c.r_shift : 0;
 }
-__device__ __forceinline__ int kv8_keys(const Kv8Args &a, const Kv8Seq &s) {
-  return min(s.past + s.n, a.max_pages << a.page_shift);
+// The most keys that a row block of the sequence reads.
+template <bool WIN>
+__device__ __forceinline__ int kv8_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &s) {
+  const int all = min(s.past + s.n, a.max_pages << a.page_shift);
+  return WIN ? min(all, c.span) : all;
 }
 
 // Rows of a row block, by the column blocks of 16 a wave takes (0: 8 rows, both terms in one).
@@ -365,14 +369,15 @@ __host__ __device__ constexpr int kv8_rows(int nc) { return nc ? 16 * nc : 8; }
 //
 // Slices are never more than slots and row blocks together: the few's sum in float 1 % up, the
 // many's product 2 %.
+template <bool WIN>
 __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first) {
   const int lane = threadIdx.x & (kWave - 1);
-  float blocks = (float)kv8_row_blocks(c, first), sum = blocks * (float)kv8_keys(a, first);
+  float blocks = (float)kv8_row_blocks(c, first), sum = blocks * (float)kv8_keys<WIN>(a, c, first);
   for (int b0 = kWave; b0 < a.B; b0 += kWave) {
     const Kv8Seq s = kv8_seq(a, b0 + lane);
     const float n = (float)kv8_row_blocks(c, s);
     blocks += n;
-    sum += n * (float)kv8_keys(a, s);
+    sum += n * (float)kv8_keys<WIN>(a, c, s);
   }
   blocks = fmaxf(wave_sum(blocks), 1.0f), sum = wave_sum(sum);
   if (c.units > 0.0f) {
@@ -415,10 +420,10 @@ struct Kv8Unit {
   Kv8Seq s;
   int rb, slice, slices, slice_keys, before, at;
 };
-template <bool BLOCK>
+template <bool BLOCK, bool WIN>
 __device__ __forceinline__ bool kv8_unit(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first, int u, Kv8Unit &w) {
   const auto blocks = [&](const Kv8Seq &s) { return kv8_row_blocks(c, s); };
-  const auto slices = [&](const Kv8Seq &s) { return kv8_slices(kv8_keys(a, s), w.slice_keys); };
+  const auto slices = [&](const Kv8Seq &s) { return kv8_slices(kv8_keys<WIN>(a, c, s), w.slice_keys); };
   const auto units = [&](const Kv8Seq &s) { return blocks(s) * slices(s); };
   if constexpr (BLOCK) {
     if (!kv8_locate(a, first, u, blocks, w.s, w.at, units, &w.before)) return false;
@@ -551,7 +556,7 @@ struct Kv8Lds {
   float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
 };
 
-template <int D, int NC>
+template <int D, int NC, bool WIN>
 __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, int kv, int unit,
                                            const float *__restrict__ q, int q_stride, float *__restrict__ out,
                                            int out_stride, float *__restrict__ work, Kv8Lds<D, NC> &lds) {
@@ -566,24 +571,32 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const int c = lane & 15, g = lane >> 4;
   const Kv8Seq first = kv8_seq(a, lane);
   Kv8Unit w;
-  w.slice_keys = kv8_slice_keys(a, cut, first);
-  if (!kv8_unit<false>(a, cut, first, unit, w)) return;
+  w.slice_keys = kv8_slice_keys<WIN>(a, cut, first);
+  if (!kv8_unit<false, WIN>(a, cut, first, unit, w)) return;
   const int place = unit - w.at + w.rb * w.slices + w.slice;  // in the workspace
   if (place >= pt.units) return;  // (rows of several sequences at once, which is not allowed)
   const int G = cut.G, rows = w.s.n * G, cap = a.max_pages << a.page_shift, page = 1 << a.page_shift;
-  // this lane's query rows, the keys they see, and those that the block's last row sees
-  int lim[NB];
+  // this lane's query rows, the keys they see (a window: from low on), and those that the block's
+  // last row sees
+  int lim[NB], low[NB];
   const float *qr[NB];
 #pragma unroll
   for (int y = 0; y < NB; y++) {
     const int r = w.rb * R + (SEP ? 16 * y + c : c & 7), rc = min(r, rows - 1), tok = kv8_token(cut, rc);
     lim[y] = r < rows ? min(w.s.past + tok + 1, cap) : 0;
+    if constexpr (WIN) low[y] = w.s.past + tok + 1 - a.window;
     qr[y] = q + (size_t)(w.s.row0 + tok) * q_stride + (kv * G + rc - tok * G) * D;
   }
   const int tok_last = kv8_token(cut, min(w.rb * R + R, rows) - 1), tok_first = kv8_token(cut, w.rb * R);
+  // A window: keys are counted without the `gap` positions between the tiles of the sinks, `sinks` of
+  // them, and the tile that the first row's window begins in.
+  const int sinks = WIN ? (a.sinks + 15) & ~15 : 0;
+  const int gap = WIN ? max((min(max(w.s.past + tok_first + 1 - a.window, 0), cap) & ~15) - sinks, 0) : 0;
   const int k_begin = w.slice * w.slice_keys;
-  const int k_end = min(min(w.s.past + tok_last + 1, cap), k_begin + w.slice_keys);
-  const int k_full = min(w.s.past + tok_first + 1, cap);  // keys below: every row sees them
+  const int k_end = min(min(w.s.past + tok_last + 1, cap) - gap, k_begin + w.slice_keys);
+  const int k_full = min(w.s.past + tok_first + 1, cap) - gap;  // keys below: every row sees them
+  // (a window: those below the sinks and from here on)
+  const int k_low = WIN && w.s.past + tok_last + 1 - a.window > a.sinks ? w.s.past + tok_last + 1 - a.window - gap : 0;
   const int chunks = max(0, (k_end - k_begin - CK * wave + CK * NW - 1) / (CK * NW));
   const int32_t *table = a.table + (size_t)w.s.b * a.max_pages;
 
@@ -595,8 +608,10 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   uint64_t t_held = 0, t_unused = 0, t_nan = 0;  // a bit a tile
   const auto tile_key = [&](int i) { return k_begin + CK * (wave + NW * (i >> 1)) + 16 * (i & 1); };
   const auto load_tiles = [&](int i0) {
-    const int key = tile_key(i0 + lane);
-    const int pg = key < k_end ? table[key >> a.page_shift] : -1;
+    int key = tile_key(i0 + lane);
+    const bool mine = key < k_end;
+    if constexpr (WIN) key += key < sinks ? 0 : gap;
+    const int pg = mine ? table[key >> a.page_shift] : -1;
     const bool in = (unsigned)pg < (unsigned)a.pages;
     const size_t block = (size_t)(in ? pg : 0) * a.KV + kv;
     t_at = ((block << a.page_shift) + (key & (page - 1))) * D;
@@ -802,7 +817,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         for (int e = 0; e < 4; e++) s[0][x][e] += dpp_f<0x128>(s[0][x][e], 0.0f);  // row_ror:8
     }
     // ---- what some row does not see: scores -inf, and V's codes, which may be anything, 0
-    const bool edge = key0 + CK > k_full || now[0].unused || now[1].unused;
+    bool edge = key0 + CK > k_full || now[0].unused || now[1].unused;
+    if constexpr (WIN) edge = edge || (key0 < k_low && key0 + CK > a.sinks);
     bool careful = false;  // a score of -inf may meet a factor of NaN or 0
     if (edge) {
       bool zero = false;
@@ -815,7 +831,14 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         for (int e = 0; e < 4; e++) {
           const int key = key0 + 16 * x + 4 * g + e;
 #pragma unroll
-          for (int y = 0; y < NB; y++) s[y][x][e] = key < lim[y] && now[x].held ? s[y][x][e] : -INFINITY;
+          for (int y = 0; y < NB; y++) {
+            bool seen = key < lim[y];
+            if constexpr (WIN) {
+              const int at = key + (key0 + 16 * x < sinks ? 0 : gap);
+              seen = at < lim[y] && (at >= low[y] || at < a.sinks);
+            }
+            s[y][x][e] = seen && now[x].held ? s[y][x][e] : -INFINITY;
+          }
           if (key >= k_end || now[x].unused) vf[x][e] = make_uint2(0, 0);
         }
     }
@@ -1025,7 +1048,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
 // (24 sequences of prompts and steps, 14 heads on 2: 36.6 us; two launches and two merges one after
 // the other took 27 % longer, 8 of up to 1100, 32 heads on 8, 25 %, and few rows first 29 %).
-template <int D, int NC, bool MIXED>
+template <int D, int NC, bool MIXED, bool WIN>
 __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
     int out_stride, float *__restrict__ work) {
@@ -1038,11 +1061,11 @@ __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend
   const int unit = (int)(blockIdx.y + blockIdx.z * kKv8GridY);
   if constexpr (MIXED) {
     if (unit >= p0.units) {
-      kv8_attend<D, 1>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
+      kv8_attend<D, 1, WIN>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
       return;
     }
   }
-  kv8_attend<D, NC>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
+  kv8_attend<D, NC, WIN>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
 }
 
 // Partial sums of a row block's slices -> out, two ways: few rows of many slices, many rows of few.
@@ -1051,7 +1074,7 @@ __global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend
 // unit and it), and the D-element sums, 256 / D slices to a wave load, go round the four waves,
 // eight loads requested before the scalars are waited for (64 slices of 8 KV heads' rows: 4.7 us; a
 // wave a row took 3.5 times as long).
-template <int D>
+template <int D, bool WIN>
 __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &pt, int block,
                                                const float *__restrict__ work, float4 (*sh)[D / 4],
                                                float *__restrict__ out, int out_stride) {
@@ -1062,7 +1085,7 @@ __device__ __forceinline__ void kv8_merge_long(const Kv8Args &a, const Kv8Part &
   const int rr = block % cut.R, idx = block / cut.R, kv = idx % a.KV;
   Kv8Unit w;
   w.slice_keys = kv8_cut_of(work, pt);
-  if (!kv8_unit<true>(a, cut, kv8_seq(a, lane), idx / a.KV, w)) return;
+  if (!kv8_unit<true, WIN>(a, cut, kv8_seq(a, lane), idx / a.KV, w)) return;
   const int ns = w.slices, ro = w.rb * cut.R + rr;
   if (ns < 2 || ro >= w.s.n * cut.G || w.before + (w.rb + 1ll) * ns > pt.units) return;
   const size_t pu = (size_t)(w.before + w.rb * ns) * a.KV + kv, step = (size_t)a.KV * cut.R;
@@ -1195,26 +1218,26 @@ __device__ __forceinline__ void kv8_merge_row(const Kv8Args &a, const Kv8Part &p
       make_float4(ldexpf(num.x * f, e), ldexpf(num.y * f, e), ldexpf(num.z * f, e), ldexpf(num.w * f, e));
 }
 
-template <int D>
+template <int D, bool WIN>
 __device__ __forceinline__ void kv8_merge(const Kv8Args &a, const Kv8Part &pt, int block,
                                           const float *__restrict__ work, float4 (*sh)[D / 4],
                                           float *__restrict__ out, int out_stride) {
   constexpr int ROWS = 1024 / D;
   if (!pt.merge) {
-    kv8_merge_long<D>(a, pt, block, work, sh, out, out_stride);
+    kv8_merge_long<D, WIN>(a, pt, block, work, sh, out, out_stride);
     return;
   }
   const int idx = block / pt.merge, kv = idx % a.KV;
   Kv8Unit w;
   w.slice_keys = kv8_cut_of(work, pt);
-  if (!kv8_unit<true>(a, pt.cut, kv8_seq(a, threadIdx.x & (kWave - 1)), idx / a.KV, w) || w.slices < 2) return;
+  if (!kv8_unit<true, WIN>(a, pt.cut, kv8_seq(a, threadIdx.x & (kWave - 1)), idx / a.KV, w) || w.slices < 2) return;
   if (w.before + (w.rb + 1ll) * w.slices > pt.units) return;
   const int rows = min(pt.cut.R, w.s.n * pt.cut.G - w.rb * pt.cut.R);
   for (int rr = block % pt.merge * ROWS + threadIdx.x / (D / 4); rr < rows; rr += pt.merge * ROWS)
     kv8_merge_row<D>(a, pt, w, kv, rr, work, out, out_stride);
 }
 
-template <int D, bool MIXED>
+template <int D, bool MIXED, bool WIN>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Part p0, Kv8Part p1, int blocks0,
                                                         const float *__restrict__ work, float *__restrict__ out,
                                                         int out_stride) {
@@ -1222,11 +1245,11 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8Args a, Kv8Part p0, K
   const int block = blockIdx.x;
   if constexpr (MIXED) {
     if (block >= blocks0) {
-      kv8_merge<D>(a, p1, block - blocks0, work, sh, out, out_stride);
+      kv8_merge<D, WIN>(a, p1, block - blocks0, work, sh, out, out_stride);
       return;
     }
   }
-  kv8_merge<D>(a, p0, block, work, sh, out, out_stride);
+  kv8_merge<D, WIN>(a, p0, block, work, sh, out, out_stride);
 }
 
 // ---------------------------------------------------------------- launchers
@@ -1284,15 +1307,18 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
   const auto add = [&](int nc, int rows_min, int rows_max) {
     Kv8Part &p = plan.p[plan.parts];
     const int R = kv8_rows(nc);
+    // a window: the sinks' tiles, the first row's window from its tile on, and the block's further tokens
+    const long long seen = ((a.sinks + 15) & ~15) + 15ll + a.window + (R - 2 + G) / G;
+    const int span = a.window ? (int)std::min<long long>(cap, seen) : cap;
     long long blocks;
     if (nc < 2) {
       blocks = std::min(a.B, a.T);  // a row block each
-      p.cut = {G, R, nc + 3, rows_min, rows_max, cap <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f, 0.0f};
+      p.cut = {G, R, nc + 3, rows_min, rows_max, span <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f, 0.0f, span};
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
       const int fits = 256 * (D == 128 ? 3 : 4);  // workgroups that the device holds
       p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), 256.0f / (float)a.KV,
-               (float)fits / (float)a.KV};
+               (float)fits / (float)a.KV, span};
     }
     const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
     if (blocks * a.KV >= 1 << 23) return false;  // threads of a launch are counted in 32 bits
@@ -1320,7 +1346,7 @@ size_t kv8_attention_work_bytes(const Kv8Args &a, int D, int H) {
   return kv8_plan(a, D, H, p) ? p.floats * sizeof(float) : 0;
 }
 
-template <int D>
+template <int D, bool WIN>
 static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, int H, float *out, int out_stride,
                                 float *work, hipStream_t s) {
   Kv8Plan plan;
@@ -1331,26 +1357,31 @@ static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, 
   const auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, grid, dim3(kKv8Waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
   };
-  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, false>);
-  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, false>);
-  if (plan.nc == 2) plan.parts == 1 ? go(kv8_attend_kernel<D, 2, false>) : go(kv8_attend_kernel<D, 2, true>);
+  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, false, WIN>);
+  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, false, WIN>);
+  if (plan.nc == 2) plan.parts == 1 ? go(kv8_attend_kernel<D, 2, false, WIN>) : go(kv8_attend_kernel<D, 2, true, WIN>);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || (a.max_pages << a.page_shift) <= p0.cut.min_keys) return e;
+  if (e != hipSuccess || p0.cut.span <= p0.cut.min_keys) return e;
   const auto groups = [&](const Kv8Part &p) { return p.blocks * a.KV * (p.merge ? p.merge : p.cut.R); };
   const auto merge = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3(groups(p0) + groups(p1)), dim3(256), 0, s, a, p0, p1, groups(p0), work, out,
                        out_stride);
   };
-  plan.parts == 1 ? merge(kv8_merge_kernel<D, false>) : merge(kv8_merge_kernel<D, true>);
+  plan.parts == 1 ? merge(kv8_merge_kernel<D, false, WIN>) : merge(kv8_merge_kernel<D, true, WIN>);
   return hipGetLastError();
 }
 
 hipError_t launch_kv8_attention(const Kv8Args &a, int D, const float *q, int q_stride, int H, float *out,
                                 int out_stride, void *work, hipStream_t s) {
   float *w = static_cast<float *>(work);
-  if (D == 32) return kv8_attention<32>(a, q, q_stride, H, out, out_stride, w, s);
-  if (D == 64) return kv8_attention<64>(a, q, q_stride, H, out, out_stride, w, s);
-  if (D == 128) return kv8_attention<128>(a, q, q_stride, H, out, out_stride, w, s);
+  const auto go = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    return a.window ? kv8_attention<DD, true>(a, q, q_stride, H, out, out_stride, w, s)
+                    : kv8_attention<DD, false>(a, q, q_stride, H, out, out_stride, w, s);
+  };
+  if (D == 32) return go(std::integral_constant<int, 32>());
+  if (D == 64) return go(std::integral_constant<int, 64>());
+  if (D == 128) return go(std::integral_constant<int, 128>());
   return hipErrorInvalidValue;
 }
 

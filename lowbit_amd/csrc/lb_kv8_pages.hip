@@ -1,0 +1,141 @@
+// Pages of the paged 8-bit cache moved about: copies within every layer's pool
+// (lbd_kv8_copy_pages), and the sequences of a beam search put in their new order
+// (lbd_kv8_reorder). No reference counterpart: its cache is one float32 array per sequence
+// (src/lowbit/model.py:264-297).
+#include "lb_device.h"
+#include "lb_internal.h"
+
+namespace lbk {
+
+constexpr int kCopyBytes = 1 << 14;  // of a page's K or V codes that a workgroup copies at a time
+
+// ---------------------------------------------------------------- copies of pages
+
+__global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Layers l, const int32_t *__restrict__ src,
+                                                       const int32_t *__restrict__ dst, int parts) {
+  const Kv8Codes c = l.of[blockIdx.y];
+  const int pair = (int)blockIdx.x / (2 * parts), rest = (int)blockIdx.x % (2 * parts);
+  const bool isv = rest >= parts;
+  const int part = isv ? rest - parts : rest, from = src[pair], to = dst[pair];
+  if ((unsigned)from >= (unsigned)l.pages || (unsigned)to >= (unsigned)l.pages || from == to) return;
+  const size_t bytes = (size_t)l.KV << (l.page_shift + l.d_shift);
+  uint8_t *codes = isv ? c.v : c.k, *exps = isv ? c.ve : c.ke;
+  const size_t end = min(bytes, ((size_t)part + 1) * kCopyBytes);
+  for (size_t i = (size_t)part * kCopyBytes + 16 * threadIdx.x; i < end; i += 16 * 256)
+    *reinterpret_cast<uint4 *>(codes + to * bytes + i) = *reinterpret_cast<const uint4 *>(codes + from * bytes + i);
+  if (part == 0)
+    for (int i = threadIdx.x; i < l.KV; i += 256) exps[(size_t)to * l.KV + i] = exps[(size_t)from * l.KV + i];
+}
+
+// ---------------------------------------------------------------- beams in their new order
+
+// What becomes of one place, the same in every lane of a wave.
+struct Kv8Move {
+  int parent, length;  // the place that it continues and the tokens that it holds; parent -1: no sequence
+  int tail, used;      // index of the page that is being written, and its tokens (0: it is begun next)
+  int from, page;      // that page: the parent's and the place's (the parent's own: no copy)
+};
+
+// The move of place `place`, by the whole wave: lane k looks at place k of the prompt.
+__device__ __forceinline__ Kv8Move kv8_move(const Kv8Order &o, int page_shift, int pages, int place) {
+  const int lane = threadIdx.x & (kWave - 1), base = place / o.W * o.W, me = place - base, cap = o.max_pages << page_shift;
+  int parent = -1, length = 0, was = -1;
+  if (lane < o.W) {
+    const int p = o.parent[base + lane];
+    if (p >= base && p < base + o.W && !(o.done && o.done[base + lane])) {
+      const int past = o.past[p];
+      if (past >= 0) parent = p, length = (int)min((long long)past + o.add, (long long)kKv8MaxPos);
+    }
+  }
+  const int tail = min(length, cap) >> page_shift, used = length < cap ? length & ((1 << page_shift) - 1) : 0;
+  const bool copied = parent >= 0 && used;
+  if (copied) was = o.table[(size_t)parent * o.max_pages + tail];
+  // the first place of those that continue a parent keeps its page
+  const unsigned long long holds = __ballot(copied);
+  bool first = copied;
+  for (int k = 0; k < o.W; k++) {
+    const int theirs = __builtin_amdgcn_readlane(parent, k);
+    if ((holds >> k & 1) && k < lane && theirs == parent) first = false;
+  }
+  const unsigned long long keep = __ballot(first);
+  const auto mine = [&](int v) { return __builtin_amdgcn_readlane(v, me); };
+  Kv8Move m = {mine(parent), mine(length), mine(tail), mine(used), mine(was), mine(was)};
+  if (!(holds >> me & 1) || (keep >> me & 1)) return m;
+  // the others take the pages that no first place keeps, in order
+  const int spare = lane < o.W ? o.own[(size_t)(base + lane) * o.max_pages + m.tail] : -1;
+  bool free = (unsigned)spare < (unsigned)pages;
+  for (int k = 0; k < o.W; k++) {
+    const int kept = __builtin_amdgcn_readlane(was, k);
+    if ((keep >> k & 1) && kept == spare) free = false;
+  }
+  unsigned long long left = __ballot(free);
+  for (unsigned long long before = __ballot(copied && !first && tail == m.tail && lane < me); before; before &= before - 1)
+    left &= left - 1;
+  m.page = left ? __builtin_amdgcn_readlane(spare, __ffsll(left) - 1) : -1;
+  return m;
+}
+
+__global__ __launch_bounds__(256) void kv8_reorder_kernel(Kv8Layers l, Kv8Order o, int copies, int parts) {
+  const int tid = threadIdx.x, id = (int)blockIdx.x;
+  if (id >= copies) {  // a place's row of the table
+    if (blockIdx.y) return;
+    const int place = id - copies;
+    const Kv8Move m = kv8_move(o, l.page_shift, l.pages, place);
+    const size_t row = (size_t)place * o.max_pages;
+    for (int j = tid; j < o.max_pages; j += 256) {
+      int p = -1;
+      if (m.parent >= 0) {
+        p = j < m.tail ? o.table[(size_t)m.parent * o.max_pages + j] : o.own[row + j];
+        if (j == m.tail && m.used) p = m.page;
+      }
+      o.new_table[row + j] = p;
+    }
+    if (tid == 0) o.new_past[place] = m.parent >= 0 ? m.length : -1;
+    return;
+  }
+  const int place = id / (2 * parts), rest = id % (2 * parts);
+  const bool isv = rest >= parts;
+  const int part = isv ? rest - parts : rest;
+  const Kv8Move m = kv8_move(o, l.page_shift, l.pages, place);
+  if (m.parent < 0 || !m.used || m.page == m.from) return;
+  if ((unsigned)m.page >= (unsigned)l.pages || (unsigned)m.from >= (unsigned)l.pages) return;
+  const Kv8Codes c = l.of[blockIdx.y];
+  const size_t bytes = (size_t)l.KV << (l.page_shift + l.d_shift);
+  uint8_t *codes = isv ? c.v : c.k, *exps = isv ? c.ve : c.ke;
+  const size_t end = min(bytes, ((size_t)part + 1) * kCopyBytes);
+  for (size_t i = (size_t)part * kCopyBytes + 16 * tid; i < end; i += 16 * 256) {
+    const int slot = (int)(i >> l.d_shift) & ((1 << l.page_shift) - 1);
+    if (slot < m.used)
+      *reinterpret_cast<uint4 *>(codes + m.page * bytes + i) = *reinterpret_cast<const uint4 *>(codes + m.from * bytes + i);
+  }
+  if (part == 0)
+    for (int i = tid; i < l.KV; i += 256) exps[(size_t)m.page * l.KV + i] = exps[(size_t)m.from * l.KV + i];
+}
+
+// ---------------------------------------------------------------- launchers
+
+static int copy_parts(const Kv8Layers &l) {
+  const long long bytes = (long long)l.KV << (l.page_shift + l.d_shift);
+  return (int)((bytes + kCopyBytes - 1) / kCopyBytes);
+}
+
+// Threads of a launch are counted in 32 bits.
+static bool fits(long long blocks, int layers) { return blocks * layers <= 0xFFFFFFFFll / 256; }
+
+hipError_t launch_kv8_copy_pages(const Kv8Layers &l, const int32_t *src, const int32_t *dst, int n, hipStream_t s) {
+  const int parts = copy_parts(l);
+  const long long grid = 2ll * n * parts;
+  if (!fits(grid, l.n)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kv8_copy_kernel, dim3((unsigned)grid, l.n), dim3(256), 0, s, l, src, dst, parts);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv8_reorder(const Kv8Layers &l, const Kv8Order &o, bool write, hipStream_t s) {
+  const int parts = copy_parts(l);
+  const long long places = (long long)o.B * o.W, copies = 2 * places * parts, grid = copies + (write ? places : 0);
+  if (!fits(grid, l.n)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kv8_reorder_kernel, dim3((unsigned)grid, l.n), dim3(256), 0, s, l, o, (int)copies, parts);
+  return hipGetLastError();
+}
+
+}  // namespace lbk

@@ -176,6 +176,12 @@ SIGNATURES = {
     "lbd_kv8_append": ([_vp, _vp, _vp, _int, _vp, _int, _vp, _vp, _int, _vp, _int, _vp], _int),
     "lbd_kv8_attention_work_bytes": ([_vp, _vp, _int], _sz),
     "lbd_kv8_attention": ([_vp, _vp, _vp, _int, _int, _vp, _int, _vp, _sz, _vp], _int),
+    "lbd_kv8_attention_window_work_bytes": ([_vp, _vp, _int, _int, _int], _sz),
+    "lbd_kv8_attention_window": ([_vp, _vp, _vp, _int, _int, _int, _int, _vp, _int, _vp, _sz, _vp], _int),
+    "lbd_kv8_copy_pages": ([_vp, _int, _vp, _vp, _int, _vp], _int),
+    "lbd_beam_select_work_bytes": ([_vp], _sz),
+    "lbd_beam_select": ([_vp, _int, _vp, _vp, _sz, _vp], _int),
+    "lbd_kv8_reorder": ([_vp, _int, _vp, _vp], _int),
     "lbd_quantize_int4_g32": ([_vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
 }
 
@@ -224,6 +230,19 @@ class LbdKv8Batch(C.Structure):
     """lbd_kv8_batch of include/lowbit_hip.h: the sequences of a call on such a cache."""
     _fields_ = [("q_start", C.c_void_p), ("past", C.c_void_p), ("table", C.c_void_p), ("B", C.c_int),
                 ("max_pages", C.c_int), ("max_new", C.c_int), ("T", C.c_int)]
+
+
+class LbdBeams(C.Structure):
+    """lbd_beams of include/lowbit_hip.h: the places of a step of beam search."""
+    _fields_ = [(f, C.c_void_p) for f in ("score", "done", "new_score", "new_done", "tok", "parent", "hist_tok",
+                                          "hist_parent", "step")] + [
+        (f, C.c_int) for f in ("hist_len", "B", "W", "V", "eos")]
+
+
+class LbdKv8Order(C.Structure):
+    """lbd_kv8_order of include/lowbit_hip.h: the beams' sequences and their new order."""
+    _fields_ = [(f, C.c_void_p) for f in ("parent", "done", "past", "table", "own", "new_past", "new_table")] + [
+        (f, C.c_int) for f in ("B", "W", "max_pages", "add")]
 
 
 @lru_cache(maxsize=1)

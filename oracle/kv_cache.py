@@ -105,10 +105,10 @@ class Pool:
         s = np.where(exps == 255, np.nan, 2.0 ** (exps.astype(np.float64) - 127))
         return E4M3[codes] * s[..., None, None]
 
-    def attention(self, q_start, past, table, max_new, q, heads, out):
-        """lbd_kv8_attention of rows q [T, >= heads d] in float64; `out` edited. Also returns, per
-        element of out, the scale of its rounding errors: (largest sum |q k| / sqrt(d), weighted
-        mean of |v|, keys)."""
+    def attention(self, q_start, past, table, max_new, q, heads, out, window=None, sinks=0):
+        """lbd_kv8_attention (lbd_kv8_attention_window with a window) of rows q [T, >= heads d] in
+        float64; `out` edited. Also returns, per element of out, the scale of its rounding errors:
+        (largest sum |q k| / sqrt(d), weighted mean of |v|, keys)."""
         kv, d, page = self.kv, self.d, self.page
         cap, g = table.shape[1] * page, heads // kv
         mags = np.zeros((len(q), heads, 3))
@@ -123,7 +123,10 @@ class Pool:
             k, v = (np.moveaxis(self.values(c[safe], e[safe]), 1, 0).reshape(kv, -1, d)[:, :last]
                     for c, e in ((self.k, self.ke), (self.v, self.ve)))
             rows = slice(int(q_start[b]), int(q_start[b]) + n)
-            see = held & (np.arange(last) <= past[b] + np.arange(n)[:, None])
+            key, at = np.arange(last), past[b] + np.arange(n)[:, None]
+            see = held & (key <= at)
+            if window is not None:
+                see &= (at - key < window) | (key < sinks)
             some = see.any(1)
             for h in range(heads):
                 x = q[rows, h * d:(h + 1) * d].astype(np.float64)
