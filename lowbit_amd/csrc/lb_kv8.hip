@@ -371,6 +371,7 @@ __host__ __device__ constexpr int kv8_rows(int nc) { return nc ? 16 * nc : 8; }
 // many's product 2 %.
 template <bool WIN>
 __device__ __forceinline__ int kv8_slice_keys(const Kv8Args &a, const Kv8Cut &c, const Kv8Seq &first) {
+  if (WIN && c.span <= c.min_keys) return c.min_keys;
   const int lane = threadIdx.x & (kWave - 1);
   float blocks = (float)kv8_row_blocks(c, first), sum = blocks * (float)kv8_keys<WIN>(a, c, first);
   for (int b0 = kWave; b0 < a.B; b0 += kWave) {
@@ -545,22 +546,21 @@ struct Kv8Tile {
 // beside this one's weights (0 to 40 %, it spills), matrix and vector instructions alternated by
 // scheduling barriers, both column blocks' weights in one stretch (3 %), two waves a workgroup (1
 // to 15 %), the place of a workgroup found by one of its waves (1 %).
-template <int D, int NC>
+template <int D, int NC, int NW>
 struct Kv8Lds {
-  static constexpr int NW = kKv8Waves;
   union {
-    float sh[NC == 2 ? NW / 2 : NW][kv8_rows(NC)][D + 4];
+    float sh[NC < 2 ? NW : NW == 4 ? 2 : 1][kv8_rows(NC)][D + 4];
     uint4 q[NC == 2 ? D / 8 : 1][kWave];  // NC 2: the query rows' operands, [column block][product][term]
+    v4f ex[NC == 2 && NW == 2 ? 2 : 1][D / 16][kWave];  // what the waves hand to each other
   };
   float cx[2][16];
   float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
 };
 
-template <int D, int NC, bool WIN>
+template <int D, int NC, bool WIN, int NW>
 __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, int kv, int unit,
                                            const float *__restrict__ q, int q_stride, float *__restrict__ out,
-                                           int out_stride, float *__restrict__ work, Kv8Lds<D, NC> &lds) {
-  constexpr int NW = kKv8Waves;
+                                           int out_stride, float *__restrict__ work, Kv8Lds<D, NC, NW> &lds) {
   constexpr bool SEP = NC > 0;
   constexpr int NB = SEP ? NC : 1, R = kv8_rows(NC), KS = D / 32, CK = 32;
   constexpr int KB = D >= 64 ? 16 : 8, KL = D / (4 * KB);  // bytes of a K load, loads per lane and tile
@@ -620,10 +620,10 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     t_ve = in ? t_ve : -1;
   };
   constexpr bool BIG = NC == 2;  // the query rows laid out by the waves together, in LDS
-  constexpr int QB = BIG ? 1 : NB;
+  constexpr int QB = BIG && NW > 1 ? 1 : NB;
   v8h qh[QB][KS], ql[QB][SEP ? KS : 1];
   float4 qf[QB][KS][2];
-  if constexpr (BIG) qr[0] = wave & 1 ? qr[1] : qr[0];
+  if constexpr (BIG && NW > 1) qr[0] = wave & 1 ? qr[1] : qr[0];
 #pragma unroll
   for (int y = 0; y < QB; y++)
 #pragma unroll
@@ -718,7 +718,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     cx[y] = down * (kKv8Log2e / sqrtf((float)D));
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      if (BIG && s * NW / 2 / KS != wave / 2) continue;  // another wave's
+      if (BIG && NW > 1 && s * NW / 2 / KS != wave / 2) continue;  // another wave's
       const float4 a0 = qf[y][s][0], a1 = qf[y][s][1];
       const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
 #pragma unroll
@@ -735,15 +735,16 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         }
       }
       if constexpr (BIG) {
-        lds.q[((wave & 1) * KS + s) * 2][lane] = __builtin_bit_cast(uint4, qh[0][s]);
-        lds.q[((wave & 1) * KS + s) * 2 + 1][lane] = __builtin_bit_cast(uint4, ql[0][s]);
+        const int at = ((NW > 1 ? wave & 1 : y) * KS + s) * 2;
+        lds.q[at][lane] = __builtin_bit_cast(uint4, qh[y][s]);
+        lds.q[at + 1][lane] = __builtin_bit_cast(uint4, ql[y][s]);
       }
     }
   }
   if constexpr (BIG) {
-    if (g == 0 && wave < 2) lds.cx[wave][c] = cx[0];
+    if (NW > 1 && g == 0 && wave < 2) lds.cx[wave][c] = cx[0];
     __syncthreads();
-    cx[0] = lds.cx[0][c], cx[NB - 1] = lds.cx[1][c];
+    if constexpr (NW > 1) cx[0] = lds.cx[0][c], cx[NB - 1] = lds.cx[1][c];
   }
 
   float m[NB], l[NB];
@@ -832,12 +833,14 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
           const int key = key0 + 16 * x + 4 * g + e;
 #pragma unroll
           for (int y = 0; y < NB; y++) {
-            bool seen = key < lim[y];
             if constexpr (WIN) {
               const int at = key + (key0 + 16 * x < sinks ? 0 : gap);
-              seen = at < lim[y] && (at >= low[y] || at < a.sinks);
+              // (bit by bit: && and || become branches, two an element)
+              const bool seen = (at < lim[y]) & ((at >= low[y]) | (at < a.sinks)) & now[x].held;
+              s[y][x][e] = seen ? s[y][x][e] : -INFINITY;
+            } else {
+              s[y][x][e] = key < lim[y] && now[x].held ? s[y][x][e] : -INFINITY;
             }
-            s[y][x][e] = seen && now[x].held ? s[y][x][e] : -INFINITY;
           }
           if (key >= k_end || now[x].unused) vf[x][e] = make_uint2(0, 0);
         }
@@ -992,7 +995,37 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     lds.sl[0][rr] = (M - u.m) + u.mid;
   }
   __syncthreads();
-  if constexpr (BIG) {
+  if constexpr (BIG && NW < 4) {
+    // each of two waves adds up one column block's rows; into LDS a row's elements lie side by side
+#pragma unroll
+    for (int y = 0; y < NB; y++) {
+      const float f = lds.sm[wave][16 * y + c];
+#pragma unroll
+      for (int j = 0; j < VB; j++) acc[y][j] *= f;
+    }
+    if constexpr (NW == 2) {
+#pragma unroll
+      for (int j = 0; j < VB; j++) lds.ex[wave][j][lane] = wave ? acc[0][j] : acc[1][j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < VB; j++) acc[0][j] = (wave ? acc[1][j] : acc[0][j]) + lds.ex[1 - wave][j][lane];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int y = 0; y < (NW == 1 ? NB : 1); y++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float *row = &lds.sh[0][16 * (NW == 1 ? y : wave) + c][4 * VB * g + VB * e];
+        if constexpr (VB >= 4) {
+#pragma unroll
+          for (int j = 0; j < VB; j += 4)
+            *reinterpret_cast<float4 *>(row + j) = make_float4(acc[y][j][e], acc[y][j + 1][e], acc[y][j + 2][e], acc[y][j + 3][e]);
+        } else {
+          *reinterpret_cast<float2 *>(row) = make_float2(acc[y][0][e], acc[y][1][e]);
+        }
+      }
+    __syncthreads();
+  } else if constexpr (BIG) {
     float fy[NB];
 #pragma unroll
     for (int y = 0; y < NB; y++) fy[y] = lds.sm[wave][16 * y + c];
@@ -1048,24 +1081,24 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
 // (NC = 1), so that the cache streaming of the ones runs beside the matrix products of the others
 // (24 sequences of prompts and steps, 14 heads on 2: 36.6 us; two launches and two merges one after
 // the other took 27 % longer, 8 of up to 1100, 32 heads on 8, 25 %, and few rows first 29 %).
-template <int D, int NC, bool MIXED, bool WIN>
-__global__ __launch_bounds__(kKv8Waves *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
+template <int D, int NC, bool MIXED, bool WIN, int NW>
+__global__ __launch_bounds__(NW *kWave, D == 128 ? 3 : 4) void kv8_attend_kernel(
     Kv8Args a, Kv8Part p0, Kv8Part p1, const float *__restrict__ q, int q_stride, float *__restrict__ out,
     int out_stride, float *__restrict__ work) {
   union Lds {
-    Kv8Lds<D, NC> one;
-    Kv8Lds<D, 1> few;
+    Kv8Lds<D, NC, NW> one;
+    Kv8Lds<D, 1, NW> few;
   };
   __shared__ Lds lds;
   const int kv = blockIdx.x;
   const int unit = (int)(blockIdx.y + blockIdx.z * kKv8GridY);
   if constexpr (MIXED) {
     if (unit >= p0.units) {
-      kv8_attend<D, 1, WIN>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
+      kv8_attend<D, 1, WIN, NW>(a, p1, kv, unit - p0.units, q, q_stride, out, out_stride, work, lds.few);
       return;
     }
   }
-  kv8_attend<D, NC, WIN>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
+  kv8_attend<D, NC, WIN, NW>(a, p0, kv, unit, q, q_stride, out, out_stride, work, lds.one);
 }
 
 // Partial sums of a row block's slices -> out, two ways: few rows of many slices, many rows of few.
@@ -1289,6 +1322,7 @@ hipError_t launch_kv8_append(const Kv8Args &a, int D, const float *qkv, int stri
 
 // Sequences of more rows a KV head than this take row blocks of 32.
 constexpr int kKv8FewRows = 16;
+constexpr int kKv8Whole = 2304;  // a window of at most so many keys may be taken whole by its row blocks
 
 struct Kv8Plan {
   Kv8Part p[2];  // the call's classes: with both, many rows first
@@ -1313,12 +1347,23 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     long long blocks;
     if (nc < 2) {
       blocks = std::min(a.B, a.T);  // a row block each
-      p.cut = {G, R, nc + 3, rows_min, rows_max, span <= 1024 ? 1024 : 256, g_inv, each(256), each(512), each(many ? 512 : 2048), 0.0f, 0.0f, span};
+      // A window's few keys may be taken whole: no slots for slices, no second launch. One step of 32 heads
+      // on 8 of 128 in a window of 512: 10.6 -> 9.3 us, of 1000: 10.6, whole 11.0; 16 and 64 of them of 1500:
+      // 16.2 -> 14.8 and 35.6 -> 29.6.
+      const bool whole = a.window && (span <= 768 || (span <= 1664 && blocks * a.KV >= 128));
+      p.cut = {G, R, nc + 3, rows_min, rows_max, whole ? kKv8Whole : !a.window && cap <= 1024 ? 1024 : 256, g_inv,
+               each(256), each(512), whole ? 0 : each(many ? 512 : 2048), 0.0f, 0.0f, span};
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
       const int fits = 256 * (D == 128 ? 3 : 4);  // workgroups that the device holds
-      p.cut = {G, R, nc + 3, rows_min, rows_max, 256, g_inv, 0, 0, each(2 * fits), 256.0f / (float)a.KV,
-               (float)fits / (float)a.KV, span};
+      // A window of few keys: row blocks enough for half of the compute units are taken whole, so that
+      // nobody decides on slices and no second launch looks for them (2048 tokens, 32 heads on 8 of 128,
+      // windows of 512 and 1024: 64.3 -> 57.9 us and 85.5 -> 78.7; 200 tokens of them, 208 row blocks, 26.1
+      // -> 22.1; 200 of 14 heads on 2 of 64, 88 row blocks: 15.8, whole 16.1, and 40 of the 32 heads, 48:
+      // 16.7 and 20.8).
+      const bool whole = a.window && span <= kKv8Whole && blocks * a.KV >= 128;
+      p.cut = {G, R, nc + 3, rows_min, rows_max, whole ? kKv8Whole : 256, g_inv, 0, 0, whole ? 0 : each(2 * fits),
+               256.0f / (float)a.KV, (float)fits / (float)a.KV, span};
     }
     const long long units = blocks + p.cut.slots, rows = blocks * a.KV * R;
     if (blocks * a.KV >= 1 << 23) return false;  // threads of a launch are counted in 32 bits
@@ -1354,14 +1399,28 @@ static hipError_t kv8_attention(const Kv8Args &a, const float *q, int q_stride, 
   const Kv8Part &p0 = plan.p[0], &p1 = plan.p[1];
   const int units = p0.units + p1.units;
   const dim3 grid(a.KV, std::min(units, kKv8GridY), (units + kKv8GridY - 1) / kKv8GridY);
-  const auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(kKv8Waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
+  const auto go = [&](auto kern, int waves) {
+    hipLaunchKernelGGL(kern, grid, dim3(waves * kWave), 0, s, a, p0, p1, q, q_stride, out, out_stride, work);
   };
-  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, false, WIN>);
-  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, false, WIN>);
-  if (plan.nc == 2) plan.parts == 1 ? go(kv8_attend_kernel<D, 2, false, WIN>) : go(kv8_attend_kernel<D, 2, true, WIN>);
+  constexpr int W4 = kKv8Waves;
+  if (plan.nc == 0) go(kv8_attend_kernel<D, 0, false, WIN, W4>, W4);
+  if (plan.nc == 1) go(kv8_attend_kernel<D, 1, false, WIN, W4>, W4);
+  if (plan.nc == 2) {
+    const bool one = plan.parts == 1;
+    // Two waves a workgroup, each with more chunks between its beginning and end, where a window is short or
+    // row blocks are many (2048 tokens, 32 heads on 8 of 128, a window of 256: 47.3 -> 43.1 us, 8192 tokens of
+    // 512: 226.9 -> 203.3; of 2048 tokens and 14 heads on 2 of 64, 898 row blocks, 256: 17.0 -> 16.1, 512:
+    // 20.1, two waves 21.5; 658 row blocks, 256: 15.0, two waves 15.5).
+    const long long groups = (long long)p0.blocks * a.KV;
+    const bool two = WIN && p0.cut.min_keys == kKv8Whole && groups >= 768 && (p0.cut.span <= 384 || (one && groups >= 3000));
+    if constexpr (WIN) {
+      if (two) one ? go(kv8_attend_kernel<D, 2, false, WIN, 2>, 2) : go(kv8_attend_kernel<D, 2, true, WIN, 2>, 2);
+    }
+    if (!two) one ? go(kv8_attend_kernel<D, 2, false, WIN, W4>, W4) : go(kv8_attend_kernel<D, 2, true, WIN, W4>, W4);
+  }
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p0.cut.span <= p0.cut.min_keys) return e;
+  const bool cut = p0.cut.span > p0.cut.min_keys || (plan.parts == 2 && p1.cut.span > p1.cut.min_keys);
+  if (e != hipSuccess || !cut) return e;
   const auto groups = [&](const Kv8Part &p) { return p.blocks * a.KV * (p.merge ? p.merge : p.cut.R); };
   const auto merge = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3(groups(p0) + groups(p1)), dim3(256), 0, s, a, p0, p1, groups(p0), work, out,

@@ -93,21 +93,35 @@ def test_slices(rng, D, KV, H, seqs, window):
     run(rng, D, 32, KV, H, seqs, window, 20)
 
 
+@pytest.mark.parametrize("D,KV,H,seqs,window", [
+    # row blocks of prompts taken whole, steps beside them cut into slices, and the other way round
+    (64, 2, 14, [(1200, 300)] * 3 + [(3000, 1), (2500, 2)] * 4, 1800),
+    (128, 1, 4, [(2500, 100), (2400, 1), (5, 1)], 500), (64, 2, 14, [(4000, 30), (3900, 1)], 2600),
+    # two waves a workgroup: short windows of many row blocks, alone and beside steps
+    (64, 8, 32, [(0, 1100)], 100), (32, 8, 64, [(10, 800), (700, 1), (0, 90), (300, 3)], 200),
+    (128, 8, 32, [(0, 790), (900, 1)], 33), (32, 64, 256, [(3, 400)], 900)], ids=str)
+def test_ways_of_cutting(rng, D, KV, H, seqs, window):
+    run(rng, D, 64, KV, H, seqs, window, 6)
+
+
 def test_many_sequences(rng):
     seqs = [(int(rng.integers(0, 90)), int(rng.integers(0, 3))) for _ in range(150)]
     run(rng, 64, 16, 1, 4, seqs, 20, 3)
 
 
 def test_a_window_of_everything(rng):
-    """A window as long as the sequences is lbd_kv8_attention, bit for bit."""
+    """A window as long as the sequences is lbd_kv8_attention: each within the tolerance of the other's
+    result in 64 bits (keys may be cut into other slices)."""
     for seqs in ([(700, 1)], [(40, 90)], [(5, 1), (300, 40), (0, 3)]):
         pages, q_start, past, table, T = batch_of(rng, 32, seqs, 1, 1)
         pool = cached(rng, pages, 32, 2, 64, table, seqs)
         q = rng.standard_normal((T, 8 * 64)).astype(np.float32)
-        dev = Device(pool, q_start, past, table, max(n for _, n in seqs), T)
-        want = dev.attention(q, 8, 8 * 64)
+        most = max(n for _, n in seqs)
+        dev, ref = Device(pool, q_start, past, table, most, T), np.full(q.shape, FILL, np.float64)
+        mags = pool.attention(q_start, past, table, most, q, 8, ref)
+        check(dev.attention(q, 8, 8 * 64), ref, mags, 64, 8)
         for window, sinks in ((2000, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 5000)):
-            assert np.array_equal(attend(dev, q, 8, 8 * 64, window, sinks), want)
+            check(attend(dev, q, 8, 8 * 64, window, sinks), ref, mags, 64, 8)
 
 
 def test_positions_past_the_table(rng):
