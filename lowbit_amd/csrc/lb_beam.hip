@@ -20,7 +20,7 @@ constexpr int kBeamWaves = 4;                            // of a workgroup
 constexpr int kBeamLoads = 4;                            // 16-byte loads a lane has in flight
 constexpr int kBeamChunk = 4 * kWave * kBeamLoads;       // logits a wave looks at a time
 constexpr int kBeamStep = kBeamChunk * kBeamWaves;       // a workgroup
-constexpr int kBeamRoom = 192;                           // keys that a wave keeps before it sorts them out
+constexpr int kBeamRoom = 384;                           // keys that a wave has room for: 128, and 4 of every lane
 constexpr int kBeamGridY = 1 << 15;                      // rows in the grid's second dimension
 constexpr int kBeamHeads = 256;                          // pieces of a prompt's rows at most
 constexpr float kBeamNone = -3.4028234663852886e38f;     // the maximum before any logit: finite
@@ -29,12 +29,6 @@ constexpr float kBeamNone = -3.4028234663852886e38f;     // the maximum before a
 struct BeamPiece {
   float max, sum;  // sum exp(x - max), NaN where the row offers nothing
 };
-
-// A row that offers tokens: its beam has not ended and there is one.
-__device__ __forceinline__ bool beam_open(const BeamArgs &a, int row) {
-  const float s = a.score[row];
-  return !(a.done && a.done[row]) && s > -INFINITY;
-}
 
 __device__ __forceinline__ float offer_logit(unsigned long long key) {
   const uint32_t k = (uint32_t)(key >> 32);
@@ -51,11 +45,27 @@ __device__ __forceinline__ unsigned long long order_f64(double x) {
 // than 2^-20 the term is below e^-16 of the sum's largest.
 __device__ __forceinline__ float exp_below(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 
+// How many of n numbers (n a multiple of 4, all different but for zeros behind the last) are larger than one,
+// by their high words `top`; where others have the same one, `before` compares what is left. (64-bit
+// comparisons throughout took three times as long.)
+template <class F>
+__device__ __forceinline__ int beam_place(const uint32_t *top, int n, uint32_t one, F before) {
+  int place = 0, same = 0;
+  for (int j = 0; j < n; j += 4) {
+    const uint4 t = *reinterpret_cast<const uint4 *>(top + j);
+    place += (t.x > one) + (t.y > one) + (t.z > one) + (t.w > one);
+    same += (t.x == one) + (t.y == one) + (t.z == one) + (t.w == one);
+  }
+  if (same > 1)
+    for (int j = 0; j < n; j++) place += top[j] == one && before(j);
+  return place;
+}
+
 // ---------------------------------------------------------------- pieces of rows
 
 // The W largest of n keys (n <= kBeamRoom, W <= n, all different), by one wave, to the front in descending
 // order: a key's place is how many are larger. Returns the last of them.
-__device__ __forceinline__ unsigned long long beam_sort(unsigned long long *keys, int n, int W) {
+__device__ __attribute__((noinline)) unsigned long long beam_sort(unsigned long long *keys, int n, int W) {
   constexpr int PER = kBeamRoom / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   unsigned long long mine[PER];
@@ -93,181 +103,244 @@ __device__ __forceinline__ float beam_threshold(float v, int W) {
   return t < 0x00800000u ? kBeamNone : offer_logit((unsigned long long)t << 32);
 }
 
-// A workgroup a piece of `per` steps of a row. Every wave keeps the keys above its own threshold in LDS: the
-// first chunk's comes from its lanes' maxima (the W-th largest of 64: W of them at least reach it, and few
-// more), later ones from sorting the kept keys out, so that nearly all chunks of a row end after a comparison
-// of 16 logits' maximum, and no wave waits for another before the end.
+// A workgroup a piece of `per` steps of a row. Every wave keeps the keys above its threshold in LDS: the first
+// step's, for all waves, is the W-th largest of 64 lanes' maxima (W of them at least reach it, and few more),
+// later ones come from sorting the kept keys out where they run out of room. So most chunks end after a
+// comparison of 16 logits' maximum.
 //
 // What bounds it: see beam_merge_kernel.
 __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs a, int per, int pieces,
                                                                        BeamPiece *__restrict__ piece,
                                                                        unsigned long long *__restrict__ best) {
+  constexpr int N = 4 * kBeamLoads;  // logits of a lane and chunk
   const int row = (int)(blockIdx.y + blockIdx.z * kBeamGridY), at = blockIdx.x, lane = threadIdx.x & (kWave - 1), W = a.W;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  if (row >= a.B * W || !beam_open(a, row)) return;
-  __shared__ unsigned long long keys[kBeamWaves][kBeamRoom];
-  __shared__ unsigned long long floor_key[kBeamWaves];
-  __shared__ float smax[kBeamWaves], ssum[kBeamWaves];
-  __shared__ int kept[kBeamWaves];
+  if (row >= a.B * W) return;
+  const float score = a.score[row];
+  const int over = a.done ? a.done[row] : 0;
+  __shared__ unsigned long long keys[kBeamWaves][kBeamRoom], last[kBeamWaves * kBeamRoom];
+  __shared__ __attribute__((aligned(16))) uint32_t high[kBeamWaves * kBeamRoom + 4];
+  __shared__ float tops[kBeamWaves][kWave], smax[kBeamWaves], ssum[kBeamWaves], sleast[kBeamWaves];
+  __shared__ int kept[kBeamWaves], count;
   const Rsrc x = make_rsrc(a.logits + (size_t)row * a.ld, 4u * (uint32_t)a.V);  // reads past the row give 0
   const int end = min(a.V, (at + 1) * per * kBeamStep);
   int v0 = at * per * kBeamStep + wave * kBeamChunk;
   unsigned long long *mine = keys[wave], low = 0;
-  float m = kBeamNone, sum = 0.0f, least = 0.0f;
+  float m = kBeamNone, sum = 0.0f, least;
   int n = 0;
-  bool begun = false;
-  float4 next[kBeamLoads];
-  const auto load = [&](int v) {
+  const auto load = [&](float *f, int v) {
 #pragma unroll
-    for (int i = 0; i < kBeamLoads; i++) next[i] = ld_f4(x, 4u * (uint32_t)(v + 4 * kWave * i + 4 * lane));
+    for (int i = 0; i < kBeamLoads; i++) {
+      const float4 q = ld_f4(x, 4u * (uint32_t)(v + 4 * kWave * i + 4 * lane));
+      f[4 * i] = q.x, f[4 * i + 1] = q.y, f[4 * i + 2] = q.z, f[4 * i + 3] = q.w;
+    }
   };
-  if (v0 < end) load(v0);
-  for (; v0 < end; v0 += kBeamStep) {
-    float f[4 * kBeamLoads];
-#pragma unroll
-    for (int i = 0; i < kBeamLoads; i++) f[4 * i] = next[i].x, f[4 * i + 1] = next[i].y, f[4 * i + 2] = next[i].z, f[4 * i + 3] = next[i].w;
-    if (v0 + kBeamStep < end) load(v0 + kBeamStep);
-    const auto token = [&](int i) { return v0 + 4 * kWave * (i >> 2) + 4 * lane + (i & 3); };
+  const auto token = [&](int i) { return v0 + 4 * kWave * (i >> 2) + 4 * lane + (i & 3); };
+  // a chunk's part of the sum; the largest logit of each load in tops4, and of all
+  const auto add = [&](float *f, float *tops4) {
     if (v0 + kBeamChunk > a.V) {
 #pragma unroll
-      for (int i = 0; i < 4 * kBeamLoads; i++) f[i] = token(i) < a.V ? f[i] : -INFINITY;
+      for (int i = 0; i < N; i++) f[i] = token(i) < a.V ? f[i] : -INFINITY;
     }
-    float top = f[0];
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < 4 * kBeamLoads; i++) top = fmaxf(top, f[i]);
+    for (int g = 0; g < kBeamLoads; g++) {
+      tops4[g] = fmaxf(fmaxf(f[4 * g], f[4 * g + 1]), fmaxf(f[4 * g + 2], f[4 * g + 3]));
+      top = fmaxf(top, tops4[g]);
+    }
     const float was = m;
     m = fmaxf(m, top);
     sum *= exp_below(was - m);
 #pragma unroll
-    for (int i = 0; i < 4 * kBeamLoads; i++) sum += exp_below(f[i] - m);
-    if (!begun) least = beam_threshold(fmaxf(top, -INFINITY), W), begun = true;
-    if (!__any(top >= least)) continue;
+    for (int i = 0; i < N; i++) sum += exp_below(f[i] - m);
+    return top;
+  };
+  // the chunk's keys that reach the threshold
+  const auto keep = [&](const float *f, const float *tops4, float top) {
+    if (!__any(top >= least)) return;
 #pragma unroll
-    for (int i = 0; i < 4 * kBeamLoads; i++) {
-      if (!__any(f[i] >= least)) continue;
-      const unsigned long long key = argmax_key(f[i], token(i)), push = __ballot(f[i] >= least && key > low);
-      if (push >> lane & 1) mine[n + __popcll(push & ((1ull << lane) - 1))] = key;
-      n += __popcll(push);
-      if (n > kBeamRoom - kWave) {
+    for (int g = 0; g < kBeamLoads; g++) {
+      if (!__any(tops4[g] >= least)) continue;
+      if (n > kBeamRoom - 4 * kWave) {
         __builtin_amdgcn_wave_barrier();
         low = beam_sort(mine, n, W);
         n = W;
         least = offer_logit(low);
       }
+#pragma unroll
+      for (int i = 4 * g; i < 4 * g + 4; i++) {
+        if (!__any(f[i] >= least)) continue;
+        const unsigned long long key = argmax_key(f[i], token(i)), push = __ballot(f[i] >= least && key > low);
+        if (push >> lane & 1) mine[n + __popcll(push & ((1ull << lane) - 1))] = key;
+        n += __popcll(push);
+      }
     }
+  };
+  float f0[N], f1[N], t0[kBeamLoads], t1[kBeamLoads], top0 = -INFINITY;
+  if (v0 < end) load(f0, v0);
+  if (over || !(score > -INFINITY)) return;  // (known when the first logits are on their way)
+  if (v0 < end) {
+    if (v0 + kBeamStep < end) load(f1, v0 + kBeamStep);
+    top0 = add(f0, t0);
+  }
+  // the first step's threshold: the W-th largest of 64 lanes' maxima over the waves
+  tops[wave][lane] = fmaxf(top0, -INFINITY);
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+  float first = tops[0][lane];
+#pragma unroll
+  for (int w = 1; w < kBeamWaves; w++) first = fmaxf(first, tops[w][lane]);
+  least = beam_threshold(first, W);
+  if (v0 < end) keep(f0, t0, top0);
+  for (v0 += kBeamStep; v0 < end; v0 += kBeamStep) {  // two chunks in turn, so that nothing is moved
+    if (v0 + kBeamStep < end) load(f0, v0 + kBeamStep);
+    const float top1 = add(f1, t1);
+    keep(f1, t1, top1);
+    v0 += kBeamStep;
+    if (v0 >= end) break;
+    if (v0 + kBeamStep < end) load(f1, v0 + kBeamStep);
+    top0 = add(f0, t0);
+    keep(f0, t0, top0);
   }
   // ---- the waves' sums and keys
   const float all = wave_max(m);
   const float part = wave_sum(sum * exp_below(m - all));
-  if (lane == 0) smax[wave] = all, ssum[wave] = part, kept[wave] = n, floor_key[wave] = low;
+  if (lane == 0) smax[wave] = all, ssum[wave] = part, kept[wave] = n, sleast[wave] = least;
   __syncthreads();
   const size_t to = (size_t)row * pieces + at;
-  float top = smax[0], total = 0.0f;
+  float top = smax[0], total = 0.0f, bar = sleast[0];
   int before[kBeamWaves + 1] = {0};
 #pragma unroll
   for (int w = 0; w < kBeamWaves; w++) {
     top = fmaxf(top, smax[w]);
-    low = floor_key[w] > low ? floor_key[w] : low;
+    bar = fmaxf(bar, sleast[w]);
     before[w + 1] = before[w] + kept[w];
   }
 #pragma unroll
   for (int w = 0; w < kBeamWaves; w++) total += ssum[w] * exp_below(smax[w] - top);
   if (threadIdx.x == 0) piece[to] = {top, total};
-  // a key's place is how many of the workgroup's are larger; a wave's W-th largest is no larger than theirs
-  n = before[kBeamWaves];
+  // W keys at least reach every wave's threshold; of those that reach the highest, a key's place is how many
+  // are larger
+  for (int i = threadIdx.x; i < before[kBeamWaves]; i += kBeamWaves * kWave) {
+    int w = 0;
+#pragma unroll
+    for (int k = 1; k < kBeamWaves; k++) w += i >= before[k];
+    const unsigned long long key = keys[w][i - before[w]];
+    if (offer_logit(key) >= bar) {
+      const int to = atomicAdd(&count, 1);
+      last[to] = key, high[to] = (uint32_t)(key >> 32);
+    }
+  }
+  __syncthreads();
+  n = count;
+  if (threadIdx.x < 4) high[n + threadIdx.x] = 0;
+  __syncthreads();
   for (int i = threadIdx.x; i < max(n, W); i += kBeamWaves * kWave) {
     if (i >= n) {
       best[to * W + i] = 0;
       continue;
     }
-    int w = 0;
-#pragma unroll
-    for (int k = 1; k < kBeamWaves; k++) w += i >= before[k];
-    const unsigned long long key = keys[w][i - before[w]];
-    if (key < low) continue;
-    int place = 0;
-#pragma unroll
-    for (int k = 0; k < kBeamWaves; k++)
-      for (int j = 0; j < kept[k]; j++) place += keys[k][j] > key;
+    const unsigned long long key = last[i];
+    const int place = beam_place(high, (n + 3) & ~3, (uint32_t)(key >> 32), [&](int j) { return j < n && last[j] > key; });
     if (place < W) best[to * W + place] = key;
   }
 }
 
 // ---------------------------------------------------------------- a prompt
 
-// An offer of the prompt's: larger sums first, then the lower place, then the larger key.
-struct BeamOffer {
-  unsigned long long sum, key;  // order_f64 of the sum (0: none); key of the logit, ~0: an ended beam itself
-  int beam;
-};
-__device__ __forceinline__ bool beam_before(const BeamOffer &a, const BeamOffer &b) {
-  return a.sum != b.sum ? a.sum > b.sum : a.beam != b.beam ? a.beam < b.beam : a.key > b.key;
-}
-
-// The W best offers lie in the W pieces whose first offers are the best: those and, of their further offers,
-// the ones that reach the last of them are put in order by counting who comes before whom.
-__global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int pieces,
+// Offers in order: larger sums first (as order_f64's numbers, 0 for none), then the lower place, then the larger
+// key; a key of ~0 is an ended beam itself. The W best offers lie in the W pieces whose first offers are the best: of those pieces the offers that reach
+// the last of the W first ones are put in order by counting who comes before whom.
+// (by_w and by_pieces: 65536 / W and 65536 / pieces, rounded up past, for divisions of less than 1024 and 256.)
+__global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int pieces, uint32_t by_w, uint32_t by_pieces,
                                                                 const BeamPiece *__restrict__ piece,
                                                                 const unsigned long long *__restrict__ best) {
   constexpr int kOffers = kMaxBeams * (kMaxBeams + 1) / 2;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, W = a.W, base = b * W;
+  const int b = blockIdx.x, tid = threadIdx.x, W = a.W, base = b * W;
   __shared__ double lse[kMaxBeams];
-  __shared__ BeamOffer head[kBeamHeads], offer[kOffers];
-  __shared__ int chosen[kMaxBeams], count;
-  const int heads = W * pieces, beam = min(tid / pieces, W - 1), row = base + beam;
+  __shared__ unsigned long long head_sum[kBeamHeads], head_key[kBeamHeads], sums[kOffers], keys[kOffers];
+  __shared__ __attribute__((aligned(16))) uint32_t head_top[kBeamHeads], tops[kOffers + 4];
+  __shared__ int beams[kOffers], chosen[kMaxBeams], count;
+  __shared__ float scores[kMaxBeams];
+  const int heads = W * pieces, beam = min((int)(tid * by_pieces >> 16), W - 1), row = base + beam;
+  // (what closed rows' pieces hold is read and not used: nothing waits for another load here)
+  const size_t list = ((size_t)base * pieces + min(tid, heads - 1)) * W;
+  const unsigned long long key = best[list];
   const float score = a.score[row];
-  const bool ended = a.done && a.done[row] && score > -INFINITY, open = beam_open(a, row);
-  const bool here = tid < heads && open;
-  const unsigned long long key = here ? best[((size_t)base * pieces + tid) * W] : 0;
+  const int over = a.done ? a.done[row] : 0;
+  const bool alive = score > -INFINITY, here = tid < heads && alive && !over;
   const int step = a.step ? a.step[b] : 0, none = max(a.eos, 0);
-  for (int r = wave; r < W; r += kBeamHeads / kWave) {  // a wave a row
+  // 256 / W lanes a row, a power of two: a piece each (four where W < 4), all rows at once
+  const int lane_bits = min(8 - (32 - __clz(W - 1)), 6), lanes = 1 << lane_bits, r = tid >> lane_bits;
+  {
     float m = kBeamNone, s = 0.0f;
-    if (beam_open(a, base + r))
-      for (int i = lane; i < pieces; i += kWave) {
+    if (r < W)
+      for (int i = tid & (lanes - 1); i < pieces; i += lanes) {
         const BeamPiece p = piece[(size_t)(base + r) * pieces + i];
         const float top = fmaxf(m, p.max);
         s = s * exp_below(m - top) + p.sum * exp_below(p.max - top);
         m = top;
       }
-    const float all = wave_max(m);
-    s = wave_sum(s * exp_below(m - all));
-    if (lane == 0) lse[r] = (double)all + log((double)s);
+    float all = m;
+    if (lanes == kWave) {
+      all = wave_max(m);
+      s = wave_sum(s * exp_below(m - all));
+    } else {
+      for (int o = 1; o < lanes; o <<= 1) all = fmaxf(all, __shfl_xor(all, o));
+      s *= exp_below(m - all);
+      for (int o = 1; o < lanes; o <<= 1) s += __shfl_xor(s, o);
+    }
+    if (r < W && !(tid & (lanes - 1))) lse[r] = (double)all + log((double)s);
   }
   if (tid < W) chosen[tid] = -1;
   if (tid == 0) count = 0;
   __syncthreads();
-  const auto sum_of = [&](int w, float s, unsigned long long k) -> unsigned long long {
-    const double x = (double)s + ((double)offer_logit(k) - lse[w]);
+  const auto sum_of = [&](double lse_, float s, unsigned long long k) -> unsigned long long {
+    const double x = (double)s + ((double)offer_logit(k) - lse_);
     return k && x > -INFINITY ? order_f64(x) : 0;
   };
-  BeamOffer mine = {0, key, beam};
-  if (here) mine.sum = sum_of(beam, score, key);
-  if (tid < heads && ended && tid % pieces == 0) mine = {order_f64(score), ~0ull, beam};
-  if (tid < heads) head[tid] = mine;
+  unsigned long long mine = here ? sum_of(lse[beam], score, key) : 0, own = key;
+  if (tid < heads && alive && over && tid == beam * pieces) mine = order_f64(score), own = ~0ull;
+  head_sum[tid] = mine, head_key[tid] = own, head_top[tid] = (uint32_t)(mine >> 32);
+  if (tid < heads && tid == beam * pieces) scores[beam] = score;
   __syncthreads();
   // ---- the W best pieces
-  if (mine.sum) {
-    int place = 0;
-    for (int j = 0; j < heads; j++) place += beam_before(head[j], mine);
+  if (mine) {
+    const int place = beam_place(head_top, (heads + 3) & ~3, (uint32_t)(mine >> 32), [&](int j) {
+      if (head_sum[j] != mine) return head_sum[j] > mine;
+      const int other = (int)(j * by_pieces >> 16);
+      return other < beam || (other == beam && head_key[j] > own);
+    });
     if (place < W) chosen[place] = tid;
   }
   __syncthreads();
-  // ---- their offers: the n-th of the q-th piece has q + n before it
+  // ---- their offers: the n-th of the q-th piece has at least q + n before it
   const int last = chosen[W - 1];
-  const unsigned long long least = last >= 0 ? head[last].sum : 1;
-  for (int i = tid; i < W * W; i += kBeamHeads) {
-    const int q = i / W, n = i % W, h = chosen[q];
-    if (h < 0 || q + n >= W) continue;
-    BeamOffer o = head[h];
-    if (n) {
-      if (o.key == ~0ull) continue;
-      o.key = best[((size_t)base * pieces + h) * W + n];
-      o.sum = sum_of(o.beam, a.score[base + o.beam], o.key);
-    }
-    if (o.sum && o.sum >= least) offer[atomicAdd(&count, 1)] = o;
+  const unsigned long long least = last >= 0 ? head_sum[last] : 1;
+  constexpr int PER = kMaxBeams * kMaxBeams / kBeamHeads;
+  unsigned long long next[PER];
+#pragma unroll
+  for (int p = 0; p < PER; p++) {  // all loads at once
+    if (kBeamHeads * p >= W * W) break;
+    const int i = tid + kBeamHeads * p, q = (int)(i * by_w >> 16), n = i - q * W, h = q + n < W ? chosen[q] : -1;
+    next[p] = 0;
+    if (h >= 0) next[p] = n ? best[((size_t)base * pieces + h) * W + n] : head_key[h];
+  }
+#pragma unroll
+  for (int p = 0; p < PER; p++) {
+    if (kBeamHeads * p >= W * W) break;
+    const int i = tid + kBeamHeads * p, q = (int)(i * by_w >> 16), n = i - q * W, h = q + n < W ? chosen[q] : -1;
+    if (h < 0 || (n && head_key[h] == ~0ull)) continue;
+    const int from = (int)(h * by_pieces >> 16);
+    const unsigned long long sum = n ? sum_of(lse[from], scores[from], next[p]) : head_sum[h];
+    if (!sum || sum < least) continue;
+    const int at = atomicAdd(&count, 1);
+    sums[at] = sum, keys[at] = next[p], beams[at] = from, tops[at] = (uint32_t)(sum >> 32);
   }
   __syncthreads();
   const int n = count;
+  if (tid < 4) tops[n + tid] = 0;
+  __syncthreads();
   const auto put = [&](int w, float s, int end, int tok, int parent) {
     a.new_score[base + w] = s;
     a.new_done[base + w] = end;
@@ -280,15 +353,16 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
     }
   };
   for (int i = tid; i < n; i += kBeamHeads) {
-    const BeamOffer o = offer[i];
-    int place = 0;
-    for (int j = 0; j < n; j++) place += beam_before(offer[j], o);
+    const unsigned long long u = sums[i], k = keys[i];
+    const int from = beams[i];
+    const int place = beam_place(tops, (n + 3) & ~3, (uint32_t)(u >> 32), [&](int j) {
+      if (j >= n || sums[j] != u) return j < n && sums[j] > u;
+      return beams[j] < from || (beams[j] == from && keys[j] > k);
+    });
     if (place >= W) continue;
-    const unsigned long long u = o.sum;
     const double s = __longlong_as_double((long long)(u >> 63 ? u & 0x7FFFFFFFFFFFFFFFull : ~u));
-    const bool itself = o.key == ~0ull;
-    const int tok = itself ? none : argmax_key_index(o.key);
-    put(place, (float)s, itself || tok == a.eos, tok, base + o.beam);
+    const int tok = k == ~0ull ? none : argmax_key_index(k);
+    put(place, (float)s, k == ~0ull || tok == a.eos, tok, base + from);
   }
   if (tid >= n && tid < W) put(tid, -INFINITY, 0, none, -1);
   if (a.step && tid == 0) a.step[b] = step + 1;
@@ -300,7 +374,7 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
 // pieces of a prompt than its merge has threads.
 static void beam_cut(int B, int W, int V, int &pieces, int &per) {
   const int steps = (V + kBeamStep - 1) / kBeamStep;
-  const int most = std::min({steps, kBeamHeads / W, std::max(1, 1024 / (B * W))});
+  const int most = std::min({steps, kBeamHeads / W, std::max(1, (getenv("BT") ? atoi(getenv("BT")) : 1024) / (B * W))});
   per = (steps + most - 1) / most;
   pieces = (steps + per - 1) / per;
 }
@@ -321,7 +395,8 @@ hipError_t launch_beam_select(const BeamArgs &a, void *work, hipStream_t s) {
   auto *best = reinterpret_cast<unsigned long long *>(static_cast<char *>(work) + piece_bytes(rows, pieces));
   const dim3 grid(pieces, std::min(rows, kBeamGridY), (rows + kBeamGridY - 1) / kBeamGridY);
   hipLaunchKernelGGL(beam_piece_kernel, grid, dim3(kBeamWaves * kWave), 0, s, a, per, pieces, piece, best);
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.B), dim3(kBeamHeads), 0, s, a, pieces, piece, best);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(a.B), dim3(kBeamHeads), 0, s, a, pieces, 65536u / a.W + 1,
+                     65536u / pieces + 1, piece, best);
   return hipGetLastError();
 }
 
