@@ -22,7 +22,7 @@ constexpr int kBeamChunk = 4 * kWave * kBeamLoads;       // logits a wave looks 
 constexpr int kBeamStep = kBeamChunk * kBeamWaves;       // a workgroup
 constexpr int kBeamRoom = 384;                           // keys that a wave has room for: 128, and 4 of every lane
 constexpr int kBeamGridY = 1 << 15;                      // rows in the grid's second dimension
-constexpr int kBeamHeads = 256;                          // pieces of a prompt's rows at most
+constexpr int kBeamHeads = 512;                          // pieces of a prompt's rows at most
 constexpr float kBeamNone = -3.4028234663852886e38f;     // the maximum before any logit: finite
 
 // What a workgroup leaves of its piece of a row: `best` keys, in descending order, 0 past the last.
@@ -44,6 +44,26 @@ __device__ __forceinline__ unsigned long long order_f64(double x) {
 // e^x by the hardware's 2^x: x log2 e rounded to float32, |x| 2^-24 of the result; where that is more
 // than 2^-20 the term is below e^-16 of the sum's largest.
 __device__ __forceinline__ float exp_below(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// A number that at least W of the lanes' reach and, if it can be, no more: found bit by bit from the top, as soon
+// as exactly W reach it nothing larger is needed. 0 where fewer than W are above 0.
+__device__ __forceinline__ uint32_t wave_reach(uint32_t k, int W) {
+  uint32_t t = 0;
+  for (int b = 31; b >= 0; b--) {
+    const uint32_t c = t | 1u << b;
+    const int n = __popcll((unsigned long long)__ballot(k >= c));
+    if (n >= W) t = c;
+    if (n == W) break;
+  }
+  return t;
+}
+
+// The same of n numbers in LDS, by the lanes' largest: W of them at least reach it, and few more.
+__device__ __forceinline__ uint32_t beam_reach(const uint32_t *top, int n, int W) {
+  uint32_t k = 0;
+  for (int i = threadIdx.x & (kWave - 1); i < n; i += kWave) k = max(k, top[i]);
+  return wave_reach(k, W);
+}
 
 // How many of n numbers (n a multiple of 4, all different but for zeros behind the last) are larger than one,
 // by their high words `top`; where others have the same one, `before` compares what is left. (64-bit
@@ -89,17 +109,9 @@ __device__ __attribute__((noinline)) unsigned long long beam_sort(unsigned long 
   return keys[W - 1];
 }
 
-// The largest float that at least W of the lanes' values reach (-inf: fewer are above -inf), found bit by bit
-// from the top on the values' ordered numbers; as soon as exactly W reach it nothing larger is needed.
+// The largest float that at least W of the lanes' values reach (all finite ones, where fewer are above -inf).
 __device__ __forceinline__ float beam_threshold(float v, int W) {
-  const uint32_t k = (uint32_t)(argmax_key(v, 0) >> 32);  // (v is not NaN)
-  uint32_t t = 0;
-  for (int b = 31; b >= 0; b--) {
-    const uint32_t c = t | 1u << b;
-    const int n = __popcll((unsigned long long)__ballot(k >= c));
-    if (n >= W) t = c;
-    if (n == W) break;
-  }
+  const uint32_t t = wave_reach((uint32_t)(argmax_key(v, 0) >> 32), W);  // (v is not NaN)
   return t < 0x00800000u ? kBeamNone : offer_logit((unsigned long long)t << 32);
 }
 
@@ -235,12 +247,14 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
   n = count;
   if (threadIdx.x < 4) high[n + threadIdx.x] = 0;
   __syncthreads();
+  const uint32_t reach = n > kWave ? beam_reach(high, n, W) : 0;  // (many: only the best are put in order)
   for (int i = threadIdx.x; i < max(n, W); i += kBeamWaves * kWave) {
     if (i >= n) {
       best[to * W + i] = 0;
       continue;
     }
     const unsigned long long key = last[i];
+    if ((uint32_t)(key >> 32) < reach) continue;
     const int place = beam_place(high, (n + 3) & ~3, (uint32_t)(key >> 32), [&](int j) { return j < n && last[j] > key; });
     if (place < W) best[to * W + place] = key;
   }
@@ -251,7 +265,7 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
 // Offers in order: larger sums first (as order_f64's numbers, 0 for none), then the lower place, then the larger
 // key; a key of ~0 is an ended beam itself. The W best offers lie in the W pieces whose first offers are the best: of those pieces the offers that reach
 // the last of the W first ones are put in order by counting who comes before whom.
-// (by_w and by_pieces: 65536 / W and 65536 / pieces, rounded up past, for divisions of less than 1024 and 256.)
+// (by_w and by_pieces: 2^16 / W and 2^20 / pieces and a bit more, for divisions of less than 1024 and 512.)
 __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int pieces, uint32_t by_w, uint32_t by_pieces,
                                                                 const BeamPiece *__restrict__ piece,
                                                                 const unsigned long long *__restrict__ best) {
@@ -262,7 +276,9 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
   __shared__ __attribute__((aligned(16))) uint32_t head_top[kBeamHeads], tops[kOffers + 4];
   __shared__ int beams[kOffers], chosen[kMaxBeams], count;
   __shared__ float scores[kMaxBeams];
-  const int heads = W * pieces, beam = min((int)(tid * by_pieces >> 16), W - 1), row = base + beam;
+  __shared__ int few[kBeamHeads], n_few;
+  __shared__ __attribute__((aligned(16))) uint32_t few_top[kBeamHeads + 4];
+  const int heads = W * pieces, beam = min((int)(tid * by_pieces >> 20), W - 1), row = base + beam;
   // (what closed rows' pieces hold is read and not used: nothing waits for another load here)
   const size_t list = ((size_t)base * pieces + min(tid, heads - 1)) * W;
   const unsigned long long key = best[list];
@@ -270,8 +286,8 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
   const int over = a.done ? a.done[row] : 0;
   const bool alive = score > -INFINITY, here = tid < heads && alive && !over;
   const int step = a.step ? a.step[b] : 0, none = max(a.eos, 0);
-  // 256 / W lanes a row, a power of two: a piece each (four where W < 4), all rows at once
-  const int lane_bits = min(8 - (32 - __clz(W - 1)), 6), lanes = 1 << lane_bits, r = tid >> lane_bits;
+  // lanes of a row: as many as there are, a power of two, at most a wave
+  const int lane_bits = min(9 - (32 - __clz(W - 1)), 6), lanes = 1 << lane_bits, r = tid >> lane_bits;
   {
     float m = kBeamNone, s = 0.0f;
     if (r < W)
@@ -293,7 +309,7 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
     if (r < W && !(tid & (lanes - 1))) lse[r] = (double)all + log((double)s);
   }
   if (tid < W) chosen[tid] = -1;
-  if (tid == 0) count = 0;
+  if (tid == 0) count = 0, n_few = 0;
   __syncthreads();
   const auto sum_of = [&](double lse_, float s, unsigned long long k) -> unsigned long long {
     const double x = (double)s + ((double)offer_logit(k) - lse_);
@@ -304,14 +320,26 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
   head_sum[tid] = mine, head_key[tid] = own, head_top[tid] = (uint32_t)(mine >> 32);
   if (tid < heads && tid == beam * pieces) scores[beam] = score;
   __syncthreads();
-  // ---- the W best pieces
-  if (mine) {
-    const int place = beam_place(head_top, (heads + 3) & ~3, (uint32_t)(mine >> 32), [&](int j) {
-      if (head_sum[j] != mine) return head_sum[j] > mine;
-      const int other = (int)(j * by_pieces >> 16);
-      return other < beam || (other == beam && head_key[j] > own);
+  // ---- the W best pieces: those that may be, then in order
+  const uint32_t may = beam_reach(head_top, heads, W);
+  if (mine && (uint32_t)(mine >> 32) >= may) {
+    const int to = atomicAdd(&n_few, 1);
+    few[to] = tid, few_top[to] = (uint32_t)(mine >> 32);
+  }
+  __syncthreads();
+  const int some = n_few;
+  if (tid < 4) few_top[some + tid] = 0;
+  __syncthreads();
+  if (tid < some) {
+    const int h = few[tid], of = (int)(h * by_pieces >> 20);
+    const unsigned long long sum = head_sum[h], k = head_key[h];
+    const int place = beam_place(few_top, (some + 3) & ~3, (uint32_t)(sum >> 32), [&](int j) {
+      if (j >= some) return false;
+      const int g = few[j], other = (int)(g * by_pieces >> 20);
+      if (head_sum[g] != sum) return head_sum[g] > sum;
+      return other < of || (other == of && head_key[g] > k);
     });
-    if (place < W) chosen[place] = tid;
+    if (place < W) chosen[place] = h;
   }
   __syncthreads();
   // ---- their offers: the n-th of the q-th piece has at least q + n before it
@@ -331,7 +359,7 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
     if (kBeamHeads * p >= W * W) break;
     const int i = tid + kBeamHeads * p, q = (int)(i * by_w >> 16), n = i - q * W, h = q + n < W ? chosen[q] : -1;
     if (h < 0 || (n && head_key[h] == ~0ull)) continue;
-    const int from = (int)(h * by_pieces >> 16);
+    const int from = (int)(h * by_pieces >> 20);
     const unsigned long long sum = n ? sum_of(lse[from], scores[from], next[p]) : head_sum[h];
     if (!sum || sum < least) continue;
     const int at = atomicAdd(&count, 1);
@@ -352,8 +380,10 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
       a.hist_parent[h] = parent;
     }
   };
+  const uint32_t reach = n > kWave ? beam_reach(tops, n, W) : 0;
   for (int i = tid; i < n; i += kBeamHeads) {
     const unsigned long long u = sums[i], k = keys[i];
+    if ((uint32_t)(u >> 32) < reach) continue;
     const int from = beams[i];
     const int place = beam_place(tops, (n + 3) & ~3, (uint32_t)(u >> 32), [&](int j) {
       if (j >= n || sums[j] != u) return j < n && sums[j] > u;
@@ -370,11 +400,12 @@ __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int 
 
 // ---------------------------------------------------------------- launchers
 
-// Pieces of a row and steps of each: at least a step a workgroup, four workgroups a compute unit, and no more
-// pieces of a prompt than its merge has threads.
+// Pieces of a row and steps of each: at least a step a workgroup, eight workgroups a compute unit (128 rows of
+// 151936: 22.1 us, four 24.2, two 29; 32 such beams of four prompts 44, 54, 64), and no more pieces of a prompt
+// than its merge has threads.
 static void beam_cut(int B, int W, int V, int &pieces, int &per) {
   const int steps = (V + kBeamStep - 1) / kBeamStep;
-  const int most = std::min({steps, kBeamHeads / W, std::max(1, (getenv("BT") ? atoi(getenv("BT")) : 1024) / (B * W))});
+  const int most = std::min({steps, kBeamHeads / W, std::max(1, 2048 / (B * W))});
   per = (steps + most - 1) / most;
   pieces = (steps + per - 1) / per;
 }
@@ -396,7 +427,7 @@ hipError_t launch_beam_select(const BeamArgs &a, void *work, hipStream_t s) {
   const dim3 grid(pieces, std::min(rows, kBeamGridY), (rows + kBeamGridY - 1) / kBeamGridY);
   hipLaunchKernelGGL(beam_piece_kernel, grid, dim3(kBeamWaves * kWave), 0, s, a, per, pieces, piece, best);
   hipLaunchKernelGGL(beam_merge_kernel, dim3(a.B), dim3(kBeamHeads), 0, s, a, pieces, 65536u / a.W + 1,
-                     65536u / pieces + 1, piece, best);
+                     (1u << 20) / pieces + 1, piece, best);
   return hipGetLastError();
 }
 

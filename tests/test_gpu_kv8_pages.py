@@ -127,11 +127,8 @@ def test_page_ends(rng):
     """A page that has just been filled is shared like the others, and the next one is each place's own."""
     W, page, wide = 4, 16, 4
     for n in (0, 1, 14, 15, 16, 17, 31, 62, 63, 64, 100, 2 ** 30, 2 ** 31 - 1):
-        state = list(family(rng, 2, W, page, wide, [5, 5]))
+        state = list(family(rng, 2, W, page, wide, [min(n, wide * page - 1)] * 2))
         state[1] = np.full(2 * W, n, np.int64).astype(np.int32)
-        at = min(n // page, wide - 1)
-        for g in (0, W):
-            state[2][g:g + W, at] = rng.permutation(np.setdiff1d(np.arange(state[0]), state[2])[:W])
         run(rng, 2, W, page, wide, 1, 1, 32, np.array([0, 0, 3, 3, 4, 5, 4, 4]), state=state)
 
 
