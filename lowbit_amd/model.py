@@ -29,7 +29,10 @@ run the unfused sequence on the matrix-core GEMMs.
 With a paged 8-bit cache (`new_cache(.., kv="e4m3")`, KV8Cache) the rotary embedding and
 the cache write are `lbd_kv8_append` and the attention `lbd_kv8_attention`, in prompts
 and steps alike; such a cache may hold several sequences, which `forward_batch` and
-`generate_batch` run together.
+`generate_batch` run together. With ModelConfig.window the attention sees a sliding window and
+the first `sinks` positions (`lbd_kv8_attention_window`, on such a cache only), and pages
+behind the window go back to the pool. `generate_beams` searches with beams: a prompt's beams
+are sequences of one cache that share their pages (`lbd_beam_select`, `lbd_kv8_reorder`).
 
 Same architecture and arithmetic as the reference model: RMSNorm in fp32, q/k/v
 projections concatenated along N and gate/up rows interleaved in (gate i, up i)
@@ -73,6 +76,8 @@ class ModelConfig:
     qkv_bias: bool = False
     max_position: int = 4096
     name: str = "custom"
+    window: int = 0  # positions that a token sees, itself among them; 0: all (no reference counterpart)
+    sinks: int = 0   # with a window: first positions that stay visible
 
 
 def tiny_config(**over) -> ModelConfig:
@@ -146,6 +151,8 @@ class KVCache:
     def __init__(self, cfg: ModelConfig, capacity: int):
         if capacity > 16000:
             raise ValueError("KV cache capacity above 16000 positions")
+        if cfg.window:
+            raise ValueError("a sliding window takes the 8-bit cache (kv='e4m3')")
         self.capacity = int(capacity)
         nb = cfg.num_kv_heads * self.capacity * cfg.head_dim * 4
         self.k = [_buf(nb) for _ in range(cfg.num_layers)]
@@ -166,7 +173,11 @@ class KV8Cache:
     codes, an E8M0 exponent for each page and KV head; lbd_kv8_* of include/lowbit_hip.h):
     a quarter of KVCache's bytes, no bound of 16000 positions, and sequences take pages as
     they grow. `lengths[s]` tokens of sequence s are valid. `capacity` positions a sequence;
-    `pages` in the pool (default: enough for every sequence at its capacity)."""
+    `pages` in the pool (default: enough for every sequence at its capacity).
+
+    Sequences may share pages (`fork`): a page belongs to all that hold it, and the first that is
+    about to write to one that others hold takes a copy. With a window pages that no later token
+    sees go back to the pool (`slide`)."""
 
     def __init__(self, cfg: ModelConfig, capacity: int, sequences: int = 1, page: int = 32, pages: int | None = None):
         if capacity <= 0 or sequences <= 0 or (pages is not None and pages <= 0):
@@ -176,23 +187,32 @@ class KV8Cache:
         if cfg.head_dim not in (32, 64, 128):
             raise ValueError("the 8-bit cache takes heads of 32, 64 or 128")
         self.capacity, self.page = int(capacity), int(page)
+        self.window, self.sinks = int(cfg.window), int(cfg.sinks)
         self.max_pages = -(-self.capacity // self.page)
         self.pages = int(sequences * self.max_pages if pages is None else pages)
-        kv, d = cfg.num_kv_heads, cfg.head_dim
-        codes, exps = self.pages * kv * self.page * d, self.pages * kv
+        self._kv, self._d = cfg.num_kv_heads, cfg.head_dim
         self.layers = []  # (lbd_kv8_pool, its buffers) of each layer; the layers share the page table
-        for _ in range(cfg.num_layers):
-            b = [_buf(codes), _buf(codes), _buf(exps), _buf(exps)]
-            self.layers.append((K.LbdKv8Pool(*(x.ptr for x in b), self.pages, self.page, kv, d), b))
+        self._set_layers([self._new_layer(self.pages) for _ in range(cfg.num_layers)])
         self.lengths = np.zeros(sequences, np.int64)
         self._held = np.zeros(sequences, np.int64)  # pages of each sequence
+        self._hole = np.zeros((sequences, 2), np.int64)  # of them those given back by slide
+        self._refs = np.zeros(self.pages, np.int64)  # sequences that hold each page
         self._free = list(range(self.pages - 1, -1, -1))
         self._table = np.full((sequences, self.max_pages), -1, np.int32)
         self._dirty = True
+        self._copies: list[list] = []  # (page, its copy) that upload makes, in batches one after the other
         self.table = _buf(self._table.nbytes)
         self.past, self.q_start = _buf(4 * sequences), _buf(4 * (sequences + 1))
         self.one = K.DeviceBuffer.from_array(np.array([0, 1], np.int32))  # q_start of a one-token step
         self.work = _buf(16)
+
+    def _new_layer(self, pages: int) -> list:
+        codes, exps = pages * self._kv * self.page * self._d, pages * self._kv
+        return [_buf(codes), _buf(codes), _buf(exps), _buf(exps)]
+
+    def _set_layers(self, buffers: list):
+        self.layers = [(K.LbdKv8Pool(*(x.ptr for x in b), self.pages, self.page, self._kv, self._d), b) for b in buffers]
+        self.pools = (K.LbdKv8Pool * len(buffers))(*(p for p, _ in self.layers))
 
     @property
     def length(self) -> int:
@@ -211,9 +231,13 @@ class KV8Cache:
         """Sequence `seq` keeps its first n tokens (pages past them return to the pool). The page that
         the last of them lies in keeps its blocks' exponents: tokens that are appended to it later
         are rounded in the unit that the dropped ones called for, and a block that a dropped token
-        made NaN stays NaN until the page is begun again (n a multiple of the page: at once)."""
+        made NaN stays NaN until the page is begun again (n a multiple of the page: at once). With a
+        window, what the next token would see must not have been given back."""
         if not 0 <= n <= self.lengths[seq]:
             raise ValueError(f"sequence {seq} does not hold {n} tokens")
+        a, b = self._hole[seq]
+        if b > a and n > a * self.page and n - self.window + 1 < b * self.page:
+            raise ValueError(f"pages of sequence {seq} that position {n} sees have been given back")
         self.commit(seq, n)
 
     def commit(self, seq: int, n: int):
@@ -222,40 +246,154 @@ class KV8Cache:
         keep = -(-int(n) // self.page)
         if n < 0 or keep > self._held[seq]:
             raise ValueError(f"sequence {seq} has no pages for {n} tokens")
-        gone = self._table[seq, keep:self._held[seq]]
-        self._free.extend(int(p) for p in gone[::-1])
+        self._drop(seq, keep, int(self._held[seq]))
+        if keep <= self._hole[seq, 0]:
+            self._hole[seq] = 0
+        self._held[seq], self.lengths[seq] = keep, n
+
+    def _drop(self, seq: int, first: int, last: int):
+        """Sequence `seq` no longer holds its pages first .. last - 1."""
+        gone = self._table[seq, first:last]
+        for p in gone[::-1]:
+            if p >= 0:
+                self._refs[p] -= 1
+                if not self._refs[p]:
+                    self._free.append(int(p))
         if len(gone):
             gone[:] = -1
             self._dirty = True
-        self._held[seq], self.lengths[seq] = keep, n
+
+    def _take(self) -> int:
+        p = self._free.pop()
+        self._refs[p] = 1
+        return p
 
     def reserve(self, seq: int, n: int):
-        """Pages for the first n positions of sequence `seq`."""
+        """Pages for the first n positions of sequence `seq`, the one that its next token goes to its own."""
         if n > self.capacity:
             raise ValueError(f"KV cache full ({n} > {self.capacity})")
         need, has = -(-int(n) // self.page), int(self._held[seq])
-        if need - has > len(self._free):
-            raise ValueError(f"KV cache full (no {need - has} pages left for sequence {seq})")
+        at, used = divmod(int(self.lengths[seq]), self.page)
+        shared = n > self.lengths[seq] and used and self._refs[self._table[seq, at]] > 1
+        more = max(need - has, 0) + bool(shared)
+        if more > len(self._free):
+            raise ValueError(f"KV cache full (no {more} pages left for sequence {seq})")
+        if shared:
+            p, mine = int(self._table[seq, at]), self._take()
+            self._refs[p] -= 1
+            self._table[seq, at] = mine
+            self._dirty = True
+            # copies of one batch are made at once: none may read or write what another writes
+            if not self._copies or any(mine in pair or p == pair[1] for pair in self._copies[-1]):
+                self._copies.append([])
+            self._copies[-1].append((p, mine))
         for i in range(has, need):
-            self._table[seq, i] = self._free.pop()
+            self._table[seq, i] = self._take()
             self._dirty = True
         self._held[seq] = max(need, has)
 
-    def upload(self):
-        """The page table to the device, where it changed."""
+    def fork(self, dst: int, src: int):
+        """Sequence `dst` becomes what `src` is (what it held returns to the pool): it shares its pages, none
+        is copied until one of them writes to it."""
+        if dst == src:
+            raise ValueError("a sequence cannot be forked onto itself")
+        self.commit(dst, 0)
+        n = -(-int(self.lengths[src]) // self.page)
+        self._table[dst, :n] = self._table[src, :n]
+        for p in self._table[dst, :n]:
+            if p >= 0:
+                self._refs[p] += 1
+        self._dirty = True
+        self._held[dst], self.lengths[dst], self._hole[dst] = n, self.lengths[src], self._hole[src]
+
+    def slide(self, seq: int):
+        """Pages that no token behind the sequence's last one sees return to the pool (with a window; the
+        model's passes call it)."""
+        if not self.window:
+            return
+        a, b = -(-self.sinks // self.page), max(int(self.lengths[seq]) - self.window + 1, 0) // self.page
+        if b > a:
+            self._drop(seq, a, b)
+            self._hole[seq] = a, b
+
+    def compact(self) -> int:
+        """The pages in use moved to the front of the pool; returns how many they are."""
+        self.upload()
+        held = np.flatnonzero(self._refs)
+        n = len(held)
+        src = held[held >= n]
+        dst = np.setdiff1d(np.arange(n), held)
+        if len(src):
+            to = np.arange(self.pages, dtype=np.int32)
+            to[src] = dst
+            self._copy(list(zip(src.tolist(), dst.tolist())), None)
+            self._table = np.where(self._table >= 0, to[self._table], -1).astype(np.int32)
+            self._refs[dst] = self._refs[src]
+            self._refs[src] = 0
+            self._dirty = True
+            _check(K.lib().lb_dev_synchronize(), "synchronize")
+        self._free = list(range(self.pages - 1, n - 1, -1))
+        return n
+
+    def resize(self, pages: int):
+        """A pool of `pages` pages; where it shrinks the pages in use are compacted first and have to fit."""
+        if pages <= 0 or pages < np.count_nonzero(self._refs):
+            raise ValueError(f"{np.count_nonzero(self._refs)} pages are in use")
+        if pages < self.pages:
+            self.compact()
+        else:
+            self.upload()
+        _check(K.lib().lb_dev_synchronize(), "synchronize")
+        keep, old = min(pages, self.pages), [b for _, b in self.layers]
+        fresh = [self._new_layer(pages) for _ in old]
+        for a, b in zip(old, fresh):
+            for x, y, n in zip(a, b, 2 * [keep * self._kv * self.page * self._d] + 2 * [keep * self._kv]):
+                _check(K.lib().lb_memcpy_d2d(y.ptr, x.ptr, n), "pool copy")
+        _check(K.lib().lb_dev_synchronize(), "synchronize")
+        self.pages = int(pages)
+        self._set_layers(fresh)
+        self._refs = np.concatenate([self._refs[:keep], np.zeros(pages - keep, np.int64)])
+        self._free = [int(p) for p in np.flatnonzero(self._refs == 0)[::-1]]
+
+    def _copy(self, pairs: list, stream):
+        """Pages copied in every layer, on `stream`."""
+        a = [K.DeviceBuffer.from_array(np.array(x, np.int32)) for x in zip(*pairs)]
+        _check(K.lib().lbd_kv8_copy_pages(self.pools, len(self.layers), a[0].ptr, a[1].ptr, len(pairs), stream),
+               "page copies")
+        self._moved = a  # alive until the next ones
+
+    def upload(self, stream=None):
+        """The page table to the device, where it changed, and the copies that forks called for."""
+        for batch in self._copies:
+            self._copy(batch, stream)
+            _check(K.lib().lb_stream_synchronize(stream), "synchronize")
+        self._copies = []
         if self._dirty:
             _check(K.lib().lb_memcpy_h2d(self.table.ptr, self._table.ctypes.data, self._table.nbytes), "table upload")
             self._dirty = False
 
-    def batch(self, q_start: int, past: int, seqs: int, max_new: int, rows: int) -> K.LbdKv8Batch:
+    def batch(self, q_start: int, past: int, seqs: int, max_new: int, rows: int, table: int | None = None) -> K.LbdKv8Batch:
         """The lbd_kv8_batch of the first `seqs` sequences (room: the workspace that its attention takes)."""
-        return K.LbdKv8Batch(q_start, past, self.table.ptr, seqs, self.max_pages, max_new, rows)
+        return K.LbdKv8Batch(q_start, past, table or self.table.ptr, seqs, self.max_pages, max_new, rows)
 
     def room(self, b: K.LbdKv8Batch, heads: int):
         """Grow `work` to what the attention of this batch takes (no call may be in flight)."""
-        need = K.lib().lbd_kv8_attention_work_bytes(C.byref(self.layers[0][0]), C.byref(b), heads)
+        L, pool, b = K.lib(), C.byref(self.layers[0][0]), C.byref(b)
+        need = (L.lbd_kv8_attention_window_work_bytes(pool, b, heads, self.window, self.sinks) if self.window
+                else L.lbd_kv8_attention_work_bytes(pool, b, heads))
         if need > self.work.nbytes:
             self.work = _buf(need)
+
+    def adopt(self, table: np.ndarray, lengths: np.ndarray):
+        """The sequences become those of a page table and their lengths (negative: none): every page belongs
+        to the sequences that name it, the others are free."""
+        self.lengths = np.maximum(np.asarray(lengths, np.int64), 0)
+        self._held = -(-self.lengths // self.page)
+        self._table = np.where(np.arange(self.max_pages) < self._held[:, None], table, -1).astype(np.int32)
+        self._refs = np.bincount(self._table[self._table >= 0], minlength=self.pages).astype(np.int64)
+        self._free = [int(p) for p in np.flatnonzero(self._refs == 0)[::-1]]
+        self._hole[self.lengths == 0] = 0
+        self._dirty = True
 
 
 @dataclass
@@ -291,6 +429,8 @@ class Model:
         for k in (cfg.hidden_size, cfg.intermediate_size, cfg.num_heads * cfg.head_dim):
             if k % blk:
                 raise ValueError(f"layer width {k} is not a multiple of the {backend} block ({blk})")
+        if cfg.window < 0 or cfg.sinks < 0 or (cfg.sinks and not cfg.window):
+            raise ValueError("window and sinks must not be negative, and sinks go with a window")
         self.cfg, self.backend, self.asym = cfg, backend, asym
         self.L = K.lib()
         s = C.c_void_p()
@@ -369,10 +509,11 @@ class Model:
     def linear_weight_bytes(self) -> int:
         return sum(x.nbytes for L in self.layers for x in (L.qkv, L.o, L.gate_up, L.down)) + self.lm_head.nbytes
 
-    def new_cache(self, max_len: int, kv: str = "fp32", sequences: int = 1, page: int = 32,
+    def new_cache(self, max_len: int, kv: str | None = None, sequences: int = 1, page: int = 32,
                   pages: int | None = None) -> "KVCache | KV8Cache":
-        """A cache of max_len positions: kv="fp32" (one sequence), or kv="e4m3", the paged 8-bit
-        cache of `sequences` sequences (KV8Cache)."""
+        """A cache of max_len positions: kv="fp32" (one sequence; the default without a window), or
+        kv="e4m3", the paged 8-bit cache of `sequences` sequences (KV8Cache)."""
+        kv = kv or ("e4m3" if self.cfg.window else "fp32")
         if kv == "fp32":
             if sequences != 1 or pages is not None:
                 raise ValueError("the fp32 cache holds one sequence, without pages")
@@ -479,8 +620,12 @@ class Model:
         width, pool, b = (H + 2 * cfg.num_kv_heads) * D, C.byref(cache.layers[li][0]), C.byref(self.batch)
         _check(L.lbd_kv8_append(pool, b, self.qkv.ptr, width, bias, H, self.cos.ptr, self.sin.ptr, cfg.max_position,
                                 self.qkv.ptr, width, s), "kv8 append")
-        _check(L.lbd_kv8_attention(pool, b, self.qkv.ptr, width, H, self.att.ptr, H * D, cache.work.ptr,
-                                   cache.work.nbytes, s), "kv8 attention")
+        if cache.window:
+            _check(L.lbd_kv8_attention_window(pool, b, self.qkv.ptr, width, H, cache.window, cache.sinks, self.att.ptr,
+                                              H * D, cache.work.ptr, cache.work.nbytes, s), "kv8 window attention")
+        else:
+            _check(L.lbd_kv8_attention(pool, b, self.qkv.ptr, width, H, self.att.ptr, H * D, cache.work.ptr,
+                                       cache.work.nbytes, s), "kv8 attention")
 
     def _plan_kv8(self, cache, T: int):
         """The batch of T tokens of a one-sequence 8-bit cache at position *pos."""
@@ -559,6 +704,7 @@ class Model:
         """A one-sequence cache after a pass that has written its first n tokens."""
         if isinstance(cache, KV8Cache):
             cache.commit(0, n)
+            cache.slide(0)
         else:
             cache.length = n
 
@@ -585,7 +731,7 @@ class Model:
         self._sync()
         if isinstance(cache, KV8Cache):
             cache.reserve(0, pos + T)
-            cache.upload()
+            cache.upload(self.stream)
             self._plan_kv8(cache, T)
         _check(self.L.lb_memcpy_h2d(self.tok.ptr, tokens.ctypes.data, 4 * T), "token upload")
         self._set_pos(pos)
@@ -625,7 +771,7 @@ class Model:
         self._sync()
         if isinstance(cache, KV8Cache):  # the whole answer's pages, so that the recorded step never changes
             cache.reserve(0, start + T + steps)
-            cache.upload()
+            cache.upload(self.stream)
             self._plan_kv8(cache, T)
         _check(L.lb_memcpy_h2d(self.tok.ptr, prompt.ctypes.data, 4 * T), "token upload")
         self._set_pos(start)
@@ -665,10 +811,9 @@ class Model:
 
     # ------------------------------------------------------------ several sequences
 
-    def forward_batch(self, tokens: list, cache: KV8Cache) -> np.ndarray:
-        """Run tokens[s] (possibly none) of each sequence s of an 8-bit cache behind what it holds:
-        prompts, chunks of prompts and single tokens in one pass. Returns the logits [S, V] of each
-        sequence's last token; rows of sequences without tokens are NaN."""
+    def _pass(self, tokens: list, cache: KV8Cache) -> tuple:
+        """tokens[s] of each sequence behind what it holds; (how many each had, the device's logits
+        [sequences, V] of their last ones, enqueued: rows of sequences without tokens are no one's)."""
         cfg, L = self.cfg, self.L
         S = len(cache.lengths) if isinstance(cache, KV8Cache) else -1
         if len(tokens) != S:
@@ -686,10 +831,8 @@ class Model:
                 cache.commit(i, int(cache.lengths[i]))
             raise
         self._sync()
-        if max(T, S) > self.tmax:
-            self._alloc(max(T, S))
-            self.tok = _buf(4 * max(T, S))
-        cache.upload()
+        self._rows(max(T, S))
+        cache.upload(self.stream)
         starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
         ends = np.where(news > 0, starts[1:] - 1, 0).astype(np.int32)
         past, tok = cache.lengths.astype(np.int32), np.concatenate(rows).astype(np.int32)
@@ -704,8 +847,23 @@ class Model:
         _check(L.lbd_embed(self.h.ptr, T, cfg.hidden_size, index.ptr, S, rows_h.ptr, self.stream), "row gather")
         self._linear(self.lm_head, rows_h.ptr, S, out.ptr)
         self._sync()
-        cache.lengths += news
-        y = out.to_array((S, cfg.vocab_size), np.float32)
+        for i in np.flatnonzero(news):
+            cache.lengths[i] += news[i]
+            cache.slide(i)
+        return news, out
+
+    def _rows(self, n: int):
+        """Buffers of at least n rows (no call may be in flight)."""
+        if n > self.tmax:
+            self._alloc(n)
+            self.tok = _buf(4 * n)
+
+    def forward_batch(self, tokens: list, cache: KV8Cache) -> np.ndarray:
+        """Run tokens[s] (possibly none) of each sequence s of an 8-bit cache behind what it holds:
+        prompts, chunks of prompts and single tokens in one pass. Returns the logits [S, V] of each
+        sequence's last token; rows of sequences without tokens are NaN."""
+        news, out = self._pass(tokens, cache)
+        y = out.to_array((len(news), self.cfg.vocab_size), np.float32)
         y[news == 0] = np.nan
         return y
 
@@ -726,4 +884,147 @@ class Model:
                 o.append(int(v))
             if i + 1 < n_new:
                 y = self.forward_batch([[int(v)] for v in tok], cache)
+        return out
+
+    def generate_beams(self, prompts: list, n_new: int, beams: int = 4, eos: int = -1, length_penalty: float = 1.0,
+                       cache: KV8Cache | None = None, graph: bool = True) -> list[list[tuple[list[int], float]]]:
+        """Beam search (lbd_beam_select): the `beams` best continuations of n_new tokens of each prompt by the
+        sum of their log-probabilities, as (tokens, sum), best first by sum / length ** length_penalty. A beam
+        that takes token `eos` has ended (its tokens end there): it keeps its sum and its place among the
+        prompt's as long as no `beams` others exceed it. Fewer beams come back where the vocabulary offers no
+        more.
+
+        Beam w of prompt p is sequence p * beams + w of the cache (default: one of its own); a given cache may
+        hold tokens in the first sequence of each prompt, which the prompt continues, and the others must be
+        empty. Beams share the pages of what they have in common. Afterwards the sequences hold the
+        beams in the order of their sums, all but their last token; ended beams hold nothing.
+
+        The search stays on the device: selection, the page tables' new order and the next token's embedding
+        read each other's results, and the steps replay one recorded HIP graph of two (graph=False launches
+        them one by one). With eos the host looks every 32 steps whether all beams have ended."""
+        cfg, L, s = self.cfg, self.L, self.stream
+        G, W, V = len(prompts), int(beams), cfg.vocab_size
+        if not G or not all(len(p) for p in prompts):
+            raise ValueError("no tokens")
+        if not 1 <= W <= 32:
+            raise ValueError("1 to 32 beams")
+        if not -1 <= eos < V:
+            raise ValueError("eos is a token or -1")
+        if n_new <= 0:
+            return [[] for _ in prompts]
+        n, steps = G * W, n_new - 1
+        if cache is None:
+            longest, page = max(len(p) for p in prompts) + steps, 16
+            own = -(-steps // page) + 1  # pages that a beam may write
+            cache = self.new_cache(longest, "e4m3", n, page, sum(-(-len(p) // page) for p in prompts) + n * own)
+        if not isinstance(cache, KV8Cache) or len(cache.lengths) != n:
+            raise ValueError(f"the cache must be a KV8Cache of {n} sequences")
+        firsts = np.arange(0, n, W)
+        if np.delete(cache.lengths, firsts).any():
+            raise ValueError("only the first sequence of each prompt may hold tokens")
+        for g, p in zip(firsts, prompts):
+            if cache.lengths[g] + len(p) + steps > cache.capacity:
+                raise ValueError(f"KV cache full ({cache.lengths[g]}+{len(p)}+{steps} > {cache.capacity})")
+        _, logits = self._pass([prompts[i // W] if i % W == 0 else [] for i in range(n)], cache)
+        hole = cache._hole[firsts].copy()
+        # every place's own pages, from the one that its prompt's next token goes to
+        own = np.full((n, cache.max_pages), -1, np.int32)
+        try:
+            for g in firsts:
+                cache.reserve(g, int(cache.lengths[g]) + steps)
+                tail = int(cache.lengths[g]) // cache.page
+                own[g, tail:cache._held[g]] = cache._table[g, tail:cache._held[g]]
+                for i in range(g + 1, g + W):
+                    if cache._held[g] - tail > len(cache._free):
+                        raise ValueError("KV cache full (no pages left for the beams)")
+                    own[i, tail:cache._held[g]] = [cache._take() for _ in range(tail, cache._held[g])]
+        except ValueError:
+            cache.adopt(cache._table, cache.lengths)
+            raise
+        cache.upload(s)
+        up, lengths = K.DeviceBuffer.from_array, np.where(np.arange(n) % W == 0, cache.lengths, -1).astype(np.int32)
+        sums = np.where(np.arange(n) % W == 0, 0.0, -np.inf).astype(np.float32)
+        # two states in turn: a step reads one and writes the other
+        state = [dict(past=up(lengths), table=up(cache._table), score=up(sums), done=up(np.zeros(n, np.int32)))
+                 for _ in range(2)]
+        parent, mine, count = up(np.zeros(n, np.int32)), up(own), up(np.zeros(G, np.int32))
+        hist = [up(np.zeros((n_new, n), np.int32)) for _ in range(2)]
+        self._rows(n)
+        choose = [K.LbdBeams(a["score"].ptr, a["done"].ptr, b["score"].ptr, b["done"].ptr, self.tok.ptr, parent.ptr,
+                             hist[0].ptr, hist[1].ptr, count.ptr, n_new, G, W, V, eos) for a, b in (state, state[::-1])]
+        work = _buf(L.lbd_beam_select_work_bytes(C.byref(choose[0])))
+        q_start = up(np.arange(n + 1, dtype=np.int32))
+        batches = [cache.batch(q_start.ptr, x["past"].ptr, n, 1, n, x["table"].ptr) for x in state]
+        cache.room(batches[0], cfg.num_heads)
+
+        def select(x: int, add: int):
+            """The beams of state x into the other one."""
+            a, b = state[x], state[1 - x]
+            _check(L.lbd_beam_select(logits.ptr, V, C.byref(choose[x]), work.ptr, work.nbytes, s), "beam selection")
+            order = K.LbdKv8Order(parent.ptr, b["done"].ptr, a["past"].ptr, a["table"].ptr, mine.ptr, b["past"].ptr,
+                                  b["table"].ptr, G, W, cache.max_pages, add)
+            _check(L.lbd_kv8_reorder(cache.pools, len(cache.layers), C.byref(order), s), "beam order")
+
+        def step(x: int):
+            self.batch = batches[x]
+            self._layers(n, cache)
+            self._linear(self.lm_head, self.h.ptr, n, logits.ptr)
+            select(x, 1)
+
+        select(0, 0)
+        x, left = 1, steps
+        if left:  # the first step builds what later ones find (tile layouts), outside of any graph
+            step(x)
+            x, left = 1 - x, left - 1
+        ex = C.c_void_p()
+        try:
+            if graph and left >= 2:
+                self._sync()
+                _check(L.lb_stream_begin_capture(s), "begin capture")
+                try:
+                    step(x)
+                    step(1 - x)
+                finally:
+                    _check(L.lb_stream_end_capture(s, C.byref(ex)), "end capture")
+            since = 0
+            while left:
+                if ex.value and left >= 2:
+                    _check(L.lb_graph_launch(ex.value, s), "graph launch")
+                    took = 2
+                else:
+                    step(x)
+                    took, x = 1, 1 - x
+                left, since = left - took, since + took
+                if eos >= 0 and since >= 32 and left:
+                    since = 0
+                    self._sync()
+                    ended = state[x]["done"].to_array((n,), np.int32) != 0
+                    if (ended | (state[x]["score"].to_array((n,), np.float32) == -np.inf)).all():
+                        break
+            self._sync()
+        finally:
+            if ex.value:
+                L.lb_graph_destroy(ex.value)
+        took = n_new - left
+        tok, back = (h.to_array((n_new, n), np.int32)[:took] for h in hist)
+        sums, ended = state[x]["score"].to_array((n,), np.float32), state[x]["done"].to_array((n,), np.int32)
+        cache.adopt(state[x]["table"].to_array((n, cache.max_pages), np.int32), state[x]["past"].to_array((n,), np.int32))
+        for i in np.flatnonzero(cache.lengths):
+            cache._hole[i] = hole[i // W]
+            cache.slide(i)
+        out = []
+        for g in firsts:
+            found = []
+            for i in range(g, g + W):
+                if back[-1, i] < 0:
+                    continue
+                answer, at = [], i
+                for t in range(took - 1, -1, -1):
+                    answer.append(int(tok[t, at]))
+                    at = back[t, at]
+                answer.reverse()
+                if ended[i]:  # it has taken eos once, and stood as it was since
+                    answer = answer[:answer.index(eos) + 1]
+                found.append((answer, float(sums[i])))
+            out.append(sorted(found, key=lambda b: -b[1] / len(b[0]) ** length_penalty))
         return out

@@ -1,0 +1,242 @@
+"""The decoder's beam search, forks and sliding window on the paged 8-bit cache (GPU).
+
+The search is compared with one driven by the host: the same passes on forked sequences, and the oracle's
+selection in 64 bits. Logits of the two differ by rounding (the LM head takes other numbers of rows), a
+sum of n of them by no more than n 1e-4 here, and the random models' offers lie further apart."""
+import numpy as np
+import pytest
+
+from lowbit_amd import model as M
+from oracle import beams as B
+from test_gpu_kv8_model import pool_of
+from test_gpu_kv8 import check
+
+pytestmark = pytest.mark.gpu
+
+
+def model_of(backend="w4a16", seed=1, **over):
+    cfg = M.tiny_config(max_position=500, **over)
+    return M.Model(cfg, M.random_weights(cfg, seed=seed), backend, max_tokens=8)
+
+
+def by_hand(model, prompts, n_new, W, eos, page):
+    """[(tokens, sum)] of each prompt, best first, by forks and passes of the cache's public calls."""
+    G, V = len(prompts), model.cfg.vocab_size
+    n = G * W
+    cache = model.new_cache(max(map(len, prompts)) + n_new, "e4m3", 2 * n, page)  # the beams and their parents
+    y = model.forward_batch([prompts[i // W] if i < n and i % W == 0 else [] for i in range(2 * n)], cache)[:n]
+    score = np.where(np.arange(n) % W == 0, 0, -np.inf).astype(np.float32)
+    done, beams = np.zeros(n, int), [[] for _ in range(n)]
+    for t in range(n_new):
+        tok, parent, total, end = B.select(np.nan_to_num(y), score, done, W, eos)
+        for i in range(n):
+            cache.truncate(n + i)
+        for i in range(n):
+            if parent[i] >= 0 and not end[i]:
+                cache.fork(n + i, parent[i])
+        for i in range(n):
+            cache.truncate(i)
+        for i in range(n):
+            if parent[i] >= 0 and not end[i]:
+                cache.fork(i, n + i)
+                cache.truncate(n + i)
+        beams = [beams[p] + ([int(v)] if p >= 0 and not done[p] else []) if p >= 0 else None
+                 for p, v in zip(parent, tok)]
+        score, done = total.astype(np.float32), end
+        if t + 1 < n_new:
+            feed = [[int(tok[i])] if parent[i] >= 0 and not done[i] else [] for i in range(n)]
+            if not any(feed):
+                break
+            y = model.forward_batch(feed + [[] for _ in range(n)], cache)[:n]
+    return [[(beams[i], float(score[i])) for i in range(g, g + W) if beams[i] is not None] for g in range(0, n, W)]
+
+
+def same(got, want, n_new):
+    for a, b in zip(got, want):
+        assert [t for t, _ in a] == [t for t, _ in sorted(b, key=lambda x: -x[1])]
+        assert np.allclose([s for _, s in a], [s for _, s in sorted(b, key=lambda x: -x[1])], atol=1e-4 * n_new)
+
+
+@pytest.mark.parametrize("backend", M.BACKENDS)
+@pytest.mark.parametrize("W", [1, 3, 4])
+def test_one_prompt(backend, W):
+    model = model_of(backend)
+    prompt = [list(np.random.default_rng(2).integers(0, 97, 21))]
+    got = model.generate_beams(prompt, 14, W, length_penalty=0.0)
+    assert len(got[0]) == W and all(len(t) == 14 for t, _ in got[0])
+    same(got, by_hand(model, prompt, 14, W, -1, 16), 14)
+    eager = model.generate_beams(prompt, 14, W, length_penalty=0.0, graph=False)
+    assert got == eager
+    if W == 1:
+        assert got[0][0][0] == model.generate(prompt[0], 14, model.new_cache(64, kv="e4m3", page=16))
+
+
+@pytest.mark.parametrize("page", [16, 32])
+def test_several_prompts(page):
+    """Prompts of other lengths, over page ends, on a given cache."""
+    model = model_of()
+    rng = np.random.default_rng(5)
+    prompts = [list(rng.integers(0, 97, n)) for n in (15, 1, 32, 47)]
+    cache = model.new_cache(47 + 40, "e4m3", 4 * 5, page)
+    got = model.generate_beams(prompts, 40, 5, length_penalty=0.0, cache=cache)
+    same(got, by_hand(model, prompts, 40, 5, -1, page), 40)
+    # the sequences hold the beams, all but their last token: one pass more gives what the search would have seen
+    for g in range(4):
+        assert list(cache.lengths[5 * g:5 * g + 5]) == [len(prompts[g]) + 39] * 5
+    assert sorted(cache._free) == list(np.flatnonzero(cache._refs == 0))
+    y = model.forward_batch([[t[-1]] for g in got for t, _ in g], cache)
+    for g in range(4):
+        for w, (t, _) in enumerate(got[g]):
+            alone = model.new_cache(200, "e4m3", page=page)
+            z = model.forward(prompts[g], alone)
+            for v in t:
+                z = model.forward([v], alone)
+            assert np.abs(y[5 * g + w] - z).max() < 1e-2 * np.abs(z).max()
+
+
+@pytest.mark.parametrize("n_new", [1, 2, 3, 4, 5, 20])
+def test_numbers_of_tokens(n_new):
+    model = model_of()
+    prompts = [list(np.random.default_rng(n).integers(0, 97, n)) for n in (16, 3)]
+    cache = model.new_cache(60, "e4m3", 8, 16)
+    got = model.generate_beams(prompts, n_new, 4, length_penalty=0.0, cache=cache)
+    same(got, by_hand(model, prompts, n_new, 4, -1, 16), n_new)
+    assert list(cache.lengths) == [16 + n_new - 1] * 4 + [3 + n_new - 1] * 4
+    held = cache._table[cache._table >= 0]
+    assert np.array_equal(np.bincount(held, minlength=cache.pages), cache._refs)
+    assert all((cache._table[i, :h] >= 0).all() for i, h in enumerate(cache._held))
+
+
+def test_beams_that_end():
+    """With an end token that comes up: ended beams keep their tokens up to it, and stop early together."""
+    model = model_of(seed=4)
+    prompts = [list(np.random.default_rng(n).integers(0, 97, n)) for n in (9, 14)]
+    free = model.generate_beams(prompts, 30, 4, length_penalty=0.0)
+    eos = free[0][0][0][5]
+    got = model.generate_beams(prompts, 30, 4, eos=eos, length_penalty=0.0)
+    want = by_hand(model, prompts, 30, 4, eos, 16)
+    same(got, want, 30)
+    assert any(len(t) < 30 and t[-1] == eos for g in got for t, _ in g)
+    assert all(eos not in t[:-1] for g in got for t, _ in g)
+    longer = model.generate_beams(prompts, 200, 4, eos=eos, length_penalty=1.0)
+    for g in longer:
+        ranks = [s / len(t) for t, s in g]
+        assert ranks == sorted(ranks, reverse=True)
+
+
+def test_continued():
+    """A search behind earlier turns whose pages are shared: the other sequence keeps what it holds."""
+    model = model_of()
+    rng = np.random.default_rng(8)
+    head, prompt = list(rng.integers(0, 97, 37)), list(rng.integers(0, 97, 6))
+    cache = model.new_cache(120, "e4m3", 3, 16, 30)
+    model.forward_batch([head, [], []], cache)
+    got = model.generate_beams([prompt], 12, 3, length_penalty=0.0, cache=cache)
+    fresh = model.new_cache(120, "e4m3", 3, 16)
+    model.forward_batch([head, [], []], fresh)
+    assert got == model.generate_beams([prompt], 12, 3, length_penalty=0.0, cache=fresh)
+    same(got, by_hand(model, [head + prompt], 12, 3, -1, 16), 12)
+
+
+def test_refusals():
+    model = model_of()
+    ok = [[1, 2], [3]]
+    full = model.new_cache(50, "e4m3", 4)
+    model.forward_batch([[1], [2], [], []], full)
+    small = model.new_cache(50, "e4m3", 4, 16, 3)
+    before = len(small._free)
+    for bad in (dict(prompts=[]), dict(prompts=[[1], []]), dict(beams=0), dict(beams=33), dict(eos=97), dict(eos=-2),
+                dict(cache=model.new_cache(50)), dict(cache=model.new_cache(50, "e4m3", 3)), dict(cache=full),
+                dict(cache=model.new_cache(10, "e4m3", 4)), dict(cache=small)):
+        with pytest.raises(ValueError):
+            model.generate_beams(**{**dict(prompts=ok, n_new=20, beams=2), **bad})
+    with pytest.raises(IndexError):
+        model.generate_beams([[97]], 3)
+    assert model.generate_beams(ok, 0) == [[], []]
+    held = small._table[small._table >= 0]
+    assert np.array_equal(np.bincount(held, minlength=3), small._refs) and before == 3
+
+
+# ---------------------------------------------------------------- forks
+
+def test_forks():
+    """A fork and a sequence that got the same tokens by itself are the same from then on, bit for bit; so
+    they are in a compacted and in a resized pool."""
+    model = model_of()
+    rng = np.random.default_rng(3)
+    t = lambda n: list(rng.integers(0, 97, n))  # noqa: E731
+    p, q = t(21), t(30)
+    a, b = (model.new_cache(100, "e4m3", 3, 16, 24) for _ in range(2))
+    for c in (a, b):
+        model.forward_batch([p, [], []], c)
+    a.fork(1, 0)
+    model.forward_batch([[], p, []], b)
+    for c in (a, b):
+        model.forward_batch([[], [], q], c)
+    assert len(a._free) == len(b._free) + 2
+    for i in range(12):
+        step = [t(1), t(1), t(1) if i % 3 else []]
+        x, y = model.forward_batch(step, a), model.forward_batch(step, b)
+        assert np.array_equal(x, y, equal_nan=True)
+        if i == 4:
+            a.truncate(2)
+            b.truncate(2)
+            assert a.compact() == len(np.unique(a._table[a._table >= 0]))
+        if i == 7:
+            a.resize(13)
+            a.resize(20)
+    a.fork(2, 1)
+    step = [[], t(1), []]
+    x, y = model.forward_batch(step, a), model.forward_batch(step, b)
+    assert np.array_equal(x[1], y[1])
+    assert np.array_equal(model.forward_batch([[], [], step[1]], a)[2], y[1])
+
+
+# ---------------------------------------------------------------- a window
+
+@pytest.mark.parametrize("window,sinks", [(24, 4), (1, 0), (50, 16), (33, 0)])
+def test_window(window, sinks):
+    """One layer: the attention of its own rows over the cache, by the oracle with a window."""
+    cfg = M.tiny_config(num_layers=1, max_position=400, window=window, sinks=sinks)
+    model = M.Model(cfg, M.random_weights(cfg, seed=3), "w4a16")
+    H, KV, D = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+    cache = model.new_cache(300, page=16, pages=16)
+    assert isinstance(cache, M.KV8Cache)
+    rng, past = np.random.default_rng(0), 0
+    for n in (37, 1, 1, 60, 1, 90, 1):
+        table = cache._table.copy()
+        model.forward(rng.integers(0, 97, n), cache)
+        rows = model.qkv.to_array((n, (H + 2 * KV) * D), np.float32)
+        cache_now = cache._table.copy()
+        # the pages as the pass saw them: those that it gave back afterwards were held
+        device = cache.table.to_array(cache._table.shape, np.int32)
+        assert (device[table >= 0] == table[table >= 0]).all() and (cache_now[device < 0] < 0).all()
+        pool, ref = pool_of(cache), np.zeros((n, H * D))
+        mags = pool.attention([0, n], [past], device, n, rows[:, :H * D], H, ref, window, sinks)
+        check(model.att.to_array((n, H * D), np.float32), ref, mags, D, H)
+        past += n
+    assert cache.length == past
+    used = (cache._table >= 0).sum()
+    assert used <= -(-sinks // 16) + window // 16 + 2
+
+
+def test_a_window_generates():
+    """Prompt, graph, eager steps and beams with a window; a cache of few pages serves a long answer by steps."""
+    model = model_of(window=20, sinks=4)
+    prompt = list(np.random.default_rng(1).integers(0, 97, 50))
+    a = model.generate(prompt, 40)
+    assert a == model.generate(prompt, 40, model.new_cache(120, page=32), graph=False)
+    cache, c = model.new_cache(120, page=16, pages=6), []
+    y = model.forward(prompt, cache)
+    for _ in range(40):
+        c.append(int(y.argmax()))
+        y = model.forward(c[-1:], cache)
+    assert a == c
+    with pytest.raises(ValueError):
+        cache.truncate(0, 60)
+    got = model.generate_beams([prompt], 25, 3, length_penalty=0.0)
+    same(got, by_hand(model, [prompt], 25, 3, -1, 16), 25)
+    with pytest.raises(ValueError):
+        model.new_cache(50, kv="fp32")
+    wide = model_of(window=400)
+    assert wide.generate(prompt, 20) == model_of().generate(prompt, 20, model_of().new_cache(100, kv="e4m3"))

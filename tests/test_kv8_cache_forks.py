@@ -1,0 +1,218 @@
+"""KV8Cache's shared pages on the CPU: forks, copies on the first write, pages behind a window, compaction and
+resizing. Its device buffers are stand-ins; page copies are carried out on a table of what each page holds."""
+import numpy as np
+import pytest
+
+from lowbit_amd import kernels as K
+from lowbit_amd import model as M
+from test_kv8_cache import Buffer
+
+
+class Lib:
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+
+@pytest.fixture
+def new(monkeypatch):
+    monkeypatch.setattr(M, "_buf", Buffer)
+    monkeypatch.setattr(K.DeviceBuffer, "from_array", classmethod(lambda cls, a: Buffer(a.nbytes)))
+    monkeypatch.setattr(K, "lib", lambda: Lib())
+
+    def make(*a, window=0, sinks=0, **k):
+        cache = M.KV8Cache(M.tiny_config(window=window, sinks=sinks), *a, **k)
+        cache.held = {p: {} for p in range(cache.pages)}  # page -> slot -> token
+
+        def copy(pairs, stream):
+            was = {p: dict(c) for p, c in cache.held.items()}
+            assert not {d for _, d in pairs} & {x for i, (x, _) in enumerate(pairs)}
+            for x, y in pairs:
+                cache.held[y] = was[x]
+        cache._copy = copy
+        return cache
+
+    return make
+
+
+def write(cache, seq, tokens):
+    """What a pass does that appends tokens: nothing is written to a page that another sequence holds."""
+    at = int(cache.lengths[seq])
+    cache.reserve(seq, at + len(tokens))
+    cache.upload()
+    for i, t in enumerate(tokens):
+        p, slot = int(cache._table[seq, (at + i) // cache.page]), (at + i) % cache.page
+        assert cache._refs[p] == 1
+        if slot == 0:
+            cache.held[p] = {}
+        cache.held[p][slot] = t
+    cache.commit(seq, at + len(tokens))
+    cache.slide(seq)
+
+
+def read(cache, seq):
+    cache.upload()
+    return [cache.held[int(cache._table[seq, i // cache.page])].get(i % cache.page) if
+            cache._table[seq, i // cache.page] >= 0 else None for i in range(int(cache.lengths[seq]))]
+
+
+def consistent(cache):
+    held = cache._table[cache._table >= 0]
+    assert np.array_equal(np.bincount(held, minlength=cache.pages), cache._refs)
+    assert sorted(cache._free) == list(np.flatnonzero(cache._refs == 0))
+    for i, n in enumerate(cache._held):
+        a, b = cache._hole[i]
+        assert (cache._table[i, n:] < 0).all() and (cache._table[i, a:b] < 0).all()
+        assert (np.delete(cache._table[i, :n], np.arange(a, min(b, n))) >= 0).all()
+
+
+def test_a_fork_shares_until_it_writes(new):
+    cache = new(100, page=16, sequences=3, pages=20)
+    write(cache, 0, list(range(40)))
+    cache.fork(1, 0)
+    assert len(cache._free) == 17 and list(cache.lengths) == [40, 40, 0]
+    write(cache, 0, [100])  # the first to write takes a copy of the third page
+    write(cache, 1, [200])  # and leaves it to the other
+    assert len(cache._free) == 16
+    assert read(cache, 0) == [*range(40), 100] and read(cache, 1) == [*range(40), 200]
+    cache.fork(2, 1)
+    cache.truncate(1, 10)
+    write(cache, 1, [5, 6])  # into a page that two others hold
+    assert read(cache, 1) == [*range(10), 5, 6] and read(cache, 2) == [*range(40), 200]
+    cache.truncate(0)
+    cache.truncate(2)
+    consistent(cache)
+    assert len(cache._free) == 19
+    with pytest.raises(ValueError):
+        cache.fork(1, 1)
+
+
+def test_full_pages_are_shared_for_good(new):
+    cache = new(64, page=16, sequences=2, pages=4)
+    write(cache, 0, list(range(32)))
+    cache.fork(1, 0)
+    write(cache, 1, [7])  # begins a page of its own: nothing is copied
+    assert not cache._copies and len(cache._free) == 1
+    with pytest.raises(ValueError):  # two pages more than there are
+        write(cache, 0, [1] * 20)
+    write(cache, 0, [8])
+    assert read(cache, 0)[-1] == 8 and read(cache, 1)[-1] == 7
+    consistent(cache)
+
+
+def test_no_page_for_a_copy(new):
+    cache = new(64, page=16, sequences=2, pages=1)
+    write(cache, 0, [1, 2])
+    cache.fork(1, 0)
+    with pytest.raises(ValueError):
+        cache.reserve(1, 3)
+    cache.reserve(1, 2)  # no new token: no copy
+    consistent(cache)
+    cache.truncate(0)
+    write(cache, 1, [3])
+    assert read(cache, 1) == [1, 2, 3]
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 0), (17, 5), (1, 0), (16, 16), (33, 40)])
+def test_at_random(new, window, sinks):
+    """Forks, writes, cuts, compactions and resizing in any order: every sequence keeps its tokens."""
+    rng = np.random.default_rng(window + sinks)
+    cache = new(90, page=16, sequences=5, pages=24, window=window, sinks=sinks)
+    want, tick = [[] for _ in range(5)], 0
+    for _ in range(800):
+        s, what = int(rng.integers(5)), rng.random()
+        try:
+            if what < 0.55:
+                n = int(rng.integers(1, 12))
+                write(cache, s, list(range(tick, tick + n)))
+                want[s] = want[s] + list(range(tick, tick + n))
+                tick += n
+            elif what < 0.7:
+                d = (s + int(rng.integers(1, 5))) % 5
+                cache.fork(d, s)
+                want[d] = list(want[s])
+            elif what < 0.85:
+                n = int(rng.integers(0, len(want[s]) + 1)) if rng.random() < 0.7 else 0
+                cache.truncate(s, n)
+                want[s] = want[s][:n]
+            elif what < 0.95:
+                assert cache.compact() == np.count_nonzero(cache._refs)
+                assert not cache._refs[np.count_nonzero(cache._refs):].any()
+            else:
+                n = int(rng.integers(18, 30))
+                cache.resize(n)
+                cache.held = {p: cache.held.get(p, {}) for p in range(n)}
+                assert cache.pages == n
+        except ValueError:
+            for i in range(5):  # what a refused pass had reserved
+                cache.commit(i, len(want[i]))
+        consistent(cache)
+        for i in range(5):
+            n = len(want[i])
+            assert cache.lengths[i] == n
+            got = read(cache, i)
+            for at in range(n):  # what the next token sees
+                if not window or at < sinks or at > n - window:
+                    assert got[at] == want[i][at]
+        held = sum(len(set(range(n)) - {x for x in range(n) if window and x >= -(-sinks // 16) * 16
+                                        and x // 16 < max(n - window + 1, 0) // 16}) for n in map(len, want))
+        assert (cache._table >= 0).sum() * 16 - 15 * 5 <= held
+
+
+def test_pages_behind_a_window(new):
+    cache = new(1000, page=16, sequences=1, pages=6, window=40, sinks=4)
+    for t in range(500):  # far more tokens than the pool has slots
+        write(cache, 0, [t])
+    assert cache.length == 500 and len(cache._free) >= 1
+    assert read(cache, 0)[:4] == [0, 1, 2, 3] and read(cache, 0)[-39:] == list(range(461, 500))
+    for n in (499, 470, 100, 17):
+        with pytest.raises(ValueError):
+            if n == 499:
+                cache.truncate(0, 459)
+            else:
+                cache.truncate(0, n)
+    cache.truncate(0, 499)  # position 499 still sees 460 .. 498
+    cache.truncate(0, 10)   # only the sinks' page
+    consistent(cache)
+    write(cache, 0, [9] * 30)
+    assert read(cache, 0)[:10] == list(range(10))
+
+
+def test_resize_refuses(new):
+    cache = new(64, page=16, sequences=2, pages=6)
+    write(cache, 0, [1] * 40)
+    for n in (0, -1, 2):
+        with pytest.raises(ValueError):
+            cache.resize(n)
+    cache.resize(3)
+    with pytest.raises(ValueError):
+        write(cache, 1, [1])
+    cache.resize(4)
+    write(cache, 1, [1])
+    consistent(cache)
+
+
+def test_batches_of_copies(new):
+    """A copy's page freed and taken again before the copies are made: they are made one after the other."""
+    cache = new(64, page=16, sequences=4, pages=4)
+    write(cache, 0, [1, 2])
+    cache.fork(1, 0)
+    cache.reserve(1, 3)        # copy of 0's page
+    cache.fork(2, 0)
+    cache.commit(1, 0)         # its page returns
+    cache.reserve(2, 3)        # and is taken for another copy
+    cache.fork(3, 2)
+    cache.commit(0, 0)
+    cache.reserve(3, 3)
+    cache.upload()
+    cache.commit(2, 2)
+    cache.commit(3, 2)
+    assert read(cache, 2) == [1, 2] and read(cache, 3) == [1, 2]
+    consistent(cache)
+
+
+def test_a_window_takes_the_8_bit_cache():
+    with pytest.raises(ValueError):
+        M.KVCache(M.tiny_config(window=8), 10)
+    for bad in (dict(window=-1), dict(window=4, sinks=-1), dict(sinks=3)):
+        with pytest.raises(ValueError):
+            M.Model(M.tiny_config(**bad), {})
