@@ -545,9 +545,9 @@ typedef struct {
  * are its new beams. Equal sums: the lower place first, within a beam the larger logit, then the
  * lower token. Sums are compared in float64 and rounded to float32 once; sum exp x is added in
  * float32. An offer of -inf (a masked token) is none; a beam whose logits hold a NaN or +inf, or
- * are all -inf, offers nothing; rows of ended beams and of no beam are not read. Where fewer than
- * W are offered the last places get parent -1, sum -inf. tok of an ended beam and of no beam is
- * eos (0 without one), a token that may be embedded like any other. work:
+ * are all -inf, offers nothing; rows of ended beams and of no beam may hold anything. Where fewer
+ * than W are offered the last places get parent -1, sum -inf. tok of an ended beam and of no beam is
+ * eos (0 without one), a token that may be embedded like any other. logits 4-byte aligned. work:
  * lbd_beam_select_work_bytes of the same arguments (0: they are refused), 16-byte aligned; it
  * needs no clearing, and calls that share it must be ordered. */
 size_t lbd_beam_select_work_bytes(const lbd_beams *beams);

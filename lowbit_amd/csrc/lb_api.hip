@@ -1681,6 +1681,7 @@ int lbd_beam_select(const float *logits, int ld, const lbd_beams *beams, void *w
   if (ld < a.V) return fail(LB_ERR_SHAPE, "bad shape: rows of ld >= V floats");
   if (!logits || !a.score || !a.new_score || !a.new_done || !a.tok || !a.parent)
     return fail(LB_ERR_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(logits) & 3) return fail(LB_ERR_ARG, "logits must be 4-byte aligned");
   const bool hist = a.hist_tok || a.hist_parent || a.step;
   if (hist && (!a.hist_tok || !a.hist_parent || !a.step || a.hist_len <= 0))
     return fail(LB_ERR_ARG, "hist_tok, hist_parent, step and hist_len come together");

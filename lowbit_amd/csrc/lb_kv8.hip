@@ -1375,8 +1375,9 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     // finds its place anew (1000 tokens, 32 heads on 8: 37.6 us, with four a row block 40.2).
     p.merge = rows <= 512 ? 0 : blocks * a.KV >= 256 ? 1 : std::max(1, R * D / 1024);
     p.at = plan.floats + kKv8CutHead;
-    p.sums = (size_t)units * a.KV * R * D;
-    plan.floats = p.at + p.sums + (size_t)units * a.KV * R * 4;
+    const size_t slots = p.cut.min_keys == kKv8Whole ? 0 : units;  // one slice each: no sums to hand on
+    p.sums = slots * a.KV * R * D;
+    plan.floats = p.at + p.sums + slots * a.KV * R * 4;
     plan.parts++;
     return true;
   };

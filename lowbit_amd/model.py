@@ -902,8 +902,8 @@ class Model:
         The search stays on the device: selection, the page tables' new order and the next token's embedding
         read each other's results, and the steps replay one recorded HIP graph of two (graph=False launches
         them one by one). With eos the host looks every 32 steps whether all beams have ended."""
-        cfg, L, s = self.cfg, self.L, self.stream
-        G, W, V = len(prompts), int(beams), cfg.vocab_size
+        cfg = self.cfg
+        G, W, V, eos = len(prompts), int(beams), cfg.vocab_size, int(eos)
         if not G or not all(len(p) for p in prompts):
             raise ValueError("no tokens")
         if not 1 <= W <= 32:
@@ -922,9 +922,16 @@ class Model:
         firsts = np.arange(0, n, W)
         if np.delete(cache.lengths, firsts).any():
             raise ValueError("only the first sequence of each prompt may hold tokens")
+        need = 0
         for g, p in zip(firsts, prompts):
-            if cache.lengths[g] + len(p) + steps > cache.capacity:
-                raise ValueError(f"KV cache full ({cache.lengths[g]}+{len(p)}+{steps} > {cache.capacity})")
+            was, end = int(cache.lengths[g]), int(cache.lengths[g]) + len(p)
+            if end + steps > cache.capacity:
+                raise ValueError(f"KV cache full ({was}+{len(p)}+{steps} > {cache.capacity})")
+            last = -(-(end + steps) // cache.page)  # every beam's pages from the one in writing on, the prompt's before
+            need += last - int(cache._held[g]) + (W - 1) * (last - end // cache.page)
+            need += bool(was % cache.page and cache._refs[cache._table[g, was // cache.page]] > 1)
+        if need > len(cache._free):
+            raise ValueError(f"KV cache full ({need} pages for the beams, {len(cache._free)} left)")
         _, logits = self._pass([prompts[i // W] if i % W == 0 else [] for i in range(n)], cache)
         hole = cache._hole[firsts].copy()
         # every place's own pages, from the one that its prompt's next token goes to
@@ -932,15 +939,21 @@ class Model:
         try:
             for g in firsts:
                 cache.reserve(g, int(cache.lengths[g]) + steps)
-                tail = int(cache.lengths[g]) // cache.page
-                own[g, tail:cache._held[g]] = cache._table[g, tail:cache._held[g]]
+                tail, last = int(cache.lengths[g]) // cache.page, int(cache._held[g])
+                own[g, tail:last] = cache._table[g, tail:last]
                 for i in range(g + 1, g + W):
-                    if cache._held[g] - tail > len(cache._free):
-                        raise ValueError("KV cache full (no pages left for the beams)")
-                    own[i, tail:cache._held[g]] = [cache._take() for _ in range(tail, cache._held[g])]
-        except ValueError:
-            cache.adopt(cache._table, cache.lengths)
+                    own[i, tail:last] = [cache._take() for _ in range(tail, last)]
+            return self._search(logits, own, hole, cache, G, W, n_new, eos, length_penalty, graph)
+        except BaseException:
+            cache.adopt(cache._table, cache.lengths)  # the prompts, as they were read
             raise
+
+    def _search(self, logits, own, hole, cache: KV8Cache, G: int, W: int, n_new: int, eos: int, length_penalty: float,
+                graph: bool) -> list:
+        """generate_beams behind its prompts' pass: `logits` of their last tokens, the places' own pages, the
+        pages that a window had given back."""
+        cfg, L, s = self.cfg, self.L, self.stream
+        n, V, steps, firsts = G * W, cfg.vocab_size, n_new - 1, np.arange(0, G * W, W)
         cache.upload(s)
         up, lengths = K.DeviceBuffer.from_array, np.where(np.arange(n) % W == 0, cache.lengths, -1).astype(np.int32)
         sums = np.where(np.arange(n) % W == 0, 0.0, -np.inf).astype(np.float32)

@@ -111,7 +111,7 @@ def test_select_shapes(over):
 
 
 @pytest.mark.parametrize("over,rc", [
-    (dict(ld=99), -1), (dict(eos=100), -6), (dict(eos=-2), -6), (dict(logits=None), -6), (dict(null=True), -6),
+    (dict(ld=99), -1), (dict(logits=P + 2), -6), (dict(eos=100), -6), (dict(eos=-2), -6), (dict(logits=None), -6), (dict(null=True), -6),
     (dict(work=None), -6), (dict(work=P + 8), -6), (dict(work_bytes=16), -6), (dict(hist_tok=P), -6),
     (dict(step=P, hist_len=3), -6), (dict(hist_tok=P, hist_parent=P, step=P), -6)] + [
     (dict([(n, None)]), -6) for n in ("score", "new_score", "new_done", "tok", "parent")], ids=str)

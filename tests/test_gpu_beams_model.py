@@ -153,6 +153,17 @@ def test_refusals():
     with pytest.raises(IndexError):
         model.generate_beams([[97]], 3)
     assert model.generate_beams(ok, 0) == [[], []]
+    assert not small.lengths.any() and len(small._free) == 3  # refused before anything was read
+    # just as many pages as the search takes: the prompt's full one, and three of each beam's own
+    for pages in (6, 7):
+        tight = model.new_cache(60, "e4m3", 2, 16, pages)
+        model.forward_batch([[5] * 20, []], tight)
+        if pages == 6:
+            with pytest.raises(ValueError):
+                model.generate_beams([[7, 8]], 39, 2, cache=tight)
+            assert list(tight.lengths) == [20, 0]
+        else:
+            assert len(model.generate_beams([[7, 8]], 39, 2, cache=tight)[0]) == 2
     held = small._table[small._table >= 0]
     assert np.array_equal(np.bincount(held, minlength=3), small._refs) and before == 3
 
