@@ -66,8 +66,7 @@ __device__ __forceinline__ uint32_t beam_reach(const uint32_t *top, int n, int W
 }
 
 // How many of n numbers (n a multiple of 4, all different but for zeros behind the last) are larger than one,
-// by their high words `top`; where others have the same one, `before` compares what is left. (64-bit
-// comparisons throughout took three times as long.)
+// by their high words `top`; where others have the same one, `before` compares what is left.
 template <class F>
 __device__ __forceinline__ int beam_place(const uint32_t *top, int n, uint32_t one, F before) {
   int place = 0, same = 0;
@@ -120,7 +119,10 @@ __device__ __forceinline__ float beam_threshold(float v, int W) {
 // later ones come from sorting the kept keys out where they run out of room. So most chunks end after a
 // comparison of 16 logits' maximum.
 //
-// What bounds it: see beam_merge_kernel.
+// What bounds it: 128 rows of 151936 logits the instructions, 17 us = 4.3 TB/s (of a wave's 530 vector
+// instructions 16 a chunk are exponentials and 48 their arguments and sum), and 2.4 steps a workgroup between its
+// beginning and end; four such rows the launch and two loads one after the other, 4 us. The threshold of a
+// wave's own first chunk kept four times as many keys (25.9 us), sixteen tests for room a chunk 20.8.
 __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs a, int per, int pieces,
                                                                        BeamPiece *__restrict__ piece,
                                                                        unsigned long long *__restrict__ best) {
@@ -265,6 +267,9 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
 // Offers in order: larger sums first (as order_f64's numbers, 0 for none), then the lower place, then the larger
 // key; a key of ~0 is an ended beam itself. The W best offers lie in the W pieces whose first offers are the best: of those pieces the offers that reach
 // the last of the W first ones are put in order by counting who comes before whom.
+// What bounds it: three loads one after the other (sums and first offers, the chosen pieces' others, none of
+// them near) and as many barriers, 4.2 us for 4 beams, 4.8 for 16 prompts' 8, 14 for 32. Counted among all 152
+// first offers, not the few that reach the threshold, 6 us; all comparisons on 64-bit structures 20.
 // (by_w and by_pieces: 2^16 / W and 2^20 / pieces and a bit more, for divisions of less than 1024 and 512.)
 __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int pieces, uint32_t by_w, uint32_t by_pieces,
                                                                 const BeamPiece *__restrict__ piece,

@@ -557,6 +557,16 @@ struct Kv8Lds {
   float sm[NW][kv8_rows(NC)], sl[NW][kv8_rows(NC)], smid[NW];
 };
 
+//
+// WIN: a window. A row block's keys are those that a row of it may see, counted without the gap
+// behind the sinks (positions come back in load_tiles and in the mask), and everything else is as
+// it is for a short sequence. What bounds it: 61 steps in windows of 4096 behind up to 30000, 32 heads on
+// 8 of 128, the bytes, 498 MB in 98 us and 5 for the merge (whole caches masked: 200 us); 2048 tokens in
+// 512 the instructions, 54 us: 18 chunks a row block, and a third of them in the waves' beginnings and
+// ends (whole caches masked: 104). Tried for those: one wave a workgroup (15 to 20 % faster at windows of
+// 128 and 2000 row blocks, as much slower at 1024), eight (8 to 15 % faster at D = 64 and up to 256 row
+// blocks, 20 to 80 % slower else), and output stored straight from the matrix layout, 16 of a line's 128
+// bytes at a time (10 to 20 % slower).
 template <int D, int NC, bool WIN, int NW>
 __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, int kv, int unit,
                                            const float *__restrict__ q, int q_stride, float *__restrict__ out,
@@ -1356,12 +1366,11 @@ static bool kv8_plan(const Kv8Args &a, int D, int H, Kv8Plan &plan) {
     } else {
       blocks = std::min((long long)a.T * G / R + a.B, (long long)a.T * ((G + R - 1) / R));
       const int fits = 256 * (D == 128 ? 3 : 4);  // workgroups that the device holds
-      // A window of few keys: row blocks enough for half of the compute units are taken whole, so that
+      // A window of few keys, or row blocks enough for half of the compute units: taken whole, so that
       // nobody decides on slices and no second launch looks for them (2048 tokens, 32 heads on 8 of 128,
-      // windows of 512 and 1024: 64.3 -> 57.9 us and 85.5 -> 78.7; 200 tokens of them, 208 row blocks, 26.1
-      // -> 22.1; 200 of 14 heads on 2 of 64, 88 row blocks: 15.8, whole 16.1, and 40 of the 32 heads, 48:
-      // 16.7 and 20.8).
-      const bool whole = a.window && span <= kKv8Whole && blocks * a.KV >= 128;
+      // windows of 512 and 1024: 64.3 -> 57.9 us and 85.5 -> 78.7; 200 tokens of them in 1024, 208 row blocks,
+      // 26.1 -> 22.1, 80 tokens, 88 row blocks: 19.4, whole 21.6; 40 tokens in 600, 48 row blocks, 18.6 -> 15.6).
+      const bool whole = a.window && (span <= 768 || (span <= kKv8Whole && blocks * a.KV >= 128));
       p.cut = {G, R, nc + 3, rows_min, rows_max, whole ? kKv8Whole : 256, g_inv, 0, 0, whole ? 0 : each(2 * fits),
                256.0f / (float)a.KV, (float)fits / (float)a.KV, span};
     }
