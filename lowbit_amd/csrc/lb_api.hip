@@ -1553,7 +1553,9 @@ int kv8_attend(const lbk::Kv8Args &a, int D, const float *q, int q_stride, int H
   if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ARG, "q and out must be 16-byte aligned");
   const size_t need = lbk::kv8_attention_work_bytes(a, D, H);
   if (!need) return fail(LB_ERR_SHAPE, "too many rows of heads for a launch");
-  if (!work || work_bytes < need) return fail(LB_ERR_ARG, "work smaller than lbd_kv8_attention_work_bytes");
+  if (!work || work_bytes < need)
+    return fail(LB_ERR_ARG, a.window ? "work smaller than lbd_kv8_attention_window_work_bytes"
+                                     : "work smaller than lbd_kv8_attention_work_bytes");
   if (!aligned16(work)) return fail(LB_ERR_ARG, "work must be 16-byte aligned");
   LB_LAUNCH(lbk::launch_kv8_attention(a, D, q, q_stride, H, out, out_stride, work, static_cast<hipStream_t>(stream)),
             "kv8 attention launch");

@@ -83,8 +83,10 @@ __device__ __forceinline__ int beam_place(const uint32_t *top, int n, uint32_t o
 // ---------------------------------------------------------------- pieces of rows
 
 // The W largest of n keys (n <= kBeamRoom, W <= n, all different), by one wave, to the front in descending
-// order: a key's place is how many are larger. Returns the last of them.
-__device__ __attribute__((noinline)) unsigned long long beam_sort(unsigned long long *keys, int n, int W) {
+// order: a key's place is how many are larger. Returns the last of them. A function of its own, as a dozen places
+// call it and hardly any call comes; by an LDS pointer, whose accesses happen in order.
+typedef __attribute__((address_space(3))) unsigned long long LdsKey;
+__device__ __attribute__((noinline)) unsigned long long beam_sort(LdsKey *keys, int n, int W) {
   constexpr int PER = kBeamRoom / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   unsigned long long mine[PER];
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
       if (!__any(tops4[g] >= least)) continue;
       if (n > kBeamRoom - 4 * kWave) {
         __builtin_amdgcn_wave_barrier();
-        low = beam_sort(mine, n, W);
+        low = beam_sort((LdsKey *)mine, n, W);
         n = W;
         least = offer_logit(low);
       }
@@ -265,8 +267,10 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
 // ---------------------------------------------------------------- a prompt
 
 // Offers in order: larger sums first (as order_f64's numbers, 0 for none), then the lower place, then the larger
-// key; a key of ~0 is an ended beam itself. The W best offers lie in the W pieces whose first offers are the best: of those pieces the offers that reach
-// the last of the W first ones are put in order by counting who comes before whom.
+// key; a key of ~0 is an ended beam itself. The W best lie in the W pieces whose first offers are the best: of
+// those pieces the offers that reach the last of the W first ones are put in order by counting who comes before
+// whom.
+//
 // What bounds it: three loads one after the other (sums and first offers, the chosen pieces' others, none of
 // them near) and as many barriers, 4.2 us for 4 beams, 4.8 for 16 prompts' 8, 14 for 32. Counted among all 152
 // first offers, not the few that reach the threshold, 6 us; all comparisons on 64-bit structures 20.

@@ -630,10 +630,10 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     t_ve = in ? t_ve : -1;
   };
   constexpr bool BIG = NC == 2;  // the query rows laid out by the waves together, in LDS
-  constexpr int QB = BIG && NW > 1 ? 1 : NB;
+  constexpr int QB = BIG ? 1 : NB;
   v8h qh[QB][KS], ql[QB][SEP ? KS : 1];
   float4 qf[QB][KS][2];
-  if constexpr (BIG && NW > 1) qr[0] = wave & 1 ? qr[1] : qr[0];
+  if constexpr (BIG) qr[0] = wave & 1 ? qr[1] : qr[0];
 #pragma unroll
   for (int y = 0; y < QB; y++)
 #pragma unroll
@@ -728,7 +728,7 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     cx[y] = down * (kKv8Log2e / sqrtf((float)D));
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      if (BIG && NW > 1 && s * NW / 2 / KS != wave / 2) continue;  // another wave's
+      if (BIG && s * NW / 2 / KS != wave / 2) continue;  // another wave's
       const float4 a0 = qf[y][s][0], a1 = qf[y][s][1];
       const float x[8] = {a0.x * up, a0.y * up, a0.z * up, a0.w * up, a1.x * up, a1.y * up, a1.z * up, a1.w * up};
 #pragma unroll
@@ -745,16 +745,15 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
         }
       }
       if constexpr (BIG) {
-        const int at = ((NW > 1 ? wave & 1 : y) * KS + s) * 2;
-        lds.q[at][lane] = __builtin_bit_cast(uint4, qh[y][s]);
-        lds.q[at + 1][lane] = __builtin_bit_cast(uint4, ql[y][s]);
+        lds.q[((wave & 1) * KS + s) * 2][lane] = __builtin_bit_cast(uint4, qh[0][s]);
+        lds.q[((wave & 1) * KS + s) * 2 + 1][lane] = __builtin_bit_cast(uint4, ql[0][s]);
       }
     }
   }
   if constexpr (BIG) {
-    if (NW > 1 && g == 0 && wave < 2) lds.cx[wave][c] = cx[0];
+    if (g == 0 && wave < 2) lds.cx[wave][c] = cx[0];
     __syncthreads();
-    if constexpr (NW > 1) cx[0] = lds.cx[0][c], cx[NB - 1] = lds.cx[1][c];
+    cx[0] = lds.cx[0][c], cx[NB - 1] = lds.cx[1][c];
   }
 
   float m[NB], l[NB];
@@ -1005,35 +1004,32 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
     lds.sl[0][rr] = (M - u.m) + u.mid;
   }
   __syncthreads();
-  if constexpr (BIG && NW < 4) {
-    // each of two waves adds up one column block's rows; into LDS a row's elements lie side by side
+  if constexpr (BIG && NW == 2) {
+    // each wave adds up one column block's rows; in LDS a row's elements lie side by side
 #pragma unroll
     for (int y = 0; y < NB; y++) {
       const float f = lds.sm[wave][16 * y + c];
 #pragma unroll
       for (int j = 0; j < VB; j++) acc[y][j] *= f;
     }
-    if constexpr (NW == 2) {
 #pragma unroll
-      for (int j = 0; j < VB; j++) lds.ex[wave][j][lane] = wave ? acc[0][j] : acc[1][j];
-      __syncthreads();
+    for (int j = 0; j < VB; j++) lds.ex[wave][j][lane] = wave ? acc[0][j] : acc[1][j];
+    __syncthreads();
 #pragma unroll
-      for (int j = 0; j < VB; j++) acc[0][j] = (wave ? acc[1][j] : acc[0][j]) + lds.ex[1 - wave][j][lane];
-      __syncthreads();
-    }
+    for (int j = 0; j < VB; j++) acc[0][j] = (wave ? acc[1][j] : acc[0][j]) + lds.ex[1 - wave][j][lane];
+    __syncthreads();
 #pragma unroll
-    for (int y = 0; y < (NW == 1 ? NB : 1); y++)
+    for (int e = 0; e < 4; e++) {
+      float *row = &lds.sh[0][16 * wave + c][4 * VB * g + VB * e];
+      if constexpr (VB >= 4) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float *row = &lds.sh[0][16 * (NW == 1 ? y : wave) + c][4 * VB * g + VB * e];
-        if constexpr (VB >= 4) {
-#pragma unroll
-          for (int j = 0; j < VB; j += 4)
-            *reinterpret_cast<float4 *>(row + j) = make_float4(acc[y][j][e], acc[y][j + 1][e], acc[y][j + 2][e], acc[y][j + 3][e]);
-        } else {
-          *reinterpret_cast<float2 *>(row) = make_float2(acc[y][0][e], acc[y][1][e]);
-        }
+        for (int j = 0; j < VB; j += 4)
+          *reinterpret_cast<float4 *>(row + j) =
+              make_float4(acc[0][j][e], acc[0][j + 1][e], acc[0][j + 2][e], acc[0][j + 3][e]);
+      } else {
+        *reinterpret_cast<float2 *>(row) = make_float2(acc[0][0][e], acc[0][1][e]);
       }
+    }
     __syncthreads();
   } else if constexpr (BIG) {
     float fy[NB];
