@@ -260,3 +260,45 @@ def test_the_same_bits_every_time(rng):
     a = call(x, 40000, s, None, 8, 3)
     for _ in range(3):
         assert all(np.array_equal(u, v) for u, v in zip(a, call(x, 40000, s, None, 8, 3)))
+
+
+@pytest.mark.parametrize("B,W,V", [(70000, 1, 33), (20000, 2, 50), (1500, 32, 40)])
+def test_many_rows(rng, B, W, V):
+    """More rows than a grid's second dimension holds."""
+    x, s = random_rows(rng, B * W, V)
+    x = np.round(x * 4096).astype(np.float32) / 4096
+    total, end, tok, parent = call(x, V, s, None, W, -1)
+    for b in np.concatenate([[0, 1, B - 1], rng.integers(0, B, 40)]):
+        rows = slice(b * W, b * W + W)
+        w_tok, w_parent, w_total, _ = O.select(x[rows], s[rows], None, W, -1)
+        assert np.array_equal(tok[rows], w_tok) and np.array_equal(parent[rows], w_parent + b * W)
+        assert np.abs(total[rows] - w_total).max() < 1e-4
+
+
+def test_logits_past_32_bits():
+    """70 rows of 2^24 logits, 4.7 GB: all 0 but for a few, so that all others tie."""
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    W, B, V = 2, 35, 1 << 24
+    n = W * B
+    x = K.DeviceBuffer(4 * n * V)
+    ok(L.lb_memset_d(x.ptr, 0, x.nbytes))
+    ok(L.lb_dev_synchronize())
+    spikes = {(0, 5): 3.0, (0, V - 1): 2.0, (69, V - 1): 4.0, (69, V // 2 + 1): 9.0, (68, 0): 1.0, (40, 1 << 23): -1.0}
+    for (row, v), y in spikes.items():
+        a = np.array([y], np.float32)
+        ok(L.lb_memcpy_h2d(x.ptr + 4 * (row * V + v), a.ctypes.data, 4))
+    s = np.where(np.arange(n) % W == 0, 0.0, -1.0).astype(np.float32)
+    d = [up(s)] + [up(np.zeros(n, np.float32))] + [up(np.zeros(n, np.int32)) for _ in range(3)]
+    b = K.LbdBeams(d[0].ptr, None, d[1].ptr, d[2].ptr, d[3].ptr, d[4].ptr, None, None, None, 0, B, W, V, -1)
+    need = L.lbd_beam_select_work_bytes(C.byref(b))
+    ws = up(np.zeros(need, np.uint8))
+    ok(L.lbd_beam_select(x.ptr, V, C.byref(b), ws.ptr, need, None))
+    ok(L.lb_dev_synchronize())
+    tok, parent, total = d[3].to_array((n,), np.int32), d[4].to_array((n,), np.int32), d[1].to_array((n,), np.float32)
+    want = [[(2 * g, 0), (2 * g, 1)] for g in range(B)]  # the first beam's lowest tokens
+    want[0] = [(0, 5), (0, V - 1)]
+    want[34] = [(69, V // 2 + 1), (69, V - 1)]  # 9 and 4 below log 2^24 and a sum of -1, against 1
+    assert list(zip(parent, tok)) == [o for g in want for o in g]
+    lse = np.log(2.0 ** 24)
+    assert abs(total[2] + lse) < 2.0 ** -10  # 2^24 terms of 1: 65536 a thread and trees, exact
+    assert abs(total[0] - (3 - lse)) < 2.0 ** -10

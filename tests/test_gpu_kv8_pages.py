@@ -63,6 +63,80 @@ def test_many_copies(rng):
     L.check([(a, b, None) for a, b in zip(order[:1400], order[1400:2800])])
 
 
+def test_recorded_copies(rng):
+    """A replayed graph copies the pages that the arrays name by then; two graphs of other layers in turn."""
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    lays = [Layers(rng, n, 12, 16, 2, 32) for n in (2, 70)]
+    ds, dd, s = up(np.zeros(4, np.int32)), up(np.zeros(4, np.int32)), C.c_void_p()
+    ok(L.lb_stream_create(C.byref(s)))
+    graphs = []
+    for lay in lays:
+        ex = C.c_void_p()
+        ok(L.lb_stream_begin_capture(s.value))
+        rc = L.lbd_kv8_copy_pages(lay.pools, len(lay.host), ds.ptr, dd.ptr, 4, s.value)
+        ok(L.lb_stream_end_capture(s.value, C.byref(ex)))
+        ok(rc)
+        graphs.append(ex.value)
+    for _ in range(4):
+        order = rng.permutation(12).astype(np.int32)
+        ok(L.lb_memcpy_h2d(ds.ptr, order.ctypes.data, 16))
+        ok(L.lb_memcpy_h2d(dd.ptr, order[4:].copy().ctypes.data, 16))
+        for g in graphs:
+            ok(L.lb_graph_launch(g, s.value))
+        ok(L.lb_stream_synchronize(s.value))
+        for lay in lays:
+            lay.check([(a, b, None) for a, b in zip(order[:4], order[4:8])])
+    for g in graphs:
+        ok(L.lb_graph_destroy(g))
+    ok(L.lb_stream_destroy(s.value))
+
+
+def test_pools_past_32_bits():
+    """Pages 5 GB into a pool copied to its front and back, whole and by a beam's tokens."""
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    pages, page, KV, D = 40000, 128, 8, 128
+    one = KV * page * D
+    bufs = [K.DeviceBuffer(pages * one), K.DeviceBuffer(pages * one), K.DeviceBuffer(pages * KV), K.DeviceBuffer(pages * KV)]
+    for b in bufs:
+        ok(L.lb_memset_d(b.ptr, 7, b.nbytes))
+    ok(L.lb_dev_synchronize())
+    pool = (K.LbdKv8Pool * 1)(K.LbdKv8Pool(*(b.ptr for b in bufs), pages, page, KV, D))
+    rng = np.random.default_rng(0)
+    held = [rng.integers(0, 256, n, dtype=np.uint8) for n in (one, one, KV, KV)]
+    far = pages - 2
+
+    def put(p, what):
+        for b, h in zip(bufs, what):
+            ok(L.lb_memcpy_h2d(b.ptr + p * len(h), h.ctypes.data, len(h)))
+
+    def get(p):
+        out = [np.empty_like(h) for h in held]
+        for b, h in zip(bufs, out):
+            ok(L.lb_memcpy_d2h(h.ctypes.data, b.ptr + p * len(h), len(h)))
+        return out
+
+    put(far, held)
+    src, dst = up(np.array([far, far], np.int32)), up(np.array([3, pages - 1], np.int32))
+    ok(L.lbd_kv8_copy_pages(pool, 1, src.ptr, dst.ptr, 2, None))
+    ok(L.lb_dev_synchronize())
+    for p in (3, pages - 1, far):
+        assert all(np.array_equal(a, b) for a, b in zip(get(p), held))
+    assert all((x == 7).all() for p in (2, 4, pages - 3) for x in get(p))
+    # two children of a beam whose page lies far: 70 tokens of it into another far page
+    table, own = np.array([[far], [-1]], np.int32), np.array([[far], [pages - 5]], np.int32)
+    a = [up(x) for x in (np.zeros(2, np.int32), np.array([69, -1], np.int32), table, own)]
+    new_past, new_table = up(np.zeros(2, np.int32)), up(np.zeros((2, 1), np.int32))
+    o = K.LbdKv8Order(a[0].ptr, None, a[1].ptr, a[2].ptr, a[3].ptr, new_past.ptr, new_table.ptr, 1, 2, 1, 1)
+    ok(L.lbd_kv8_reorder(pool, 1, C.byref(o), None))
+    ok(L.lb_dev_synchronize())
+    assert list(new_table.to_array((2,), np.int32)) == [far, pages - 5]
+    got = get(pages - 5)
+    for x, h in zip(got[:2], held):
+        x, h = x.reshape(KV, page, D), h.reshape(KV, page, D)
+        assert np.array_equal(x[:, :70], h[:, :70]) and (x[:, 70:] == 7).all()
+    assert np.array_equal(got[2], held[2]) and np.array_equal(got[3], held[3])
+
+
 # ---------------------------------------------------------------- beams
 
 def family(rng, prompts, W, page, wide, lengths=None):

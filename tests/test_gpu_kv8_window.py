@@ -227,3 +227,47 @@ def test_a_recorded_call_takes_other_lengths(rng):
     for g in graphs:
         ok(L.lb_graph_destroy(g))
     ok(L.lb_stream_destroy(s.value))
+
+
+@pytest.mark.parametrize("seqs", [[(200, 1)], [(150, 60)], [(200, 1), (170, 40)]], ids=str)
+def test_far_positions(rng, seqs):
+    """Behind 2^30 - 2^12 positions in a table of 2^30 a window reads what it reads near the beginning, bit for bit."""
+    D, page, KV, H, far = 64, 128, 2, 4, (1 << 30) - (1 << 12)
+    pages, q_start, past, table, T = batch_of(rng, page, seqs, 1, 0)
+    pool = cached(rng, pages, page, KV, D, table, seqs)
+    q, most = rng.standard_normal((T, H * D)).astype(np.float32), max(n for _, n in seqs)
+    near = np.full((len(seqs), 32), -1, np.int32)
+    near[:, :table.shape[1]] = table
+    long = np.full((len(seqs), 1 << 23), -1, np.int32)
+    long[:, far // page:far // page + table.shape[1]] = table
+    for window in (1, 100, 128):  # (longer ones see positions that only one of the two has)
+        want = attend(Device(pool, q_start, past, near, most, T), q, H, H * D, window, 0)
+        got = attend(Device(pool, q_start, past + far, long, most, T), q, H, H * D, window, 0)
+        assert np.array_equal(got, want)
+        ref = np.full(got.shape, FILL, np.float64)
+        check(got, ref, pool.attention(q_start, past, near, most, q, H, ref, window, 0), D, H)
+
+
+def test_two_streams(rng):
+    """Two calls at once on two streams, with a workspace each."""
+    L, up = K.lib(), K.DeviceBuffer.from_array
+    D, page, KV, H = 128, 32, 2, 8
+    runs = []
+    for seqs, window in (([(3000, 1), (900, 1)], 2000), ([(40, 400)], 900)):
+        pages, q_start, past, table, T = batch_of(rng, page, seqs, 0, 0)
+        pool = cached(rng, pages, page, KV, D, table, seqs)
+        q, most = rng.standard_normal((T, H * D)).astype(np.float32), max(n for _, n in seqs)
+        dev, st = Device(pool, q_start, past, table, most, T), C.c_void_p()
+        ok(L.lb_stream_create(C.byref(st)))
+        need = L.lbd_kv8_attention_window_work_bytes(C.byref(dev.pool), C.byref(dev.batch), H, window, 4)
+        runs.append((dev, up(q), up(np.zeros_like(q)), up(np.zeros(need, np.uint8)), need, st, window,
+                     attend(dev, q, H, H * D, window, 4)))
+    ok(L.lb_dev_synchronize())
+    for _ in range(5):
+        for dev, dq, do, ws, need, st, window, _ in runs:
+            ok(L.lbd_kv8_attention_window(C.byref(dev.pool), C.byref(dev.batch), dq.ptr, H * D, H, window, 4, do.ptr,
+                                          H * D, ws.ptr, need, st.value))
+    ok(L.lb_dev_synchronize())
+    for dev, dq, do, ws, need, st, window, want in runs:
+        assert np.array_equal(do.to_array(want.shape, np.float32), want)
+        ok(L.lb_stream_destroy(st.value))
