@@ -118,8 +118,9 @@ __device__ __forceinline__ float beam_threshold(float v, int W) {
 
 // A workgroup a piece of `per` steps of a row. Every wave keeps the keys above its threshold in LDS: the first
 // step's, for all waves, is the W-th largest of 64 lanes' maxima (W of them at least reach it, and few more),
-// later ones come from sorting the kept keys out where they run out of room. So most chunks end after a
-// comparison of 16 logits' maximum.
+// later ones come from a chunk of many larger logits, and from sorting the kept keys out where they run out of
+// room. So most chunks end after a comparison of 16 logits' maximum. (128 rows of 151936: rising logits 26 us,
+// 367 without a threshold for them; all equal ones, where keys differ by their tokens only, 81.)
 //
 // What bounds it: 128 rows of 151936 logits the instructions, 17 us = 4.3 TB/s (of a wave's 530 vector
 // instructions 16 a chunk are exponentials and 48 their arguments and sum), and 2.4 steps a workgroup between its
@@ -136,13 +137,13 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
   const int over = a.done ? a.done[row] : 0;
   __shared__ unsigned long long keys[kBeamWaves][kBeamRoom], last[kBeamWaves * kBeamRoom];
   __shared__ __attribute__((aligned(16))) uint32_t high[kBeamWaves * kBeamRoom + 4];
-  __shared__ float tops[kBeamWaves][kWave], smax[kBeamWaves], ssum[kBeamWaves], sleast[kBeamWaves];
+  __shared__ float tops[kBeamWaves][kWave], smax[kBeamWaves], ssum[kBeamWaves], ssure[kBeamWaves];
   __shared__ int kept[kBeamWaves], count;
   const Rsrc x = make_rsrc(a.logits + (size_t)row * a.ld, 4u * (uint32_t)a.V);  // reads past the row give 0
   const int end = min(a.V, (at + 1) * per * kBeamStep);
   int v0 = at * per * kBeamStep + wave * kBeamChunk;
   unsigned long long *mine = keys[wave], low = 0;
-  float m = kBeamNone, sum = 0.0f, least;
+  float m = kBeamNone, sum = 0.0f, least, sure;
   int n = 0;
   const auto load = [&](float *f, int v) {
 #pragma unroll
@@ -171,9 +172,16 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
     for (int i = 0; i < N; i++) sum += exp_below(f[i] - m);
     return top;
   };
-  // the chunk's keys that reach the threshold
+  // the chunk's keys that reach the threshold `least`; W of the workgroup's reach `sure`
   const auto keep = [&](const float *f, const float *tops4, float top) {
-    if (!__any(top >= least)) return;
+    // (a logit equal to the W-th best so far comes after it, by its token)
+    if (low) least = fmaxf(least, offer_logit(((low >> 32) + 1) << 32));
+    const int hits = __popcll((unsigned long long)__ballot(top >= least));
+    if (!hits) return;
+    if (hits > W + 8) {  // rising logits
+      const float t = beam_threshold(top, W);
+      least = fmaxf(least, t), sure = fmaxf(sure, t);
+    }
 #pragma unroll
     for (int g = 0; g < kBeamLoads; g++) {
       if (!__any(tops4[g] >= least)) continue;
@@ -181,7 +189,7 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
         __builtin_amdgcn_wave_barrier();
         low = beam_sort((LdsKey *)mine, n, W);
         n = W;
-        least = offer_logit(low);
+        least = fmaxf(least, offer_logit(low)), sure = fmaxf(sure, offer_logit(low));
       }
 #pragma unroll
       for (int i = 4 * g; i < 4 * g + 4; i++) {
@@ -206,7 +214,7 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
   float first = tops[0][lane];
 #pragma unroll
   for (int w = 1; w < kBeamWaves; w++) first = fmaxf(first, tops[w][lane]);
-  least = beam_threshold(first, W);
+  least = sure = beam_threshold(first, W);
   if (v0 < end) keep(f0, t0, top0);
   for (v0 += kBeamStep; v0 < end; v0 += kBeamStep) {  // two chunks in turn, so that nothing is moved
     if (v0 + kBeamStep < end) load(f0, v0 + kBeamStep);
@@ -221,15 +229,15 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
   // ---- the waves' sums and keys
   const float all = wave_max(m);
   const float part = wave_sum(sum * exp_below(m - all));
-  if (lane == 0) smax[wave] = all, ssum[wave] = part, kept[wave] = n, sleast[wave] = least;
+  if (lane == 0) smax[wave] = all, ssum[wave] = part, kept[wave] = n, ssure[wave] = sure;
   __syncthreads();
   const size_t to = (size_t)row * pieces + at;
-  float top = smax[0], total = 0.0f, bar = sleast[0];
+  float top = smax[0], total = 0.0f, bar = ssure[0];
   int before[kBeamWaves + 1] = {0};
 #pragma unroll
   for (int w = 0; w < kBeamWaves; w++) {
     top = fmaxf(top, smax[w]);
-    bar = fmaxf(bar, sleast[w]);
+    bar = fmaxf(bar, ssure[w]);
     before[w + 1] = before[w] + kept[w];
   }
 #pragma unroll
