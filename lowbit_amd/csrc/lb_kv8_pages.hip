@@ -152,11 +152,11 @@ hipError_t launch_kv8_copy_pages(const Kv8Layers &l, const int32_t *src, const i
 hipError_t launch_kv8_reorder(const Kv8Layers &l, const Kv8Order &o, bool write, hipStream_t s) {
   const int parts = copy_parts(l);
   const long long places = (long long)o.B * o.W, copies = 2 * places * parts, grid = copies + (write ? places : 0);
-  // Workgroups in all, ten or four a CU, so that a place's move is found for several layers where there are many.
-  // Pages of 128 KB: 40 places in 32 layers 13.0 us with four rows of workgroups, 14.0 with seven, 21.8 with one a
+  // Workgroups in all, so that a place's move is found for several layers where there are many. Pages of 128 KB:
+  // 40 places in 32 layers 13.6 us with four rows of workgroups, 13.2 with five, 14.0 with seven, 21.8 with one a
   // layer; 128 places 70 with one row, 56 with two, 87 with one a layer. Of 8 KB, whose parts leave lanes idle:
   // 32 places in 24 layers 5.1 us with 1024 in all, 6.2 with 2048.
-  const long long want = ((long long)l.KV << (l.page_shift + l.d_shift)) < kCopyBytes ? 1024 : 2560;
+  const long long want = ((long long)l.KV << (l.page_shift + l.d_shift)) < kCopyBytes ? 1024 : 3200;
   const int rows = (int)std::min<long long>(l.n, std::max<long long>(1, (want + copies - 1) / copies));
   if (!fits(grid, rows)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kv8_reorder_kernel, dim3((unsigned)grid, rows), dim3(256), 0, s, l, o, (int)copies, parts, rows);
