@@ -253,14 +253,14 @@ class KV8Cache:
 
     def _drop(self, seq: int, first: int, last: int):
         """Sequence `seq` no longer holds its pages first .. last - 1."""
-        gone = self._table[seq, first:last]
+        part = self._table[seq, first:last]
+        gone = part[part >= 0]
         for p in gone[::-1]:
-            if p >= 0:
-                self._refs[p] -= 1
-                if not self._refs[p]:
-                    self._free.append(int(p))
+            self._refs[p] -= 1
+            if not self._refs[p]:
+                self._free.append(int(p))
         if len(gone):
-            gone[:] = -1
+            part[:] = -1
             self._dirty = True
 
     def _take(self) -> int:
@@ -312,8 +312,8 @@ class KV8Cache:
         if not self.window:
             return
         a, b = -(-self.sinks // self.page), max(int(self.lengths[seq]) - self.window + 1, 0) // self.page
-        if b > a:
-            self._drop(seq, a, b)
+        if b > max(a, self._hole[seq, 1]):  # what was given back before is not looked at again
+            self._drop(seq, max(a, int(self._hole[seq, 1])), b)
             self._hole[seq] = a, b
 
     def compact(self) -> int:

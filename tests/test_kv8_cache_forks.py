@@ -216,3 +216,32 @@ def test_a_window_takes_the_8_bit_cache():
     for bad in (dict(window=-1), dict(window=4, sinks=-1), dict(sinks=3)):
         with pytest.raises(ValueError):
             M.Model(M.tiny_config(**bad), {})
+
+
+@pytest.mark.parametrize("sinks", [0, 4, 40])
+def test_a_step_gives_back_only_what_it_left_behind(new, sinks):
+    """Behind the window a step looks at no page that has been given back, and a step that gives none back
+    leaves the table as the device has it."""
+    cache = new(4000, page=16, sequences=2, pages=40, window=50, sinks=sinks)
+    walked, drop = [], cache._drop
+    cache._drop = lambda seq, first, last: (walked.append(last - first), drop(seq, first, last))
+    for t in range(1500):
+        held = cache._table.copy()
+        for s in (0, 1):
+            at = int(cache.lengths[s])
+            cache.reserve(s, at + 1)
+        cache.upload()
+        assert not cache._dirty
+        for s in (0, 1):
+            cache.lengths[s] += 1
+            cache.slide(s)
+        assert cache._dirty == ((held >= 0) & (cache._table < 0)).any()
+        consistent(cache)
+    assert max(walked) == 1 and len(walked) <= 2 * (1500 // 16)
+    # cut down to the sinks the hole is gone, and grows anew
+    left = min(sinks, 3)
+    cache.truncate(0, left)
+    assert not cache._hole[0].any()
+    write(cache, 0, [7] * 200)
+    consistent(cache)
+    assert cache._hole[0, 1] == (200 + left - 50 + 1) // 16
