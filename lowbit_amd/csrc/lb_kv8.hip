@@ -605,7 +605,8 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
   const int k_begin = w.slice * w.slice_keys;
   const int k_end = min(min(w.s.past + tok_last + 1, cap) - gap, k_begin + w.slice_keys);
   const int k_full = min(w.s.past + tok_first + 1, cap) - gap;  // keys below: every row sees them
-  // (a window: those below the sinks and from here on)
+  // (a window: those below the sinks and from k_low on; positions from the sinks to `begin` no row sees)
+  const int begin = WIN ? w.s.past + tok_first + 1 - a.window : 0;
   const int k_low = WIN && w.s.past + tok_last + 1 - a.window > a.sinks ? w.s.past + tok_last + 1 - a.window - gap : 0;
   const int chunks = max(0, (k_end - k_begin - CK * wave + CK * NW - 1) / (CK * NW));
   const int32_t *table = a.table + (size_t)w.s.b * a.max_pages;
@@ -851,7 +852,12 @@ __device__ __forceinline__ void kv8_attend(const Kv8Args &a, const Kv8Part &pt, 
               s[y][x][e] = key < lim[y] && now[x].held ? s[y][x][e] : -INFINITY;
             }
           }
-          if (key >= k_end || now[x].unused) vf[x][e] = make_uint2(0, 0);
+          bool none = key >= k_end || now[x].unused;
+          if constexpr (WIN) {
+            const int at = key + (key0 + 16 * x < sinks ? 0 : gap);
+            none = none | ((at < begin) & (at >= a.sinks));
+          }
+          if (none) vf[x][e] = make_uint2(0, 0);
         }
     }
     constexpr int NT = SEP ? 3 : 2;  // matrix instructions for a weight's terms

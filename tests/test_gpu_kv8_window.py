@@ -271,3 +271,37 @@ def test_two_streams(rng):
     for dev, dq, do, ws, need, st, window, want in runs:
         assert np.array_equal(do.to_array(want.shape, np.float32), want)
         ok(L.lb_stream_destroy(st.value))
+
+
+@pytest.mark.parametrize("D,page,KV,H,seqs,window,sinks", [
+    # row blocks of 8 and of 16, in one slice and in many, the window's first position anywhere in a tile
+    (64, 16, 2, 14, [(150, 1), (151, 1), (165, 1)], 39, 5), (64, 64, 2, 14, [(9000, 1), (80, 1)], 4001, 7),
+    (128, 128, 1, 4, [(700, 1), (90, 2), (33, 1)], 50, 21), (32, 32, 3, 3, [(200, 2), (71, 1)], 17, 0),
+    (128, 64, 1, 16, [(500, 1), (333, 1)], 101, 3), (64, 16, 1, 9, [(3000, 1)], 2900, 1),
+    # row blocks of 32, whole and in slices
+    (64, 32, 2, 14, [(150, 60)], 39, 5), (128, 64, 1, 5, [(1000, 300)], 333, 21), (32, 128, 1, 1, [(77, 400)], 21, 3),
+    (128, 16, 1, 16, [(6000, 90)], 3001, 9),
+    # of two waves, alone and beside steps
+    (64, 64, 8, 32, [(333, 1100)], 100, 5), (32, 32, 8, 64, [(90, 800), (701, 1), (50, 90), (300, 3)], 201, 3),
+    (128, 64, 8, 32, [(61, 790), (900, 1)], 33, 9)], ids=str)
+def test_slots_that_no_token_sees_may_hold_anything(rng, D, page, KV, H, seqs, window, sinks):
+    """NaN codes in the slots of partly visible pages that lie before the first token's window, behind the
+    sinks or behind the last token reach no row."""
+    pages, q_start, past, table, T = batch_of(rng, page, seqs, 2, 0)
+    pool = cached(rng, pages, page, KV, D, table, seqs)
+    table = give_back(table, page, seqs, window, sinks)
+    q = (rng.standard_normal((T, H * D)) * 1.5).astype(np.float32)
+    most = max(n for _, n in seqs)
+    ref = np.full(q.shape, FILL, np.float64)
+    mags = pool.attention(q_start, past, table, most, q, H, ref, window, sinks)
+    held, hidden = pool.copy(), 0
+    for b, (p, n) in enumerate(seqs):
+        for x in range(table.shape[1] * page):
+            pg = table[b, x // page]
+            if pg >= 0 and not (x < p + n and (x >= p + 1 - window or x < sinks)):
+                hidden += x < p + n
+                held.k[pg, :, x % page] = 0xFF if x & 1 else 0x7F
+                held.v[pg, :, x % page] = 0x7F if x & 1 else 0xFF
+    assert hidden
+    got = attend(Device(held, q_start, past, table, most, T), q, H, H * D, window, sinks)
+    check(got, ref, mags, D, H)
