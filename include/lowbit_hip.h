@@ -568,11 +568,14 @@ typedef struct {
 /* new_table and new_past of every place, and in each of the n_pools pools the copies that they
  * call for. A sequence shares its parent's full pages. The page that is being written (past + add
  * not a multiple of the page) stays with the first place that continues the parent; for each
- * other one its tokens are copied, slots behind them left as they are, into a page that no
- * first place keeps: of own[i][that index], i the prompt's places in order, the next one. Pages
- * behind it are own's of the place itself. Places without a sequence get entries of -1. So with
- * own's pages all different, and a prompt's first page in writing among them, every sequence
- * writes to pages of its own, however parents change. pools as for lbd_kv8_copy_pages. */
+ * other one its tokens are copied, slots behind them left as they are, into another page. That
+ * page and those behind the one being written are, at each index j of the table, own[i][j] of the
+ * place i itself where no sequence of the prompt holds a page there, and else, for the places
+ * that hold none in order, the pages own[.][j] of the prompt that none holds, in order. Places
+ * without a sequence get entries of -1. So with own's pages all different and in no other prompt's
+ * tables, and from the page in writing on those that the prompt's tables hold among them, every
+ * sequence writes to pages of its own, however parents change and whatever the sequences'
+ * lengths. pools as for lbd_kv8_copy_pages. */
 int lbd_kv8_reorder(const lbd_kv8_pool *pools, int n_pools, const lbd_kv8_order *order,
                     void *stream);
 

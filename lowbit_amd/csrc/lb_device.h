@@ -63,6 +63,16 @@ __device__ __forceinline__ float wave_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+__device__ __forceinline__ int wave_max_i32(int v) {
+  v = max(v, dpp_i<kDppQuad1032>(v, v));
+  v = max(v, dpp_i<kDppQuad2301>(v, v));
+  v = max(v, dpp_i<kDppRowHalfMirror>(v, v));
+  v = max(v, dpp_i<kDppRowMirror>(v, v));
+  v = max(v, dpp_i<kDppRowBcast15, 0xA>(v, v));
+  v = max(v, dpp_i<kDppRowBcast31, 0xC>(v, v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 // Lane `lane` (wave-uniform) of v takes the wave-uniform value `bits`; the other
 // lanes keep theirs: v_writelane_b32 through LLVM's intrinsic, which clang exposes
 // as no builtin. The compiler then sets M0 for the lane select itself (gfx9 reads

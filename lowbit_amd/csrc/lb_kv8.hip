@@ -32,16 +32,6 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-__device__ __forceinline__ int wave_max_i32(int v) {
-  v = max(v, dpp_i<kDppQuad1032>(v, v));
-  v = max(v, dpp_i<kDppQuad2301>(v, v));
-  v = max(v, dpp_i<kDppRowHalfMirror>(v, v));
-  v = max(v, dpp_i<kDppRowMirror>(v, v));
-  v = max(v, dpp_i<kDppRowBcast15, 0xA>(v, v));
-  v = max(v, dpp_i<kDppRowBcast31, 0xC>(v, v));
-  return __builtin_amdgcn_readlane(v, 63);
-}
-
 // One sequence's new tokens: rows row0 .. row0 + n - 1 at positions past ..
 struct Kv8Seq {
   int b, row0, n, past;

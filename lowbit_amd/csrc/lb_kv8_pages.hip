@@ -34,49 +34,68 @@ __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Layers l, const int32_
 
 // ---------------------------------------------------------------- beams in their new order
 
-// What becomes of one place, the same in every lane of a wave.
-struct Kv8Move {
-  int parent, length;  // the place that it continues and the tokens that it holds; parent -1: no sequence
-  int tail, used;      // index of the page that is being written, and its tokens (0: it is begun next)
-  int from, page;      // that page: the parent's and the place's (the parent's own: no copy)
+// The places of a prompt, one a lane: what each continues (parent -1: no sequence) and the tokens that it holds;
+// the index of the page that is being written, its tokens (0: it is begun next) and the parent's page there, which
+// the first of a parent's children keeps.
+struct Kv8Family {
+  int parent, length, tail, used, was;
+  bool first;
 };
 
-// The move of place `place`, by the whole wave: lane k looks at place k of the prompt.
-__device__ __forceinline__ Kv8Move kv8_move(const Kv8Order &o, int page_shift, int pages, int place) {
-  const int lane = threadIdx.x & (kWave - 1), base = place / o.W * o.W, me = place - base, cap = o.max_pages << page_shift;
-  int parent = -1, length = 0, was = -1;
+__device__ __forceinline__ Kv8Family kv8_family(const Kv8Order &o, int page_shift, int base) {
+  const int lane = threadIdx.x & (kWave - 1), cap = o.max_pages << page_shift;
+  Kv8Family f = {-1, 0, 0, 0, -1, false};
   if (lane < o.W) {
     const int p = o.parent[base + lane];
     if (p >= base && p < base + o.W && !(o.done && o.done[base + lane])) {
       const int past = o.past[p];
-      if (past >= 0) parent = p, length = (int)min((long long)past + o.add, (long long)kKv8MaxPos);
+      if (past >= 0) f.parent = p, f.length = (int)min((long long)past + o.add, (long long)kKv8MaxPos);
     }
   }
-  const int tail = min(length, cap) >> page_shift, used = length < cap ? length & ((1 << page_shift) - 1) : 0;
-  const bool copied = parent >= 0 && used;
-  if (copied) was = o.table[(size_t)parent * o.max_pages + tail];
-  // the first place of those that continue a parent keeps its page
-  const unsigned long long holds = __ballot(copied);
-  bool first = copied;
+  f.tail = min(f.length, cap) >> page_shift, f.used = f.length < cap ? f.length & ((1 << page_shift) - 1) : 0;
+  f.first = f.parent >= 0 && f.used;
+  if (f.first) f.was = o.table[(size_t)f.parent * o.max_pages + f.tail];
+  const unsigned long long writes = __ballot(f.first);
   for (int k = 0; k < o.W; k++) {
-    const int theirs = __builtin_amdgcn_readlane(parent, k);
-    if ((holds >> k & 1) && k < lane && theirs == parent) first = false;
+    const int theirs = __builtin_amdgcn_readlane(f.parent, k);
+    if ((writes >> k & 1) && k < lane && theirs == f.parent) f.first = false;
   }
-  const unsigned long long keep = __ballot(first);
-  const auto mine = [&](int v) { return __builtin_amdgcn_readlane(v, me); };
-  Kv8Move m = {mine(parent), mine(length), mine(tail), mine(used), mine(was), mine(was)};
-  if (!(holds >> me & 1) || (keep >> me & 1)) return m;
-  // the others take the pages that no first place keeps, in order
-  const int spare = lane < o.W ? o.own[(size_t)(base + lane) * o.max_pages + m.tail] : -1;
+  return f;
+}
+
+// The page that place base + me, whose sequence holds none at index j, gets there, by the whole wave: its own
+// where no sequence of the prompt holds one, else of own's pages that none holds, in order, the next one. (There
+// are W of them, and a place holds one or gets one, so they suffice whatever the sequences' lengths.)
+__device__ __forceinline__ int kv8_page_at(const Kv8Order &o, const Kv8Family &f, int pages, int base, int me, int j) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const bool holds = f.parent >= 0 && (f.tail > j || (f.tail == j && f.first));
+  const int spare = lane < o.W ? o.own[(size_t)(base + lane) * o.max_pages + j] : -1;
+  const unsigned long long held = __ballot(holds);
+  if (!held) return __builtin_amdgcn_readlane(spare, me);
+  int page = f.was;
+  if (holds && f.tail > j) page = o.table[(size_t)f.parent * o.max_pages + j];
   bool free = (unsigned)spare < (unsigned)pages;
   for (int k = 0; k < o.W; k++) {
-    const int kept = __builtin_amdgcn_readlane(was, k);
-    if ((keep >> k & 1) && kept == spare) free = false;
+    const int kept = __builtin_amdgcn_readlane(page, k);
+    if ((held >> k & 1) && kept == spare) free = false;
   }
   unsigned long long left = __ballot(free);
-  for (unsigned long long before = __ballot(copied && !first && tail == m.tail && lane < me); before; before &= before - 1)
+  for (unsigned long long before = __ballot(f.parent >= 0 && !holds && lane < me); before; before &= before - 1)
     left &= left - 1;
-  m.page = left ? __builtin_amdgcn_readlane(spare, __ffsll(left) - 1) : -1;
+  return left ? __builtin_amdgcn_readlane(spare, __ffsll(left) - 1) : -1;
+}
+
+// What becomes of one place, the same in every lane of a wave.
+struct Kv8Move {
+  int parent, length, tail, used;  // as above
+  int from, page;                  // the page in writing: the parent's and the place's (the parent's own: no copy)
+};
+
+// The move of place base + me, by the whole wave.
+__device__ __forceinline__ Kv8Move kv8_move(const Kv8Order &o, const Kv8Family &f, int pages, int base, int me) {
+  const auto mine = [&](int v) { return __builtin_amdgcn_readlane(v, me); };
+  Kv8Move m = {mine(f.parent), mine(f.length), mine(f.tail), mine(f.used), mine(f.was), mine(f.was)};
+  if (m.parent >= 0 && m.used && !mine(f.first)) m.page = kv8_page_at(o, f, pages, base, me, m.tail);
   return m;
 }
 
@@ -88,10 +107,19 @@ __global__ __launch_bounds__(256) void kv8_reorder_kernel(Kv8Layers l, Kv8Order 
   const int tid = threadIdx.x, id = (int)blockIdx.x;
   if (id >= copies) {  // a place's row of the table
     if (blockIdx.y) return;
-    const int place = id - copies;
-    const Kv8Move m = kv8_move(o, l.page_shift, l.pages, place);
+    const int place = id - copies, base = place / o.W * o.W;
+    const Kv8Family f = kv8_family(o, l.page_shift, base);
+    const Kv8Move m = kv8_move(o, f, l.pages, base, place - base);
     const size_t row = (size_t)place * o.max_pages;
+    // up to here other sequences of the prompt, longer ones, hold pages
+    const int last = m.parent >= 0 ? wave_max_i32(f.parent < 0 ? -1 : f.first ? f.tail : f.tail - 1) : -1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), next = m.used ? m.tail + 1 : m.tail;
+    for (int j = next + wave; j <= last; j += 256 / kWave) {
+      const int p = kv8_page_at(o, f, l.pages, base, place - base, j);
+      if (tid % kWave == 0) o.new_table[row + j] = p;
+    }
     for (int j = tid; j < o.max_pages; j += 256) {
+      if (j >= next && j <= last) continue;
       int p = -1;
       if (m.parent >= 0) {
         p = j < m.tail ? o.table[(size_t)m.parent * o.max_pages + j] : o.own[row + j];
@@ -105,7 +133,8 @@ __global__ __launch_bounds__(256) void kv8_reorder_kernel(Kv8Layers l, Kv8Order 
   const int place = id / (2 * parts), rest = id % (2 * parts);
   const bool isv = rest >= parts;
   const int part = isv ? rest - parts : rest;
-  const Kv8Move m = kv8_move(o, l.page_shift, l.pages, place);
+  const int base = place / o.W * o.W;
+  const Kv8Move m = kv8_move(o, kv8_family(o, l.page_shift, base), l.pages, base, place - base);
   if (m.parent < 0 || !m.used || m.page == m.from) return;
   if ((unsigned)m.page >= (unsigned)l.pages || (unsigned)m.from >= (unsigned)l.pages) return;
   const size_t bytes = (size_t)l.KV << (l.page_shift + l.d_shift);

@@ -58,24 +58,27 @@ def reorder(parent, done, past, table, own, beams, add, page, pages):
         for i, p in goes.items():
             if used[i]:
                 heir.setdefault(p, i)
-        kept = {int(table[p, tail[i]]) for p, i in heir.items()}
-        taken = {}
+
+        def holds(i, j):
+            return tail[i] > j or (tail[i] == j and used[i] > 0 and heir[goes[i]] == i)
+
+        def page_at(i, j):
+            """Of a place that holds none at index j."""
+            held = {int(table[goes[k], j]) for k in goes if holds(k, j)}
+            if not any(holds(k, j) for k in goes):
+                return int(own[i, j])
+            free = [int(own[k, j]) for k in here if 0 <= own[k, j] < pages and own[k, j] not in held]
+            n = sum(k < i and not holds(k, j) for k in goes)
+            return free[n] if n < len(free) else -1
+
         for i, p in goes.items():
             new_past[i] = length[i]
-            new_table[i, :tail[i]] = table[p, :tail[i]]
-            new_table[i, tail[i]:] = own[i, tail[i]:]
-            if not used[i]:
-                continue
-            if heir[p] == i:
-                new_table[i, tail[i]] = table[p, tail[i]]
-                continue
-            free = [int(own[j, tail[i]]) for j in here if 0 <= own[j, tail[i]] < pages and own[j, tail[i]] not in kept]
-            n = taken.get(tail[i], 0)
-            taken[tail[i]] = n + 1
-            to = free[n] if n < len(free) else -1
-            new_table[i, tail[i]] = to
-            if to >= 0 and 0 <= table[p, tail[i]] < pages:
-                moves.append((int(table[p, tail[i]]), to, used[i]))
+            for j in range(wide):
+                new_table[i, j] = table[p, j] if holds(i, j) else page_at(i, j)
+            if used[i] and heir[p] != i:
+                a, b = int(table[p, tail[i]]), int(new_table[i, tail[i]])
+                if b >= 0 and 0 <= a < pages:
+                    moves.append((a, b, used[i]))
     return new_past, new_table, moves
 
 

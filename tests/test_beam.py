@@ -135,3 +135,57 @@ def test_oracle_reorders():
     assert list(past) == [21] * 3 and new.tolist() == [[7, 1], [7, 0], [7, 2]] and moves == [(1, 0, 5)]
     _, new, moves = O.reorder(np.array([1, 1, 2]), None, np.array([15, 15, 15]), table, own, 3, 1, 16, 8)
     assert new.tolist() == [[7, 0], [7, 1], [7, 2]] and not moves
+
+
+def written_once(new_past, new_table, moves, page):
+    """No page that a step writes belongs to a second sequence: destinations of the copies, and the pages that
+    the next tokens go to."""
+    places, wide = new_table.shape
+    to = [b for _, b, _ in moves]
+    assert len(set(to)) == len(to) and not set(to) & {a for a, _, _ in moves}
+    live = [i for i in range(places) if new_past[i] >= 0]
+    full = {i: {int(new_table[i, j]) for j in range(new_past[i] // page)} for i in live}
+    for i in live:
+        for j in range(new_past[i] // page, wide):
+            p = int(new_table[i, j])
+            assert p >= 0
+            for k in live:
+                assert k == i or (p not in full[k] and p not in new_table[k, new_past[k] // page:])
+
+
+@pytest.mark.parametrize("W", [2, 3, 4, 7])
+def test_oracle_reorders_other_lengths(W):
+    """Over many steps of sequences of other lengths every sequence keeps its own tokens, and no page that is
+    written has two owners. Places that go without a sequence for a while come back as children."""
+    rng = np.random.default_rng(W)
+    page, wide, G = 16, 6, 2
+    places, pages = G * W, G * W * wide
+    for trial in range(30):
+        own = rng.permutation(pages).reshape(places, wide)
+        table, past = own.copy(), rng.integers(0, 40, places)
+        held = np.full((pages, page), -1)  # the token in each slot
+        hist, tick = [[] for _ in range(places)], 0
+        for i in range(places):
+            for x in range(past[i]):
+                held[table[i, x // page], x % page] = tick
+                hist[i].append(tick)
+                tick += 1
+        for _ in range(25):
+            add = int(rng.integers(0, 4))
+            for i in range(places):  # the pass appends
+                for x in range(past[i], past[i] + add) if past[i] >= 0 else ():
+                    held[table[i, x // page], x % page] = tick
+                    hist[i].append(tick)
+                    tick += 1
+            parent = np.arange(places) // W * W + rng.integers(0, W, places)
+            done = rng.random(places) < 0.1
+            past, new_table, moves = O.reorder(parent, done, past, table, own, W, add, page, pages)
+            written_once(past, new_table, moves, page)
+            before = held.copy()
+            for a, b, n in moves:
+                held[b, :n] = before[a, :n]
+            table, hist = new_table, [list(hist[p]) if past[i] >= 0 else [] for i, p in enumerate(parent)]
+            for i in range(places):
+                assert [held[table[i, x // page], x % page] for x in range(past[i])] == hist[i]
+            if past.max() + 4 > wide * page:
+                break

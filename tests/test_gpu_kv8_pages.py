@@ -9,6 +9,7 @@ from lowbit_amd import kernels as K
 from oracle import beams as B
 from oracle import kv_cache as O
 from test_gpu_kv8 import ok
+from test_beam import written_once
 from test_gpu_kv8_guards import Guarded
 
 pytestmark = pytest.mark.gpu
@@ -314,3 +315,27 @@ def test_recorded(rng):
         lay.check([])
     ok(L.lb_graph_destroy(ex.value))
     ok(L.lb_stream_destroy(s.value))
+
+
+@pytest.mark.parametrize("prompts,W,page,wide,layers,KV,D", [
+    (1, 2, 16, 4, 1, 1, 32), (3, 4, 16, 7, 2, 2, 64), (2, 7, 32, 5, 3, 1, 32), (1, 32, 16, 12, 1, 1, 32),
+    (2, 5, 128, 3, 2, 8, 128), (4, 3, 16, 40, 1, 1, 32)])
+def test_lengths_of_any_kind(rng, prompts, W, page, wide, layers, KV, D):
+    """Sequences of other lengths within a prompt, over several steps from any state that a step leaves: no
+    page that is written has a second owner, and the pools are the oracle's."""
+    places, top = prompts * W, wide * page
+    pages = places * wide + 3
+    own = rng.permutation(pages)[:places * wide].reshape(places, wide).astype(np.int32)
+    for kind in ("near", "far", "ended", "full"):
+        table = own.copy()
+        past = rng.integers(0, top - 2, places) if kind != "near" else rng.integers(0, 2 * page, places)
+        if kind == "full":
+            past = past // page * page
+        for add in (1, 0, 3):
+            parent = np.arange(places) // W * W + rng.integers(0, W, places)
+            done = (rng.random(places) < 0.3).astype(int) if kind == "ended" else None
+            if kind == "far":
+                parent[rng.random(places) < 0.2] = -1
+            past, table, moves = run(rng, prompts, W, page, wide, layers, KV, D, parent, done, add,
+                                     state=(pages, past.astype(np.int32), table.astype(np.int32), own))
+            written_once(past, table, moves, page)
