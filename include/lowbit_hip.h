@@ -517,7 +517,8 @@ int lbd_kv8_attention_window(const lbd_kv8_pool *pool, const lbd_kv8_batch *batc
  * memory, so that a recorded graph replays with other pages; a pair with an entry outside
  * [0, pages) is skipped. No page may be dst twice, nor dst of one pair and src of another (in
  * such a pair what the page holds is not defined); src may repeat. `pools` is host memory, read
- * before the call returns. n == 0 does nothing. */
+ * before the call returns. n == 0 does nothing. n at most 2^24, and n times the 16 KB (begun) of a
+ * page's K codes in 64 layers (or n_pools, if fewer) at most 2^31: more than a card holds. */
 int lbd_kv8_copy_pages(const lbd_kv8_pool *pools, int n_pools, const int32_t *src,
                        const int32_t *dst, int n, void *stream);
 

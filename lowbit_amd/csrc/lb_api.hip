@@ -1665,7 +1665,7 @@ int lbd_kv8_copy_pages(const lbd_kv8_pool *pools, int n_pools, const int32_t *sr
   for (int first = 0; n && first < n_pools; first += l.n) {
     if (first && (rc = kv8_layers(pools, n_pools, first, l)) < 0) return rc;
     const hipError_t e = lbk::launch_kv8_copy_pages(l, src, dst, n, static_cast<hipStream_t>(stream));
-    if (e == hipErrorInvalidValue) return fail(LB_ERR_SHAPE, "too many pages for a launch");
+    if (e == hipErrorInvalidValue) return fail(LB_ERR_SHAPE, "bad shape: more pages than a device holds");
     if (e != hipSuccess) return fail_hip(e, "kv8 page copy launch");
   }
   return ok(0);

@@ -10,6 +10,8 @@
 namespace lbk {
 
 constexpr int kCopyBytes = 1 << 14;  // of a page's K or V codes that a workgroup copies at a time
+constexpr long long kCopyGroups = 1ll << 32;  // workgroups of a call and 64 layers: pages of 1 KB and more that
+                                              // fill the card, at most 2^24 of them, take fewer
 
 // ---------------------------------------------------------------- copies of pages
 
@@ -172,9 +174,12 @@ static bool fits(long long blocks, int layers) { return blocks * layers <= 0xFFF
 
 hipError_t launch_kv8_copy_pages(const Kv8Layers &l, const int32_t *src, const int32_t *dst, int n, hipStream_t s) {
   const int parts = copy_parts(l);
-  const long long grid = 2ll * n * parts;
-  if (!fits(grid, l.n)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kv8_copy_kernel, dim3((unsigned)grid, l.n), dim3(256), 0, s, l, src, dst, parts);
+  if (2ll * n * parts * l.n > kCopyGroups) return hipErrorInvalidValue;
+  const int most = (int)(0xFFFFFFFFll / 256 / l.n / (2 * parts));  // pairs of a launch
+  for (int at = 0; at < n; at += most) {
+    const int pairs = std::min(n - at, most);
+    hipLaunchKernelGGL(kv8_copy_kernel, dim3(2 * pairs * parts, l.n), dim3(256), 0, s, l, src + at, dst + at, parts);
+  }
   return hipGetLastError();
 }
 

@@ -357,10 +357,12 @@ class KV8Cache:
 
     def _copy(self, pairs: list, stream):
         """Pages copied in every layer, on `stream`."""
-        a = [K.DeviceBuffer.from_array(np.array(x, np.int32)) for x in zip(*pairs)]
-        _check(K.lib().lbd_kv8_copy_pages(self.pools, len(self.layers), a[0].ptr, a[1].ptr, len(pairs), stream),
-               "page copies")
-        self._moved = a  # alive until the next ones
+        most, self._moved = 1 << 24, []  # pairs of a call; their arrays live until the next copies
+        for at in range(0, len(pairs), most):
+            a = [K.DeviceBuffer.from_array(np.array(x, np.int32)) for x in zip(*pairs[at:at + most])]
+            self._moved.append(a)
+            _check(K.lib().lbd_kv8_copy_pages(self.pools, len(self.layers), a[0].ptr, a[1].ptr,
+                                              min(most, len(pairs) - at), stream), "page copies")
 
     def upload(self, stream=None):
         """The page table to the device, where it changed, and the copies that forks called for."""

@@ -64,6 +64,24 @@ def test_many_copies(rng):
     L.check([(a, b, None) for a, b in zip(order[:1400], order[1400:2800])])
 
 
+@pytest.mark.parametrize("n,layers,page,KV,D", [(9 << 20, 1, 16, 1, 32), (1 << 21, 5, 16, 1, 32), (70000, 64, 128, 2, 128)])
+def test_more_copies_than_a_launch_holds(rng, n, layers, page, KV, D):
+    """Calls of more than 2^24 workgroups: pairs at their beginning and end and around the launches' ends, all
+    others skipped."""
+    pages, up = 40, K.DeviceBuffer.from_array
+    L = Layers(rng, layers, pages, page, KV, D)
+    parts = -(-KV * page * D // (1 << 14))
+    most = (2 ** 32 - 1) // 256 // layers // (2 * parts)
+    assert 2 * n * parts * layers >= 1 << 24 and most < n
+    src, dst, order = np.full(n, -1, np.int32), np.full(n, 3, np.int32), rng.permutation(pages)
+    at = [0, 1, most - 1, most, most + 1, n - 2, n - 1]
+    src[at], dst[at] = order[:7], order[7:14]
+    ds, dd = up(src), up(dst)
+    ok(K.lib().lbd_kv8_copy_pages(L.pools, layers, ds.ptr, dd.ptr, n, None))
+    ok(K.lib().lb_dev_synchronize())
+    L.check([(a, b, None) for a, b in zip(order[:7], order[7:14])])
+
+
 def test_recorded_copies(rng):
     """A replayed graph copies the pages that the arrays name by then; two graphs of other layers in turn."""
     L, up = K.lib(), K.DeviceBuffer.from_array

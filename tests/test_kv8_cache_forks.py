@@ -245,3 +245,23 @@ def test_a_step_gives_back_only_what_it_left_behind(new, sinks):
     write(cache, 0, [7] * 200)
     consistent(cache)
     assert cache._hole[0, 1] == (200 + left - 50 + 1) // 16
+
+
+def test_many_copies_in_several_calls(new, monkeypatch):
+    """A call takes 2^24 pairs; more of them are cut."""
+    cache, calls = new(64, page=16), []
+    del cache._copy  # the method itself
+    monkeypatch.setattr(Lib, "__getattr__", lambda self, name: lambda *a: calls.append(a[4]) or 0)
+    monkeypatch.setattr(K.DeviceBuffer, "from_array", classmethod(lambda cls, a: Buffer(a.nbytes)))
+    cache._copy([(0, 1)] * 5, None)
+    assert calls == [5]
+
+    class Pairs:  # as long as a pool of small pages may be, without its memory
+        def __len__(self):
+            return (1 << 25) + 3
+
+        def __getitem__(self, part):
+            return [(part.start, 0)]
+
+    cache._copy(Pairs(), None)
+    assert calls[1:] == [1 << 24, 1 << 24, 3]
