@@ -576,7 +576,8 @@ typedef struct {
  * without a sequence get entries of -1. So with own's pages all different and in no other prompt's
  * tables, and from the page in writing on those that the prompt's tables hold among them, every
  * sequence writes to pages of its own, however parents change and whatever the sequences'
- * lengths. pools as for lbd_kv8_copy_pages. */
+ * lengths. pools as for lbd_kv8_copy_pages; B W times one more than twice the 16 KB (begun) of a
+ * page's K codes (KV page D bytes) below 2^24. */
 int lbd_kv8_reorder(const lbd_kv8_pool *pools, int n_pools, const lbd_kv8_order *order,
                     void *stream);
 

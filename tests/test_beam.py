@@ -189,3 +189,8 @@ def test_oracle_reorders_other_lengths(W):
                 assert [held[table[i, x // page], x % page] for x in range(past[i])] == hist[i]
             if past.max() + 4 > wide * page:
                 break
+
+
+def test_reorder_bounds_its_places():
+    """B W (2 x a page's 16 KB of K codes + 1) below 2^24: a page of 64 heads of 64 and 128 tokens has 32."""
+    assert order(B=((1 << 24) - 1) // 65 + 1, W=1, KV=64, page=128) == -1
