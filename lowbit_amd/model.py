@@ -336,7 +336,9 @@ class KV8Cache:
         return n
 
     def resize(self, pages: int):
-        """A pool of `pages` pages; where it shrinks the pages in use are compacted first and have to fit."""
+        """A pool of `pages` pages; where it shrinks the pages in use are compacted first and have to fit. One
+        buffer of a layer at a time, so that there is room for little more than the larger of the two pools; if
+        there is not, what is in use stays, in a pool of the fewer pages."""
         if pages <= 0 or pages < np.count_nonzero(self._refs):
             raise ValueError(f"{np.count_nonzero(self._refs)} pages are in use")
         if pages < self.pages:
@@ -344,16 +346,25 @@ class KV8Cache:
         else:
             self.upload()
         _check(K.lib().lb_dev_synchronize(), "synchronize")
-        keep, old = min(pages, self.pages), [b for _, b in self.layers]
-        fresh = [self._new_layer(pages) for _ in old]
-        for a, b in zip(old, fresh):
-            for x, y, n in zip(a, b, 2 * [keep * self._kv * self.page * self._d] + 2 * [keep * self._kv]):
-                _check(K.lib().lb_memcpy_d2d(y.ptr, x.ptr, n), "pool copy")
+        keep, buffers = min(int(pages), self.pages), [b for _, b in self.layers]
+        code, self.pages = self._kv * self.page * self._d, keep
+        try:
+            for b in buffers:
+                for i, of_page in enumerate((code, code, self._kv, self._kv)):
+                    b[i] = self._resized(b[i], keep * of_page, int(pages) * of_page)
+            self.pages = int(pages)
+        finally:
+            self._set_layers(buffers)
+            self._refs = np.concatenate([self._refs[:keep], np.zeros(self.pages - keep, np.int64)])
+            self._free = [int(p) for p in np.flatnonzero(self._refs == 0)[::-1]]
+
+    @staticmethod
+    def _resized(old, keep: int, nbytes: int):
+        """A buffer of nbytes that begins as `old` does."""
+        new = _buf(nbytes)
+        _check(K.lib().lb_memcpy_d2d(new.ptr, old.ptr, keep), "pool copy")
         _check(K.lib().lb_dev_synchronize(), "synchronize")
-        self.pages = int(pages)
-        self._set_layers(fresh)
-        self._refs = np.concatenate([self._refs[:keep], np.zeros(pages - keep, np.int64)])
-        self._free = [int(p) for p in np.flatnonzero(self._refs == 0)[::-1]]
+        return new
 
     def _copy(self, pairs: list, stream):
         """Pages copied in every layer, on `stream`."""

@@ -265,3 +265,55 @@ def test_many_copies_in_several_calls(new, monkeypatch):
 
     cache._copy(Pairs(), None)
     assert calls[1:] == [1 << 24, 1 << 24, 3]
+
+
+class Counted(Buffer):
+    """A stand-in whose bytes are counted while it lives."""
+    live, peak, room = 0, 0, 1 << 60
+
+    def __init__(self, nbytes):
+        if Counted.live + nbytes > Counted.room:
+            self.nbytes = 0
+            raise MemoryError
+        super().__init__(nbytes)
+        Counted.live += nbytes
+        Counted.peak = max(Counted.peak, Counted.live)
+
+    def __del__(self):
+        Counted.live -= self.nbytes
+
+
+def test_resize_does_not_need_two_pools(new, monkeypatch):
+    """Peak: the larger pool and one buffer. Where even that is too much the cache is a whole one of the fewer
+    pages, with what it held."""
+    monkeypatch.setattr(M, "_buf", Counted)
+    Counted.live, Counted.room = 0, 1 << 60
+    cache = new(3200, page=16, pages=200)
+    layers, code, exps = len(cache.layers), cache._kv * 16 * cache._d, cache._kv
+    rest = Counted.live - layers * 200 * 2 * (code + exps)
+    size = lambda pages: rest + layers * pages * 2 * (code + exps)  # noqa: E731
+    write(cache, 0, list(range(100)))
+    whole = lambda: [[b.nbytes for b in x] for _, x in cache.layers]  # noqa: E731
+    for pages in (50, 170, 170, 169):
+        top = max(size(cache.pages), size(pages))
+        Counted.peak = 0
+        cache.resize(pages)
+        assert Counted.live == size(pages) == size(cache.pages) and Counted.peak <= top + pages * code
+        assert whole() == [[pages * code] * 2 + [pages * exps] * 2] * layers
+        assert read(cache, 0) == list(range(100)) and len(cache._free) == pages - 7
+    for pages, room, left in ((300, size(240), 169), (20, size(169) + 10 * code, 20)):
+        Counted.room = room
+        with pytest.raises(MemoryError):
+            cache.resize(pages)
+        Counted.room = 1 << 60
+        assert cache.pages == left and len(cache._refs) == left and all(p.pages == left for p in cache.pools)
+        assert all(n >= left * m for b in whole() for n, m in zip(b, (code, code, exps, exps)))
+        consistent(cache)
+        assert read(cache, 0) == list(range(100))
+    write(cache, 0, list(range(100, 320)))
+    with pytest.raises(ValueError):
+        write(cache, 0, [1])
+    cache.resize(40)
+    assert Counted.live == size(40)
+    write(cache, 0, [320])
+    assert read(cache, 0) == list(range(321))
