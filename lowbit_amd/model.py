@@ -295,6 +295,7 @@ class KV8Cache:
     def fork(self, dst: int, src: int):
         """Sequence `dst` becomes what `src` is (what it held returns to the pool): it shares its pages, none
         is copied until one of them writes to it."""
+        dst, src = (range(len(self.lengths))[i] for i in (dst, src))  # negative ones count from the end
         if dst == src:
             raise ValueError("a sequence cannot be forked onto itself")
         self.commit(dst, 0)

@@ -317,3 +317,22 @@ def test_resize_does_not_need_two_pools(new, monkeypatch):
     assert Counted.live == size(40)
     write(cache, 0, [320])
     assert read(cache, 0) == list(range(321))
+
+
+def test_fork_by_negative_and_wrong_indexes(new):
+    """A sequence named in two ways is one sequence; a source that is none leaves the destination as it is."""
+    cache = new(64, page=16, sequences=3, pages=9)
+    write(cache, 0, list(range(20)))
+    write(cache, 2, [7] * 5)
+    for dst, src in ((2, -1), (-1, 2), (0, -3)):
+        with pytest.raises(ValueError):
+            cache.fork(dst, src)
+    for dst, src in ((2, 3), (2, -4), (3, 0), (-4, 0)):
+        with pytest.raises(IndexError):
+            cache.fork(dst, src)
+    assert read(cache, 0) == list(range(20)) and read(cache, 2) == [7] * 5
+    cache.fork(-2, -3)
+    assert read(cache, 1) == list(range(20))
+    write(cache, 1, [9])
+    assert read(cache, 0) == list(range(20)) and read(cache, 1)[-1] == 9
+    consistent(cache)
