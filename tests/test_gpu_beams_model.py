@@ -251,3 +251,43 @@ def test_a_window_generates():
         model.new_cache(50, kv="fp32")
     wide = model_of(window=400)
     assert wide.generate(prompt, 20) == model_of().generate(prompt, 20, model_of().new_cache(100, kv="e4m3"))
+
+
+class Calls:
+    """The library with its calls counted."""
+
+    def __init__(self, lib):
+        self.lib, self.n = lib, {}
+
+    def __getattr__(self, name):
+        self.n[name] = self.n.get(name, 0) + 1
+        return getattr(self.lib, name)
+
+
+@pytest.mark.parametrize("seed,chunks", [(4, 1), (5, 2)])
+@pytest.mark.parametrize("graph", [True, False])
+def test_all_beams_ended(seed, chunks, graph):
+    """The search stops at the first look, every 32 steps behind the first two, that finds all beams ended, with
+    the history up to there: tokens and sums are the host-driven search's. The end token is likely by a channel
+    that all embeddings share."""
+    eos, n_new, W = 11, 150, 4
+    cfg = M.tiny_config(max_position=500, tie_word_embeddings=False)
+    weights = M.random_weights(cfg, seed=seed)
+    embed, head = weights["model.embed_tokens.weight"], weights["lm_head.weight"]
+    embed[:, 0], head[eos] = 3, 0
+    head[eos, 0] = 0.6
+    head *= 0.3
+    model = M.Model(cfg, weights, "w4a16", max_tokens=8)
+    prompts = [list(np.random.default_rng(n).integers(0, 97, n)) for n in (9, 14)]
+    cache = model.new_cache(14 + n_new, "e4m3", 2 * W, 16)
+    model.L = Calls(model.L)
+    got = model.generate_beams(prompts, n_new, W, eos=eos, length_penalty=0.0, cache=cache, graph=graph)
+    calls, model.L = model.L.n, model.L.lib
+    if graph:
+        assert calls["lb_graph_launch"] == 16 * chunks
+    else:
+        assert calls["lbd_beam_select"] == 2 + 32 * chunks
+    assert not cache.lengths.any() and len(cache._free) == cache.pages
+    assert all(t.index(eos) == len(t) - 1 for g in got for t, _ in g)
+    assert 32 * (chunks - 1) + 2 < max(len(t) for g in got for t, _ in g) <= 32 * chunks + 2
+    same(got, by_hand(model, prompts, n_new, W, eos, 16), n_new)
