@@ -168,6 +168,13 @@ class KVCache:
         self.fused_merge = slices <= 8 and cfg.num_heads * cfg.head_dim <= 2048
 
 
+def _pages_at(n, page: int, cfg):
+    """Pages that a sequence of n tokens (an array) holds while its next one is written: with a window those that it
+    sees. `cfg`: what has `window` and `sinks`."""
+    first, last = -(-cfg.sinks // page), n // page + 1
+    return last - (np.maximum(np.maximum(n - cfg.window + 1, 0) // page - first, 0) if cfg.window else 0)
+
+
 class KV8Cache:
     """K and V of one or more sequences in pages of a shared pool, 8 bits an element (E4M3
     codes, an E8M0 exponent for each page and KV head; lbd_kv8_* of include/lowbit_hip.h):
@@ -768,11 +775,12 @@ class Model:
         n_new - 1 decode forwards. The argmax runs on the device and feeds the next
         step's embedding lookup; the decode steps replay one recorded HIP graph
         (graph=False launches them one by one). timings["decode_s"] includes the
-        recording of the graph."""
+        recording of the graph. With a window the steps take what pages the pool has, and
+        where these run out those behind the window go back to it."""
         prompt = self._tokens(prompt)
         T = len(prompt)
         steps = max(0, n_new - 1)
-        cache = cache or self.new_cache(T + n_new)
+        cache = cache or self._window_cache([T], T + n_new) or self.new_cache(T + n_new)
         start = cache.length
         if start + T + steps > cache.capacity:
             raise ValueError(f"KV cache full ({start}+{T}+{steps} > {cache.capacity})")
@@ -783,8 +791,12 @@ class Model:
         self.hist = _buf(4 * (cache.capacity + 1))
         L = self.L
         self._sync()
-        if isinstance(cache, KV8Cache):  # the whole answer's pages, so that the recorded step never changes
-            cache.reserve(0, start + T + steps)
+        if isinstance(cache, KV8Cache):  # the whole answer's pages where there is no window
+            if cache.window and steps:
+                need = int(_pages_at(np.arange(start + T, start + T + steps), cache.page, cache).max())
+                if need > len(cache._free) + np.count_nonzero(cache._table[0] >= 0):
+                    raise ValueError(f"KV cache full (a window of {need} pages)")
+            cache.reserve(0, start + T + (0 if cache.window else steps))
             cache.upload(self.stream)
             self._plan_kv8(cache, T)
         _check(L.lb_memcpy_h2d(self.tok.ptr, prompt.ctypes.data, 4 * T), "token upload")
@@ -805,15 +817,17 @@ class Model:
             finally:
                 _check(L.lb_stream_end_capture(s, C.byref(ex)), "end capture")
             try:
-                for _ in range(steps):
-                    _check(L.lb_graph_launch(ex.value, s), "graph launch")
-                self._sync()
+                for n in self._runs(cache, start + T, steps):
+                    for _ in range(n):
+                        _check(L.lb_graph_launch(ex.value, s), "graph launch")
+                    self._sync()
             finally:
                 L.lb_graph_destroy(ex.value)
         else:
-            for _ in range(steps):
-                self._step(1, cache, "last", argmax_hist=True)
-            self._sync()
+            for n in self._runs(cache, start + T, steps):
+                for _ in range(n):
+                    self._step(1, cache, "last", argmax_hist=True)
+                self._sync()
         t2 = time.perf_counter()
         self._set_length(cache, start + T + steps)
         out = self.hist.to_array((cache.capacity + 1,), np.int32)[start + T:start + T + n_new]
@@ -822,6 +836,31 @@ class Model:
             timings["decode_s"] = t2 - t1
             timings["decode_forwards"] = steps
         return [int(v) for v in out]
+
+    def _runs(self, cache, at: int, steps: int):
+        """`steps` steps of a one-sequence cache from position `at` on in runs for which it has pages: the device
+        is idle between them, when pages behind a window go back and the next ones are taken."""
+        end = at + steps
+        while at < end:
+            n = end - at
+            if isinstance(cache, KV8Cache) and cache.window:
+                cache.commit(0, at)
+                cache.slide(0)
+                n = min(end, (int(cache._held[0]) + len(cache._free)) * cache.page) - at
+                cache.reserve(0, at + n)
+                cache.upload(self.stream)
+            yield n
+            at += n
+
+    def _window_cache(self, prompts: list, capacity: int) -> "KV8Cache | None":
+        """With a window, a cache for prompts of these lengths whose pool holds them and then their answers' windows
+        (with eight pages more each, so that pages seldom run out)."""
+        if not self.cfg.window:
+            return None
+        page = 32
+        most = int(_pages_at(np.arange(capacity), page, self.cfg).max()) + 8
+        pages = sum(min(-(-capacity // page), max(-(-n // page), most)) for n in prompts)
+        return self.new_cache(capacity, "e4m3", len(prompts), page, pages)
 
     # ------------------------------------------------------------ several sequences
 
@@ -889,7 +928,9 @@ class Model:
         if n_new <= 0:
             return [[] for _ in prompts]
         if cache is None:
-            cache = self.new_cache(max(len(p) for p in prompts) + n_new, kv="e4m3", sequences=len(prompts))
+            lengths = [len(p) for p in prompts]
+            cache = self._window_cache(lengths, max(lengths) + n_new) or self.new_cache(
+                max(lengths) + n_new, kv="e4m3", sequences=len(prompts))
         out = [[] for _ in prompts]
         y = self.forward_batch(list(prompts), cache)
         for i in range(n_new):

@@ -291,3 +291,35 @@ def test_all_beams_ended(seed, chunks, graph):
     assert all(t.index(eos) == len(t) - 1 for g in got for t, _ in g)
     assert 32 * (chunks - 1) + 2 < max(len(t) for g in got for t, _ in g) <= 32 * chunks + 2
     same(got, by_hand(model, prompts, n_new, W, eos, 16), n_new)
+
+
+@pytest.mark.parametrize("window,sinks,page", [(20, 4, 16), (33, 0, 16), (1, 20, 32), (70, 33, 32)])
+@pytest.mark.parametrize("graph", [True, False])
+def test_a_window_generates_in_few_pages(window, sinks, page, graph):
+    """A pool of no more than the prompt's or a window's pages serves an answer of any length, with the tokens of
+    a large one; one of a page less is refused before anything is read."""
+    model = model_of(window=window, sinks=sinks)
+    rng = np.random.default_rng(2)
+    head, prompt, n = list(rng.integers(0, 97, 13)), list(rng.integers(0, 97, 37)), 330
+    want = model.generate(head + prompt, n, model.new_cache(400, page=page))
+    seen = lambda p: {j for x in range(p + 1) if p - x < window or x < sinks for j in [x // page]}  # noqa: E731
+    need = max(-(-50 // page), max(len(seen(p)) for p in range(50, 50 + n - 1)))
+    for extra in (0, 1, 3):
+        cache = model.new_cache(400, page=page, pages=need + extra)
+        model.forward(head, cache)
+        assert model.generate(prompt, n, cache, graph=graph) == want
+        assert cache.length == 50 + n - 1
+        held = cache._table[cache._table >= 0]
+        assert np.array_equal(np.bincount(held, minlength=cache.pages), cache._refs)
+        assert len(cache._free) == cache.pages - len(held)
+    # and goes on: the next pass sees what a large cache's would
+    large = model.new_cache(400, page=page)
+    model.generate(head + prompt, n, large)
+    assert np.array_equal(model.forward(want[-1:], cache), model.forward(want[-1:], large))
+    small = model.new_cache(400, page=page, pages=need - 1)
+    model.forward(head, small)
+    with pytest.raises(ValueError):
+        model.generate(prompt, n, small, graph=graph)
+    assert small.length == 13
+    assert model.generate(head + prompt, n, graph=graph) == want
+    assert model.generate_batch([head + prompt, prompt], 60)[0] == want[:60]
