@@ -405,6 +405,54 @@ class KV8Cache:
         if need > self.work.nbytes:
             self.work = _buf(need)
 
+    def beam_pages(self, seq: int, end: int, steps: int, beams: int) -> np.ndarray:
+        """Pages that beams behind the first `end` tokens of sequence `seq` take beyond those it holds: with a window
+        at each of their steps, for the next two, less what the sequence has given back by then."""
+        last, full = -(-(end + steps) // self.page), end // self.page
+        j = np.arange(max(last, int(self._held[seq])))
+        held = (j < self._held[seq]) & (self._table[seq, :len(j)] >= 0)
+        alone = held & (self._refs[np.where(held, self._table[seq, :len(j)], 0)] == 1)
+        upto = lambda x: np.concatenate([[0], np.cumsum(x)])  # noqa: E731
+        takes, alone = upto(np.where(j < full, 1, beams) - held), upto(alone)
+        if not self.window:
+            return takes[[last]]
+        at = end + np.arange(max(steps, 1))
+        b = np.maximum(at - self.window + 1, 0) // self.page  # pages in sight: those of the sinks, and b .. to - 1
+        a, to = np.minimum(-(-self.sinks // self.page), b), -(-np.minimum(at + 2, end + steps) // self.page)
+        return takes[a] + takes[to] - takes[b] - (alone[b] - alone[a])
+
+    def beam_room(self, beams: int, steps: int, first: int) -> tuple:
+        """Pages for the next tokens of `beams` places a prompt, those without a sequence among them where one has
+        one: (the steps that they suffice for, all of them without a window, else a number as odd as `first` where
+        it is not all; [sequences, max_pages] each place's own pages from the one in writing on, else -1)."""
+        live, held = self.lengths > 0, self._held
+        length = np.repeat(self.lengths.reshape(-1, beams).max(1), beams)  # (one within a prompt)
+        tail = length // self.page
+
+        def last(n):
+            return np.where(length > 0, -(-(length + n) // self.page), 0)
+
+        def takes(n):
+            return int(np.maximum(last(n) - np.where(live, held, tail), 0).sum())
+
+        n = steps
+        if self.window and takes(n) > len(self._free):
+            n = 0
+            for bit in range(steps.bit_length() - 1, -1, -1):
+                if n + (1 << bit) < steps and takes(n + (1 << bit)) <= len(self._free):
+                    n += 1 << bit
+            n -= n % 2 != first
+        if takes(n) > len(self._free) or (steps and n <= 0):
+            raise ValueError("KV cache full")
+        own, to = np.full(self._table.shape, -1, np.int32), last(n)
+        for i in np.flatnonzero(length):
+            if live[i]:
+                self.reserve(i, int(length[i]) + n)
+                own[i, tail[i]:to[i]] = self._table[i, tail[i]:to[i]]
+            else:
+                own[i, tail[i]:to[i]] = [self._take() for _ in range(tail[i], to[i])]
+        return n, own
+
     def adopt(self, table: np.ndarray, lengths: np.ndarray):
         """The sequences become those of a page table and their lengths (negative: none): every page belongs
         to the sequences that name it, the others are free."""
@@ -956,7 +1004,9 @@ class Model:
 
         The search stays on the device: selection, the page tables' new order and the next token's embedding
         read each other's results, and the steps replay one recorded HIP graph of two (graph=False launches
-        them one by one). With eos the host looks every 32 steps whether all beams have ended."""
+        them one by one). With eos the host looks every 32 steps whether all beams have ended. With a window the
+        steps take what pages the pool has, and where these run out the host gives back those behind the window
+        (an error after that leaves the sequences empty, one before it the prompts)."""
         cfg = self.cfg
         G, W, V, eos = len(prompts), int(beams), cfg.vocab_size, int(eos)
         if not G or not all(len(p) for p in prompts):
@@ -971,44 +1021,41 @@ class Model:
         if cache is None:
             longest, page = max(len(p) for p in prompts) + steps, 16
             own = -(-steps // page) + 1  # pages that a beam may write
+            if cfg.window:  # those in sight, and eight, so that pages seldom run out
+                own = min(own, -(-(cfg.window + 1) // page) + 1 + -(-cfg.sinks // page) + 8)
             cache = self.new_cache(longest, "e4m3", n, page, sum(-(-len(p) // page) for p in prompts) + n * own)
         if not isinstance(cache, KV8Cache) or len(cache.lengths) != n:
             raise ValueError(f"the cache must be a KV8Cache of {n} sequences")
         firsts = np.arange(0, n, W)
         if np.delete(cache.lengths, firsts).any():
             raise ValueError("only the first sequence of each prompt may hold tokens")
-        need = 0
+        read, search = 0, 0
         for g, p in zip(firsts, prompts):
             was, end = int(cache.lengths[g]), int(cache.lengths[g]) + len(p)
             if end + steps > cache.capacity:
                 raise ValueError(f"KV cache full ({was}+{len(p)}+{steps} > {cache.capacity})")
-            last = -(-(end + steps) // cache.page)  # every beam's pages from the one in writing on, the prompt's before
-            need += last - int(cache._held[g]) + (W - 1) * (last - end // cache.page)
-            need += bool(was % cache.page and cache._refs[cache._table[g, was // cache.page]] > 1)
+            copy = bool(was % cache.page and cache._refs[cache._table[g, was // cache.page]] > 1)
+            read += max(-(-end // cache.page) - int(cache._held[g]), 0) + copy
+            search = search + cache.beam_pages(g, end, steps, W) + copy
+        need = max(read, int(search.max()))
         if need > len(cache._free):
             raise ValueError(f"KV cache full ({need} pages for the beams, {len(cache._free)} left)")
         _, logits = self._pass([prompts[i // W] if i % W == 0 else [] for i in range(n)], cache)
-        hole = cache._hole[firsts].copy()
-        # every place's own pages, from the one that its prompt's next token goes to
-        own = np.full((n, cache.max_pages), -1, np.int32)
+        held = cache.lengths.copy()
         try:
-            for g in firsts:
-                cache.reserve(g, int(cache.lengths[g]) + steps)
-                tail, last = int(cache.lengths[g]) // cache.page, int(cache._held[g])
-                own[g, tail:last] = cache._table[g, tail:last]
-                for i in range(g + 1, g + W):
-                    own[i, tail:last] = [cache._take() for _ in range(tail, last)]
-            return self._search(logits, own, hole, cache, G, W, n_new, eos, length_penalty, graph)
+            return self._search(logits, cache, G, W, n_new, eos, length_penalty, graph)
         except BaseException:
-            cache.adopt(cache._table, cache.lengths)  # the prompts, as they were read
+            # the prompts, as they were read, or nothing where a window has given pages of theirs back
+            cache.adopt(cache._table, held if np.array_equal(cache.lengths, held) else 0 * held)
             raise
 
-    def _search(self, logits, own, hole, cache: KV8Cache, G: int, W: int, n_new: int, eos: int, length_penalty: float,
+    def _search(self, logits, cache: KV8Cache, G: int, W: int, n_new: int, eos: int, length_penalty: float,
                 graph: bool) -> list:
-        """generate_beams behind its prompts' pass: `logits` of their last tokens, the places' own pages, the
-        pages that a window had given back."""
+        """generate_beams behind its prompts' pass, `logits` of their last tokens."""
         cfg, L, s = self.cfg, self.L, self.stream
         n, V, steps, firsts = G * W, cfg.vocab_size, n_new - 1, np.arange(0, G * W, W)
+        hole = cache._hole[firsts].copy()  # what a window has given back of each prompt's beams
+        room, own = cache.beam_room(W, steps, 1)  # steps that there are pages for (odd: one, and then pairs)
         cache.upload(s)
         up, lengths = K.DeviceBuffer.from_array, np.where(np.arange(n) % W == 0, cache.lengths, -1).astype(np.int32)
         sums = np.where(np.arange(n) % W == 0, 0.0, -np.inf).astype(np.float32)
@@ -1039,11 +1086,27 @@ class Model:
             self._linear(self.lm_head, self.h.ptr, n, logits.ptr)
             select(x, 1)
 
+        def slide(x: int) -> int:
+            """Pages behind the window of state x's sequences go back; the steps that there are pages for now."""
+            self._sync()
+            cache.adopt(state[x]["table"].to_array((n, cache.max_pages), np.int32),
+                        state[x]["past"].to_array((n,), np.int32))
+            for i in np.flatnonzero(cache.lengths):
+                cache._hole[i] = hole[i // W]
+            for i in np.flatnonzero(cache.lengths):
+                cache.slide(i)
+                hole[i // W] = cache._hole[i]
+            room, own = cache.beam_room(W, left, 0)
+            past = np.where(cache.lengths > 0, cache.lengths, -1).astype(np.int32)
+            for buf, a in ((state[x]["past"], past), (state[x]["table"], cache._table), (mine, own)):
+                _check(L.lb_memcpy_h2d(buf.ptr, a.ctypes.data, a.nbytes), "state upload")
+            return room
+
         select(0, 0)
         x, left = 1, steps
         if left:  # the first step builds what later ones find (tile layouts), outside of any graph
             step(x)
-            x, left = 1 - x, left - 1
+            x, left, room = 1 - x, left - 1, room - 1
         ex = C.c_void_p()
         try:
             if graph and left >= 2:
@@ -1056,13 +1119,15 @@ class Model:
                     _check(L.lb_stream_end_capture(s, C.byref(ex)), "end capture")
             since = 0
             while left:
+                if not room:
+                    room = slide(x)
                 if ex.value and left >= 2:
                     _check(L.lb_graph_launch(ex.value, s), "graph launch")
                     took = 2
                 else:
                     step(x)
                     took, x = 1, 1 - x
-                left, since = left - took, since + took
+                left, room, since = left - took, room - took, since + took
                 if eos >= 0 and since >= 32 and left:
                     since = 0
                     self._sync()

@@ -323,3 +323,74 @@ def test_a_window_generates_in_few_pages(window, sinks, page, graph):
     assert small.length == 13
     assert model.generate(head + prompt, n, graph=graph) == want
     assert model.generate_batch([head + prompt, prompt], 60)[0] == want[:60]
+
+
+@pytest.mark.parametrize("window,sinks,page", [(20, 4, 16), (33, 0, 16), (1, 20, 32), (50, 33, 16)])
+@pytest.mark.parametrize("graph", [True, False])
+def test_a_window_searches_in_few_pages(window, sinks, page, graph):
+    """A pool of the prompts' pages and those in sight serves a search of any length, with the beams of a large
+    one and a sequence's earlier turns; smaller ones are refused before anything is read."""
+    model = model_of(window=window, sinks=sinks)
+    rng = np.random.default_rng(6)
+    head, prompts = list(rng.integers(0, 97, 45)), [list(rng.integers(0, 97, n)) for n in (3, 60)]
+    large = model.new_cache(360, "e4m3", 8, page)
+    model.forward_batch([head] + [[]] * 7, large)
+    want = model.generate_beams(prompts, 250, 4, length_penalty=0.0, cache=large)
+    same(want, by_hand(model, [head + prompts[0], prompts[1]], 250, 4, -1, page), 250)
+    small, taken = None, 0
+    for pages in range(5, 8 * -(-350 // page)):
+        cache = model.new_cache(360, "e4m3", 8, page, pages)
+        try:
+            model.forward_batch([head] + [[]] * 7, cache)
+            free = list(cache._free)
+            got = model.generate_beams(prompts, 250, 4, length_penalty=0.0, cache=cache, graph=graph)
+        except ValueError:
+            assert list(cache.lengths) in ([0] * 8, [45] + [0] * 7) and (not cache.lengths.any() or cache._free == free)
+            continue
+        taken += 1
+        assert got == want
+        assert list(cache.lengths) == [45 + 3 + 249] * 4 + [60 + 249] * 4
+        held = cache._table[cache._table >= 0]
+        assert np.array_equal(np.bincount(held, minlength=cache.pages), cache._refs)
+        assert sorted(cache._free) == list(np.flatnonzero(cache._refs == 0))
+        small = small or pages
+        if taken == 3:
+            break
+    in_sight = -(-(window + 1) // page) + 1 + -(-sinks // page)
+    assert small <= -(-48 // page) + -(-60 // page) + 8 * in_sight < 8 * 15
+    # and on from there: the next pass sees what a large cache's would
+    feed = [[t[-1]] for g in want for t, _ in g]
+    assert np.array_equal(model.forward_batch(feed, cache), model.forward_batch(feed, large))
+    assert model.generate_beams([head + prompts[0], prompts[1]], 250, 4, length_penalty=0.0, graph=graph) == want
+
+
+def test_a_search_in_few_pages_that_ends(monkeypatch):
+    """With end tokens, and with an error in the middle: the sequences are empty where pages of the prompt's have
+    been given back."""
+    model = model_of(seed=4, window=24, sinks=4)
+    prompts = [list(np.random.default_rng(n).integers(0, 97, n)) for n in (9, 14)]
+    free = model.generate_beams(prompts, 80, 4, length_penalty=0.0)
+    eos = free[0][0][0][40]
+    caches = [model.new_cache(120, "e4m3", 8, 16, pages) for pages in (None, 34)]
+    got = [model.generate_beams(prompts, 80, 4, eos=eos, length_penalty=0.0, cache=c) for c in caches]
+    assert got[0] == got[1] and any(len(t) < 80 for g in got[0] for t, _ in g)
+    for c in caches:
+        assert [bool(n) for n in c.lengths] == [t[-1] != eos for g in got[0] for t, _ in g]
+    cache, n, room = model.new_cache(300, "e4m3", 8, 16, 34), [0], M.KV8Cache.beam_room
+    model.forward_batch([prompts[1]] + [[]] * 7, cache)
+
+    def fails(self, *a):
+        n[0] += 1
+        if n[0] == 3:
+            raise KeyboardInterrupt
+        return room(self, *a)
+
+    monkeypatch.setattr(M.KV8Cache, "beam_room", fails)
+    with pytest.raises(KeyboardInterrupt):
+        model.generate_beams(prompts, 250, 4, length_penalty=0.0, cache=cache)
+    assert n[0] == 3 and not cache.lengths.any() and len(cache._free) == 34
+    n[0] = 2  # before the first step: the prompts, as they were read
+    model.forward_batch([prompts[1]] + [[]] * 7, cache)
+    with pytest.raises(KeyboardInterrupt):
+        model.generate_beams(prompts, 250, 4, length_penalty=0.0, cache=cache)
+    assert list(cache.lengths) == [23, 0, 0, 0, 14, 0, 0, 0]

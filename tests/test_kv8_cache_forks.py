@@ -5,6 +5,7 @@ import pytest
 
 from lowbit_amd import kernels as K
 from lowbit_amd import model as M
+from oracle import beams as B
 from test_kv8_cache import Buffer
 
 
@@ -336,3 +337,85 @@ def test_fork_by_negative_and_wrong_indexes(new):
     write(cache, 1, [9])
     assert read(cache, 0) == list(range(20)) and read(cache, 1)[-1] == 9
     consistent(cache)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 4), (1, 0), (40, 50), (33, 0), (17, 16)])
+@pytest.mark.parametrize("W,prompts,steps", [(1, [5], 60), (3, [37], 100), (4, [16, 3, 50], 70), (2, [90, 32], 1), (5, [7], 0)])
+def test_beams_in_as_many_pages_as_they_are_said_to_take(new, window, sinks, W, prompts, steps):
+    """A search's table work by hand, on a pool of exactly the pages that beam_pages asks for: sequences of random
+    parents, some ended, find their tokens again, and the pool never runs out."""
+    rng = np.random.default_rng(W + steps + window)
+    n, G = len(prompts) * W, len(prompts)
+    for turn in range(3):  # earlier turns in the first sequences, the last of them shared with another prompt's
+        cache = new(300, page=16, sequences=n, pages=400, window=window, sinks=sinks)
+        for g in range(G):
+            if turn == 1 or (turn == 2 and g == 0):
+                write(cache, g * W, list(range(1000, 1021 + 30 * g + 20 * (turn == 2))))
+            elif turn == 2:
+                cache.fork(g * W, 0)
+        ends = [int(cache.lengths[g * W]) + p for g, p in enumerate(prompts)]
+        copies = [bool(cache.lengths[g * W] % 16 and cache._refs[cache._table[g * W, cache.lengths[g * W] // 16]] > 1)
+                  for g in range(G)]
+        more = sum(cache.beam_pages(g * W, ends[g], steps, W) + copies[g] for g in range(G)).max()
+        read = sum(max(-(-ends[g] // 16) - int(cache._held[g * W]), 0) + copies[g] for g in range(G))
+        cache.resize(int(np.count_nonzero(cache._refs) + max(more, read)))
+        assert len(cache._free) == max(more, read)
+        want = [[] for _ in range(n)]
+        for g, p in enumerate(prompts):
+            tokens = list(range(10000 * (g + 1), 10000 * (g + 1) + p))
+            was = [cache.held[int(cache._table[g * W, x // 16])].get(x % 16) if cache._table[g * W, x // 16] >= 0 else None
+                   for x in range(int(cache.lengths[g * W]))]
+            want[g * W] = was + tokens
+        for g, p in enumerate(prompts):  # all prompts' pages at once, as in a pass
+            cache.reserve(g * W, ends[g])
+        cache.upload()
+        for g, p in enumerate(prompts):
+            at = ends[g] - p
+            for i, t in enumerate(want[g * W][at:]):
+                page, slot = int(cache._table[g * W, (at + i) // 16]), (at + i) % 16
+                cache.held[page] = {**(cache.held[page] if slot else {}), slot: t}
+            cache.commit(g * W, ends[g])
+        for g in range(G):
+            cache.slide(g * W)
+        hole = cache._hole[::W].copy()
+        room, own = cache.beam_room(W, steps, 1)
+        table, past, tick, left, rounds = cache._table.copy(), np.where(cache.lengths > 0, cache.lengths, -1), 0, steps, 0
+        parent, add = np.arange(n) // W * W, 0
+        while True:
+            done = (rng.random(n) < 0.02) | (past[parent] < 0)
+            past, table, moves = B.reorder(parent, done, past, table, own, W, add, 16, cache.pages)
+            for a, b, k in moves:
+                cache.held[b] = {s: v for s, v in cache.held[a].items() if s < k} | {
+                    s: v for s, v in cache.held[b].items() if s >= k}
+            want = [list(want[p]) if past[i] >= 0 else [] for i, p in enumerate(parent)]
+            for i in range(n):
+                for x in range(max(past[i], 0)):
+                    if not window or x < sinks or x > past[i] - window:
+                        assert cache.held[int(table[i, x // 16])].get(x % 16) == want[i][x]
+            if not left:
+                break
+            if not room:
+                rounds += 1
+                cache.adopt(table, past)
+                for i in np.flatnonzero(cache.lengths):
+                    cache._hole[i] = hole[i // W]
+                for i in np.flatnonzero(cache.lengths):
+                    cache.slide(i)
+                    hole[i // W] = cache._hole[i]
+                room, own = cache.beam_room(W, left, 0)
+                assert room == left or room % 2 == 0
+                table = cache._table.copy()
+            for i in np.flatnonzero(past >= 0):  # a step
+                page, slot = int(table[i, past[i] // 16]), past[i] % 16
+                assert page >= 0
+                cache.held[page] = {**(cache.held[page] if slot else {}), slot: tick}
+                want[i].append(tick)
+                tick += 1
+            left, room = left - 1, room - 1
+            parent, add = np.arange(n) // W * W + rng.integers(0, W, n), 1
+        assert not rounds if not window else rounds or turn or steps < 60 or sinks > 16 or window > 33 or W == 1
+        cache.adopt(table, past)
+        for i in np.flatnonzero(cache.lengths):
+            cache._hole[i] = hole[i // W]
+            cache.slide(i)
+        consistent(cache)
