@@ -186,11 +186,14 @@ hipError_t launch_kv8_copy_pages(const Kv8Layers &l, const int32_t *src, const i
 hipError_t launch_kv8_reorder(const Kv8Layers &l, const Kv8Order &o, bool write, hipStream_t s) {
   const int parts = copy_parts(l);
   const long long places = (long long)o.B * o.W, copies = 2 * places * parts, grid = copies + (write ? places : 0);
-  // Workgroups in all, so that a place's move is found for several layers where there are many. Pages of 128 KB:
-  // 40 places in 32 layers 13.6 us with four rows of workgroups, 13.2 with five, 14.0 with seven, 21.8 with one a
-  // layer; 128 places 70 with one row, 56 with two, 87 with one a layer. Of 8 KB, whose parts leave lanes idle:
-  // 32 places in 24 layers 5.1 us with 1024 in all, 6.2 with 2048.
-  const long long want = ((long long)l.KV << (l.page_shift + l.d_shift)) < kCopyBytes ? 1024 : 3200;
+  // Workgroups in all, so that a place's move is found for several layers where there are many: ten a compute unit.
+  // us a call at 1600, 2560, 3200 and 4096 of them (rows of workgroups), heads of 128, a page's K codes of
+  //   64 KB: 40 places in 32 layers 15.0 (5), 14.5 (8), 14.0 (10), 14.1 (13), and 38.7 with one row; 16 places 8.4
+  //          (13), 8.5 (20), 8.7 (25), 9.9 (32); 130 places 59.4 (2), 54.5 (3), 51.7 (4), 51.6 (4)
+  //   128 KB: 40 places in 32 layers 45.0 (3), 40.8 (4), 40.5 (5), 38.7 (7); 128 places 135 (1), 103 (2), 103 (2), 103 (2)
+  //   16 KB: 128 places in 28 layers 15.5 (7), 14.5 (10), 16.1 (13), 16.5 (16)
+  // Of 4 KB, whose parts leave lanes idle: 128 places in 24 layers 10.6 with 1024 in all, 11.2 with 2560; 32 places 6.2, 6.3.
+  const long long want = ((long long)l.KV << (l.page_shift + l.d_shift)) < kCopyBytes ? 1024 : 2560;
   const int rows = (int)std::min<long long>(l.n, std::max<long long>(1, (want + copies - 1) / copies));
   if (!fits(grid, rows)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kv8_reorder_kernel, dim3((unsigned)grid, rows), dim3(256), 0, s, l, o, (int)copies, parts, rows);
