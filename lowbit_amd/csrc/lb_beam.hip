@@ -122,9 +122,9 @@ __device__ __forceinline__ float beam_threshold(float v, int W) {
 // room. So most chunks end after a comparison of 16 logits' maximum. (128 rows of 151936: rising logits 26 us,
 // 367 without a threshold for them; all equal ones, where keys differ by their tokens only, 81.)
 //
-// What bounds it: 128 rows of 151936 logits the instructions, 17 us = 4.3 TB/s (of a wave's 530 vector
-// instructions 16 a chunk are exponentials and 48 their arguments and sum), and 2.4 steps a workgroup between its
-// beginning and end; four such rows the launch and two loads one after the other, 4 us. The threshold of a
+// What bounds it: 128 rows of 151936 logits the instructions, 17 us = 4.3 TB/s (of a wave's 549 vector
+// instructions 16 a chunk are exponentials and 48 their arguments and sum), and 2.85 steps a workgroup between its
+// beginning and end; four such rows the launch and two loads one after the other, 4.8 us. The threshold of a
 // wave's own first chunk kept four times as many keys (25.9 us), sixteen tests for room a chunk 20.8.
 __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs a, int per, int pieces,
                                                                        BeamPiece *__restrict__ piece,
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(kBeamWaves *kWave) void beam_piece_kernel(BeamArgs 
 // whom.
 //
 // What bounds it: three loads one after the other (sums and first offers, the chosen pieces' others, none of
-// them near) and as many barriers, 4.2 us for 4 beams, 4.8 for 16 prompts' 8, 14 for 32. Counted among all 152
+// them near) and as many barriers, 4.6 us for 4 beams, 5.3 for 16 prompts' 8, 14 for 32. Counted among all 152
 // first offers, not the few that reach the threshold, 6 us; all comparisons on 64-bit structures 20.
 // (by_w and by_pieces: 2^16 / W and 2^20 / pieces and a bit more, for divisions of less than 1024 and 512.)
 __global__ __launch_bounds__(kBeamHeads) void beam_merge_kernel(BeamArgs a, int pieces, uint32_t by_w, uint32_t by_pieces,

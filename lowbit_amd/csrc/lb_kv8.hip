@@ -552,7 +552,7 @@ struct Kv8Lds {
 // behind the sinks (positions come back in load_tiles and in the mask), and everything else is as
 // it is for a short sequence. What bounds it: 61 steps in windows of 4096 behind up to 30000, 32 heads on
 // 8 of 128, the bytes, 498 MB in 98 us and 5 for the merge (whole caches masked: 200 us); 2048 tokens in
-// 512 the instructions, 54 us: 18 chunks a row block, and a third of them in the waves' beginnings and
+// 512 the instructions, 55 us: 18 chunks a row block, and a third of them in the waves' beginnings and
 // ends (whole caches masked: 104). Tried for those: one wave a workgroup (15 to 20 % faster at windows of
 // 128 and 2000 row blocks, as much slower at 1024), eight (8 to 15 % faster at D = 64 and up to 256 row
 // blocks, 20 to 80 % slower else), and output stored straight from the matrix layout, 16 of a line's 128

@@ -16,8 +16,8 @@ constexpr long long kCopyGroups = 1ll << 32;  // workgroups of a call and 64 lay
 // ---------------------------------------------------------------- copies of pages
 
 // A workgroup a part of one page's K or V in one layer. What bounds it: the bytes; 250 pages of 128 KB in 16
-// layers, 524 MB read and written, 101 us = 5.2 TB/s, what a large copy reaches; 3 pages of 4 KB in 24 layers
-// the launch, 2.3 us.
+// layers, 524 MB read and written, 100 us = 5.2 TB/s, what a large copy reaches; 3 pages of 4 KB in 24 layers
+// the launch, 2.8 us.
 __global__ __launch_bounds__(256) void kv8_copy_kernel(Kv8Layers l, const int32_t *__restrict__ src,
                                                        const int32_t *__restrict__ dst, int parts) {
   const Kv8Codes c = l.of[blockIdx.y];
@@ -103,8 +103,8 @@ __device__ __forceinline__ Kv8Move kv8_move(const Kv8Order &o, const Kv8Family &
 
 // A workgroup takes one place's part of K or V in every `step`-th layer, so that it finds the place's move once
 // (four loads one after the other) for several copies. What bounds it: a few places those loads and the launch
-// (4 beams in 24 layers of 14 heads on 2 of 64 3.7 us); many the bytes: 8 prompts' 5 beams in 32 layers of 8 heads
-// of 128, 50 MB read and written, 13 us = 3.8 TB/s.
+// (4 beams in 24 layers of 14 heads on 2 of 64 4.4 us); many the bytes: 8 prompts' 5 beams in 32 layers of 8 heads
+// of 128, 50 MB read and written, 13.2 us = 3.8 TB/s.
 __global__ __launch_bounds__(256) void kv8_reorder_kernel(Kv8Layers l, Kv8Order o, int copies, int parts, int step) {
   const int tid = threadIdx.x, id = (int)blockIdx.x;
   if (id >= copies) {  // a place's row of the table
