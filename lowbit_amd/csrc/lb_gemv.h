@@ -1249,7 +1249,7 @@ static hipError_t launch_gemv_paced(const GemmArgs &a, int cus, size_t lds, hipS
 // both): otherwise the second waits for the first to finish, and one workgroup per
 // CU with twice the rows is faster (long rows: 9-16 % at 1 x 4096 x 11008 cold).
 // W4A8 quantizes the activation row in every workgroup, so below two rows per wave
-// it takes one workgroup per CU as well (3-9 % at N = 3072 .. 6144), and so does a
+// it takes one workgroup per CU as well (3-9 % up to N = 6144), and so does a
 // W4A8 GEMV with a prologue whose workgroups would get under 32 KB of weights.
 template <int F, int MB, int PRO>
 static hipError_t launch_gemv_mb(const GemmArgs &a, int num_cus, size_t lds, hipStream_t s, GemvPlan *plan) {
